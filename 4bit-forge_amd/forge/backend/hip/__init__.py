@@ -98,6 +98,13 @@ def _declare(lib: ctypes.CDLL) -> ctypes.CDLL:
         "forge_gather_scaled_rows": ([vp, i32, i64, i64, i64, vp, vp, vp, i64, vp], i32),
         "forge_rows_operands": ([vp, i32, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, vp], i32),
         "forge_rows_diagonal": ([vp, i32, vp, vp, vp, vp, i64, i64, vp], i32),
+        "forge_rms_norm": ([vp, i32, i64, vp, i64, vp, i32, i64, i64, f32, vp, vp, vp], i32),
+        "forge_rms_norm_fp8": ([vp, i32, i64, vp, i64, vp, i32, i64, i64, f32, vp, vp, vp, vp], i32),
+        "forge_gated_rows": ([vp, i64, vp, vp, vp, i64, i64, i64, i64, i64, i64, i32, vp, vp, vp, vp], i32),
+        "forge_gated_rows_backward": ([vp, vp, vp, vp, i64, vp, vp, vp, i64, i64, i64, i64, i64, i64, i32,
+                                       vp, vp, vp, vp, i64, vp], i32),
+        "forge_gated_rows_backward_workspace_bytes": ([i64, i64], i64),
+        "forge_linear_int4": ([vp, i64, vp, vp, i64, vp, vp, i64, i64, i64, i64, i32, vp, vp], i32),
     }
     for name, (args, res) in sigs.items():
         fn = getattr(lib, name)          # AttributeError here = library/header mismatch
@@ -131,7 +138,12 @@ EXPORTED_SYMBOLS = (
     "forge_rows_factor_blocked", "forge_rows_factor_workspace_bytes",
     "forge_gptq_sweep_rows_blocked", "forge_gptq_sweep_rows_workspace_bytes",
     "forge_rows_operands", "forge_rows_diagonal",
+    "forge_rms_norm", "forge_rms_norm_fp8", "forge_gated_rows", "forge_gated_rows_backward",
+    "forge_gated_rows_backward_workspace_bytes", "forge_linear_int4",
 )
+
+# FORGE_ACT_* of include/forge_hip.h
+ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "relu": 3}
 
 
 def load_library() -> ctypes.CDLL:
@@ -157,6 +169,28 @@ def _dtype_code(t: torch.Tensor) -> int:
     if t.dtype == torch.bfloat16:
         return FORGE_BF16
     raise RuntimeError(f"unsupported dtype {t.dtype} (float32 or bfloat16 expected)")
+
+
+def _act_code(activation) -> int:
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r} (one of {list(ACTIVATIONS)})")
+    return ACTIVATIONS[activation]
+
+
+def _unit_rows(t):
+    """A tensor whose rows the kernels can read as they are (unit column stride, rows that follow one
+    another without overlapping); anything else is copied."""
+    if t.stride(-1) == 1 and all(a >= b * n for a, b, n in
+                                 zip(t.stride()[:-1], t.stride()[1:], t.shape[1:])):
+        return t
+    return t.contiguous()
+
+
+def _need_one_device(*tensors):
+    _need_cuda(*tensors)
+    devs = {t.device for t in tensors if t is not None}
+    if len(devs) > 1:
+        raise RuntimeError(f"tensors on different devices: {sorted(map(str, devs))}")
 
 
 def _need_cuda(*tensors):
@@ -877,6 +911,110 @@ class _HipKernels:
                 _ptr(X), _dtype_code(X), X.stride(0), T, C, _ptr(row_idx), _ptr(weight), _ptr(out),
                 N, _stream()))
         return out
+
+    # -- the block around the solve (forge/engine.py checks the arguments) ----------------
+    def rms_norm(self, x, weight, eps, residual=None):
+        """x, residual [T,C] bf16/f32 (unit column stride), weight [C] -> y, residual out (None
+        without residual), both [T,C] of x's dtype."""
+        _need_one_device(x, weight, residual)
+        T, C = x.shape
+        assert x.stride(1) == 1 and weight.is_contiguous() and weight.numel() == C
+        assert residual is None or (residual.dtype == x.dtype and residual.shape == x.shape
+                                    and residual.stride(1) == 1)
+        y = torch.empty((T, C), dtype=x.dtype, device=x.device)
+        out = None if residual is None else torch.empty_like(y)
+        with torch.cuda.device(x.device):
+            self._check(self._lib.forge_rms_norm(
+                _ptr(x), _dtype_code(x), max(x.stride(0), C), _ptr(residual),
+                0 if residual is None else max(residual.stride(0), C), _ptr(weight), _dtype_code(weight), T, C,
+                float(eps), _ptr(y), _ptr(out), _stream()))
+        return y, out
+
+    def rms_norm_fp8(self, x, weight, eps, residual=None):
+        """The same with codes [T,C] float8_e4m3fn and scale_inv [T,ceil(C/128)] f32 in y's place."""
+        _need_one_device(x, weight, residual)
+        T, C = x.shape
+        assert x.stride(1) == 1 and weight.is_contiguous() and weight.numel() == C
+        assert residual is None or (residual.dtype == x.dtype and residual.shape == x.shape
+                                    and residual.stride(1) == 1)
+        codes = torch.empty((T, C), dtype=torch.float8_e4m3fn, device=x.device)
+        scale_inv = torch.empty((T, (C + 127) // 128), dtype=torch.float32, device=x.device)
+        out = None if residual is None else torch.empty((T, C), dtype=x.dtype, device=x.device)
+        with torch.cuda.device(x.device):
+            self._check(self._lib.forge_rms_norm_fp8(
+                _ptr(x), _dtype_code(x), max(x.stride(0), C), _ptr(residual),
+                0 if residual is None else max(residual.stride(0), C), _ptr(weight), _dtype_code(weight), T, C,
+                float(eps), _ptr(codes), _ptr(scale_inv), _ptr(out), _stream()))
+        return codes, scale_inv, out
+
+    def gated_rows(self, rows, offsets, w_gate, w_up, activation="silu", keep=False):
+        """rows [N,H] bf16 grouped by expert, offsets [E+1] int32 on the device, w_gate / w_up
+        [E,I,H] bf16 with equal strides -> h [N,I] bf16; keep: also g and u [N,I] f32, for
+        gated_rows_backward.  Allocates its results and nothing else; nothing waits for the GPU."""
+        _need_one_device(rows, offsets, w_gate, w_up)
+        E, I, H = w_gate.shape
+        N = rows.shape[0]
+        assert rows.dtype == w_gate.dtype == w_up.dtype == torch.bfloat16 and rows.shape[1] == H
+        assert offsets.dtype == torch.int32 and offsets.is_contiguous() and offsets.numel() == E + 1
+        assert rows.stride(1) == w_gate.stride(2) == 1 and w_gate.stride() == w_up.stride()
+        assert w_up.shape == w_gate.shape
+        h = torch.empty((N, I), dtype=torch.bfloat16, device=rows.device)
+        g = u = None
+        if keep:
+            g = torch.empty((N, I), dtype=torch.float32, device=rows.device)
+            u = torch.empty_like(g)
+        with torch.cuda.device(rows.device):
+            self._check(self._lib.forge_gated_rows(
+                _ptr(rows), max(rows.stride(0), H), _ptr(offsets), _ptr(w_gate), _ptr(w_up),
+                max(w_gate.stride(1), H), w_gate.stride(0), N, E, H, I, _act_code(activation), _ptr(h), _ptr(g),
+                _ptr(u), _stream()))
+        return (h, g, u) if keep else h
+
+    def gated_rows_backward(self, dh, g, u, rows, offsets, w_gate, w_up, activation="silu",
+                            need=(True, True, True)):
+        """Gradients of gated_rows for dh [N,I] bf16 contiguous: (d rows [N,H], d w_gate, d w_up
+        [E,I,H]) in bf16, None where `need` says so."""
+        _need_one_device(dh, g, u, rows, offsets, w_gate, w_up)
+        E, I, H = w_gate.shape
+        N = rows.shape[0]
+        assert dh.dtype == rows.dtype == w_gate.dtype == w_up.dtype == torch.bfloat16
+        assert tuple(dh.shape) == tuple(g.shape) == tuple(u.shape) == (N, I) and dh.is_contiguous()
+        assert g.dtype == u.dtype == torch.float32 and g.is_contiguous() and u.is_contiguous()
+        assert offsets.dtype == torch.int32 and offsets.is_contiguous() and offsets.numel() == E + 1
+        assert rows.stride(1) == w_gate.stride(2) == 1 and w_gate.stride() == w_up.stride()
+        dev = rows.device
+        dx = torch.empty((N, H), dtype=torch.bfloat16, device=dev) if need[0] else None
+        dwg = torch.empty((E, I, H), dtype=torch.bfloat16, device=dev) if need[1] else None
+        dwu = torch.empty((E, I, H), dtype=torch.bfloat16, device=dev) if need[2] else None
+        nbytes = int(self._lib.forge_gated_rows_backward_workspace_bytes(N, I))
+        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+        with torch.cuda.device(dev):
+            self._check(self._lib.forge_gated_rows_backward(
+                _ptr(dh), _ptr(g), _ptr(u), _ptr(rows), max(rows.stride(0), H), _ptr(offsets), _ptr(w_gate),
+                _ptr(w_up), max(w_gate.stride(1), H), w_gate.stride(0), N, E, H, I, _act_code(activation),
+                _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(ws), ws.numel(), _stream()))
+        return dx, dwg, dwu
+
+    def linear_int4(self, x, packed, scale, group_size, bias=None, activation=None, residual=None):
+        """x [M,C] bf16, packed [R,ceil(C/8)] int32, scale [R,G] f32 (pack_int4's words and its
+        groups' scales) -> act(x W^T + bias) + residual [M,R] bf16."""
+        _need_one_device(x, packed, scale, bias, residual)
+        M, C = x.shape
+        R = packed.shape[0]
+        assert x.dtype == torch.bfloat16 and x.stride(1) == 1
+        assert packed.dtype == torch.int32 and packed.is_contiguous() and packed.shape[1] == (C + 7) // 8
+        assert scale.dtype == torch.float32 and scale.is_contiguous()
+        assert tuple(scale.shape) == (R, (C + group_size - 1) // group_size)
+        assert bias is None or (bias.dtype == torch.bfloat16 and bias.is_contiguous() and bias.numel() == R)
+        assert residual is None or (residual.dtype == torch.bfloat16 and residual.stride(1) == 1
+                                    and tuple(residual.shape) == (M, R))
+        y = torch.empty((M, R), dtype=torch.bfloat16, device=x.device)
+        with torch.cuda.device(x.device):
+            self._check(self._lib.forge_linear_int4(
+                _ptr(x), max(x.stride(0), C), _ptr(packed), _ptr(scale), int(group_size), _ptr(bias),
+                _ptr(residual), 0 if residual is None else max(residual.stride(0), R), M, C, R,
+                _act_code(activation), _ptr(y), _stream()))
+        return y
 
 
 class _HipUnavailable(ModuleType):

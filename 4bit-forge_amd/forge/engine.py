@@ -1,13 +1,16 @@
 """Callers either side of the solve (forge/utils/engine.py, forge/utils/quant.py of the
 reference): the dequantised weight that is written back into the layer before the block is
-run again, and the routed-row gather in front of the per-expert Hessian update."""
+run again, the routed-row gather in front of the per-expert Hessian update, and the block's own
+arithmetic around both: the norm in front of the router (``rms_norm``, ``rms_norm_fp8``), the
+experts' gated rows that the down projection's Hessian takes (``expert_gated_rows``, with
+gradients) and the product with the packed result of the solve (``linear_int4``)."""
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Dict, Optional, Sequence, Tuple, Union
 
 import torch
 
-from forge.backend.hip import kernels
+from forge.backend.hip import kernels, _unit_rows, ACTIVATIONS
 
 
 @torch.no_grad()
@@ -56,3 +59,168 @@ def routed_rows(x: torch.Tensor, router_indices: torch.Tensor,
     x2 = x if x.stride(-1) == 1 else x.contiguous()
     rows = kernels.gather_scaled_rows(x2, tok[order].contiguous(), w)
     return rows, offsets
+
+
+def _no_gradient(name: str, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached "
+                           "tensors")
+
+
+def _norm_arguments(name, x, weight, eps, residual):
+    _no_gradient(name, x, weight, residual)
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"{name}: x is {x.dtype}, expected float32 or bfloat16")
+    if weight.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"{name}: weight is {weight.dtype}, expected float32 or bfloat16")
+    if x.dim() < 1 or x.shape[-1] == 0 or tuple(weight.shape) != (x.shape[-1],):
+        raise ValueError(f"{name}: weight {tuple(weight.shape)} does not fit rows of x {tuple(x.shape)}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError(f"{name}: residual {tuple(residual.shape)} {residual.dtype}, "
+                         f"x {tuple(x.shape)} {x.dtype}")
+    if not eps >= 0:
+        raise ValueError(f"{name}: eps={eps}")
+    C = x.shape[-1]
+    flat = lambda t: None if t is None else _unit_rows(t.reshape(-1, C))   # noqa: E731
+    return flat(x), weight.contiguous(), flat(residual)
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+             residual: Optional[torch.Tensor] = None):
+    """Root-mean-square norm over the last dimension of x [..., C] (bf16 or f32), the residual
+    added first:  s = x + residual,  y = s * rsqrt(mean(s^2) + eps) * weight.  Returns y, or
+    (y, s) with a residual (s is the residual stream for the next addition), in x's dtype.
+    Everything in f32 with one rounding at the end; the statistics come from the unrounded s.
+    weight [C] bf16 or f32.  New tensors; no backward pass (refused where one is asked for)."""
+    x2, w, r2 = _norm_arguments("rms_norm", x, weight, eps, residual)
+    y, out = kernels.rms_norm(x2, w, eps, r2)
+    return y.view(x.shape) if residual is None else (y.view(x.shape), out.view(x.shape))
+
+
+def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+                 residual: Optional[torch.Tensor] = None):
+    """rms_norm with y in 8 bits: (codes [..., C] float8_e4m3fn, scale_inv [..., ceil(C/128)] f32
+    [, s]), one scale = max(max |y|, 1e-12) / 448 per 128 columns, so that y = codes * scale_inv as
+    ``kernels.fp8_block_dequant`` reads block-scaled weights."""
+    x2, w, r2 = _norm_arguments("rms_norm_fp8", x, weight, eps, residual)
+    codes, scale_inv, out = kernels.rms_norm_fp8(x2, w, eps, r2)
+    codes, scale_inv = codes.view(x.shape), scale_inv.view(*x.shape[:-1], scale_inv.shape[1])
+    return (codes, scale_inv) if residual is None else (codes, scale_inv, out.view(x.shape))
+
+
+class _GatedRows(torch.autograd.Function):
+    """expert_gated_rows under autograd: keeps g and u in f32 (8 bytes per row and feature), which
+    costs less than forming them again (two of the backward pass's four products)."""
+
+    @staticmethod
+    def forward(ctx, rows, offsets, w_gate, w_up, activation):
+        h, g, u = kernels.gated_rows(rows, offsets, w_gate, w_up, activation, keep=True)
+        ctx.save_for_backward(rows, offsets, w_gate, w_up, g, u)
+        ctx.activation = activation
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        rows, offsets, w_gate, w_up, g, u = ctx.saved_tensors
+        need = (ctx.needs_input_grad[0], ctx.needs_input_grad[2], ctx.needs_input_grad[3])
+        dx, dwg, dwu = kernels.gated_rows_backward(dh.contiguous(), g, u, rows, offsets, w_gate, w_up,
+                                                   ctx.activation, need)
+        return dx, None, dwg, dwu, None
+
+
+def expert_gated_rows(rows: torch.Tensor, offsets: Union[torch.Tensor, Sequence[int], None],
+                      w_gate: torch.Tensor, w_up: torch.Tensor, activation: Optional[str] = "silu"
+                      ) -> torch.Tensor:
+    """The rows that reach each expert's down projection, for all experts at once:
+    h_i = act(w_gate[e] x_i) * (w_up[e] x_i) for the rows x_i of expert e, i.e. what
+    ``ExpertGroupGPTQ.update`` of the down projections takes.  rows [N, H] bf16 grouped by expert
+    and offsets [E + 1] as ``routed_rows`` returns them; offsets may also be an int32 or int64 tensor on
+    the rows' device, which is taken without looking at it on the host (ascending within [0, N] is
+    then the caller's duty; values outside are clamped).  w_gate, w_up [E, I, H] bf16, or [I, H]
+    for a dense layer (offsets None: all rows are its own).  Rows of no expert (before offsets[0],
+    from offsets[E] on) get 0.  activation: "silu", "gelu" (tanh form), "relu" or None.
+    Sums in f32, h [N, I] bf16 rounded once.
+
+    Differentiable in rows, w_gate and w_up (once); gradients are bf16, with dg and du rounded to
+    bf16 between the products.  A HIP graph of a training step captures ``kernels.gated_rows(...,
+    keep=True)`` and ``kernels.gated_rows_backward`` directly, not autograd's engine."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"expert_gated_rows: unknown activation {activation!r} (one of {list(ACTIVATIONS)})")
+    for n, t in (("rows", rows), ("w_gate", w_gate), ("w_up", w_up)):
+        if t.dtype != torch.bfloat16:
+            raise ValueError(f"expert_gated_rows: {n} is {t.dtype}, expected bfloat16")
+    if w_gate.shape != w_up.shape or w_gate.dim() not in (2, 3):
+        raise ValueError(f"expert_gated_rows: w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)}: "
+                         "expected one [E, I, H] or [I, H] for both")
+    if rows.dim() != 2 or rows.shape[1] != w_gate.shape[-1]:
+        raise ValueError(f"expert_gated_rows: rows {tuple(rows.shape)} do not fit weights {tuple(w_gate.shape)}")
+    if 0 in w_gate.shape:
+        raise ValueError(f"expert_gated_rows: empty weights {tuple(w_gate.shape)}")
+    if w_gate.dim() == 2:
+        w_gate, w_up = w_gate.unsqueeze(0), w_up.unsqueeze(0)
+    E, N = w_gate.shape[0], rows.shape[0]
+    if offsets is None:
+        if E != 1:
+            raise ValueError(f"expert_gated_rows: {E} experts need offsets")
+        offsets = [0, N]
+    if isinstance(offsets, torch.Tensor) and offsets.is_cuda:
+        if offsets.dtype not in (torch.int32, torch.int64) or tuple(offsets.shape) != (E + 1,):
+            raise ValueError(f"expert_gated_rows: offsets {tuple(offsets.shape)} {offsets.dtype}, expected "
+                             f"[{E + 1}] int32 or int64")
+        off = offsets.to(torch.int32).contiguous()
+    else:
+        off = [int(v) for v in offsets]
+        if len(off) != E + 1 or off[0] < 0 or off[-1] > N or any(a > b for a, b in zip(off, off[1:])):
+            raise ValueError(f"expert_gated_rows: offsets must be {E + 1} ascending numbers within "
+                             f"[0, {N}]")
+        off = torch.tensor(off, dtype=torch.int32).to(rows.device)
+    rows = _unit_rows(rows)
+    if w_gate.stride() != w_up.stride() or _unit_rows(w_gate) is not w_gate:
+        w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
+    if torch.is_grad_enabled() and (rows.requires_grad or w_gate.requires_grad or w_up.requires_grad):
+        return _GatedRows.apply(rows, off, w_gate, w_up, activation)
+    return kernels.gated_rows(rows, off, w_gate, w_up, activation)
+
+
+def linear_int4(x: torch.Tensor, packed: Dict[str, torch.Tensor], bias: Optional[torch.Tensor] = None,
+                activation: Optional[str] = None, residual: Optional[torch.Tensor] = None,
+                group_size: Optional[int] = None) -> torch.Tensor:
+    """A layer's product with its packed weights, as ``export.pack_weight`` returns them:
+    act(x W^T + bias) + residual with W[r, c] = (nibble - 8) * weight_scale[r, c / group_size] (the
+    zero points are in the nibbles).  x [..., C] bf16, bias [R] bf16, residual [..., R] bf16;
+    activation "silu", "gelu" (tanh form), "relu" or None; result [..., R] bf16, rounded once.
+    group_size may be left out when the groups divide C evenly (or there is one).  The weights stay
+    4 bits wide in memory; no layout of them is kept.  No backward pass (refused where one is asked
+    for)."""
+    w, scale = packed["weight_packed"], packed["weight_scale"]
+    _no_gradient("linear_int4", x, scale, bias, residual)
+    R, C = (int(v) for v in packed["weight_shape"])
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"linear_int4: unknown activation {activation!r} (one of {list(ACTIVATIONS)})")
+    if x.dtype != torch.bfloat16:
+        raise ValueError(f"linear_int4: x is {x.dtype}, expected bfloat16")
+    if x.dim() < 1 or x.shape[-1] != C:
+        raise ValueError(f"linear_int4: x {tuple(x.shape)} does not fit a weight of {R} x {C}")
+    if w.dtype != torch.int32 or tuple(w.shape) != (R, (C + 7) // 8):
+        raise ValueError(f"linear_int4: weight_packed {tuple(w.shape)} {w.dtype}, expected "
+                         f"[{R}, {(C + 7) // 8}] int32")
+    if scale.dim() != 2 or scale.shape[0] != R or not 1 <= scale.shape[1] <= C:
+        raise ValueError(f"linear_int4: weight_scale {tuple(scale.shape)}, expected [{R}, groups]")
+    G = scale.shape[1]
+    if group_size is None:
+        if C % G:
+            raise ValueError(f"linear_int4: {G} groups do not divide {C} columns evenly: pass group_size")
+        group_size = C // G
+    if group_size < 1 or (C + group_size - 1) // group_size != G:
+        raise ValueError(f"linear_int4: group_size={group_size} does not give {G} groups of {C} columns")
+    if bias is not None and (bias.dtype != torch.bfloat16 or tuple(bias.shape) != (R,)):
+        raise ValueError(f"linear_int4: bias {tuple(bias.shape)} {bias.dtype}, expected [{R}] bfloat16")
+    shape = (*x.shape[:-1], R)
+    if residual is not None and (residual.dtype != torch.bfloat16 or tuple(residual.shape) != shape):
+        raise ValueError(f"linear_int4: residual {tuple(residual.shape)} {residual.dtype}, expected "
+                         f"{shape} bfloat16")
+    y = kernels.linear_int4(_unit_rows(x.reshape(-1, C)), w.contiguous(), scale.float().contiguous(), group_size,
+                            None if bias is None else bias.contiguous(), activation,
+                            None if residual is None else _unit_rows(residual.reshape(-1, R)))
+    return y.view(shape)

@@ -31,6 +31,12 @@ extern "C" {
 #define FORGE_F32 0
 #define FORGE_BF16 1
 
+/* activations of forge_gated_rows and forge_linear_int4 (gelu: the tanh form) */
+#define FORGE_ACT_NONE 0
+#define FORGE_ACT_SILU 1
+#define FORGE_ACT_GELU 2
+#define FORGE_ACT_RELU 3
+
 typedef void* forge_stream_t;
 
 /* Library identification and error text. */
@@ -523,6 +529,65 @@ int forge_dequantize_groups(const uint8_t* q, const float* scales, const float* 
 int forge_gather_scaled_rows(const void* X, int x_dtype, int64_t ldx, int64_t T, int64_t C,
                              const int64_t* row_idx, const void* weight, void* out, int64_t N,
                              forge_stream_t stream);
+
+/* ------------------------------------------------------------------ the block around the solve */
+
+/* Root-mean-square norm with the residual's addition, no counterpart among the reference's own
+ * kernels (its block forward runs the model's modules, forge/utils/engine.py:100-130).  For each
+ * of T rows of C columns:  s = x + residual (f32),  y = s * rsqrt(mean(s^2) + eps) * weight,
+ * residual_out = s; y and residual_out are rounded once each, from f32, to x's dtype.
+ * x [T, C] with row pitch ldx, residual [T, C] with row pitch ldr (NULL: none; residual_out must
+ * then be NULL too), both of `dtype`; weight [C] of w_dtype; y and residual_out [T, C] contiguous.
+ * The statistics come from the unrounded f32 sum, not from residual_out.  No output may overlap an
+ * input or another output. */
+int forge_rms_norm(const void* x, int dtype, int64_t ldx, const void* residual, int64_t ldr,
+                   const void* weight, int w_dtype, int64_t T, int64_t C, float eps, void* y,
+                   void* residual_out, forge_stream_t stream);
+/* The same with y in 8 bits: per row and run of 128 columns (the last one may be shorter)
+ * scale_inv = max(max |y|, 1e-12) / 448 and codes = float8 e4m3fn nearest to y / scale_inv, y
+ * unrounded: the form forge_fp8_e4m3_block_dequant reads with so = 1, si = 128.  A NaN in a run
+ * makes its scale NaN.  codes [T, C] bytes, scale_inv [T, ceil(C/128)] f32, contiguous. */
+int forge_rms_norm_fp8(const void* x, int dtype, int64_t ldx, const void* residual, int64_t ldr,
+                       const void* weight, int w_dtype, int64_t T, int64_t C, float eps,
+                       uint8_t* codes, float* scale_inv, void* residual_out, forge_stream_t stream);
+
+/* Gated feed-forward rows of all experts in one launch: the gate and up projections, the
+ * activation and the product, i.e. the rows that reach the down projection (what the hooks of
+ * forge/utils/engine.py:210-256 see after the expert's own modules have run).
+ *   row i in [offsets[e], offsets[e+1]):  g = Wg[e] x_i, u = Wu[e] x_i, h_i = act(g) * u
+ * rows [N, H] bf16 with row pitch ldx, grouped by expert; offsets [E + 1] int32 on the DEVICE,
+ * ascending within [0, N] (values outside are clamped, so that no call reads or writes out of
+ * bounds); Wg, Wu [E, I, H] bf16 with row pitch ldw and expert stride w_stride (both the same for the two);
+ * h [N, I] bf16 contiguous.  Sums in f32, h rounded once.  Rows that belong to no expert (before
+ * offsets[0], from offsets[E] on) get h = 0.  gate_out, up_out (both or neither): g and u
+ * [N, I] f32, contiguous, for forge_gated_rows_backward (0 in rows of no expert). */
+int forge_gated_rows(const void* rows, int64_t ldx, const int32_t* offsets, const void* Wg,
+                     const void* Wu, int64_t ldw, int64_t w_stride, int64_t N, int64_t E, int64_t H,
+                     int64_t I, int act, void* h, float* gate_out, float* up_out,
+                     forge_stream_t stream);
+/* Its gradients: with dh [N, I] bf16 contiguous and g, u as forge_gated_rows left them,
+ *   dg = dh * u * act'(g), du = dh * act(g)           (f32, rounded to bf16 once, into ws)
+ *   drows = dg Wg + du Wu [N, H],  dWg[e] = dg_e^T x_e,  dWu[e] = du_e^T x_e [E, I, H]
+ * all bf16 contiguous, sums in f32; any of the three may be NULL.  Rows of no expert: drows = 0 (what
+ * dh holds there is not read into any gradient); experts without rows: dW = 0.  ws: device
+ * workspace of forge_gated_rows_backward_workspace_bytes(N, I), 16-byte aligned.  Results do not
+ * depend on the order in which workgroups run. */
+int forge_gated_rows_backward(const void* dh, const float* g, const float* u, const void* rows,
+                              int64_t ldx, const int32_t* offsets, const void* Wg, const void* Wu,
+                              int64_t ldw, int64_t w_stride, int64_t N, int64_t E, int64_t H,
+                              int64_t I, int act, void* drows, void* dWg, void* dWu, void* ws,
+                              int64_t ws_bytes, forge_stream_t stream);
+int64_t forge_gated_rows_backward_workspace_bytes(int64_t N, int64_t I);
+
+/* Product with forge_pack_int4's weights:  y = act(x W^T + bias) + residual,
+ * W[r][c] = (nibble c of row r - 8) * scale[r][c / gs]; the zero points are in the nibbles already.
+ * x [M, C] bf16 with row pitch ldx, packed [R, ceil(C/8)] int32, scale [R, ceil(C/gs)] f32, bias
+ * [R] bf16 (NULL: none), residual [M, R] bf16 with row pitch ldr (NULL: none), y [M, R] bf16
+ * contiguous.  The nibbles enter the products as integers (exact in bf16); every group's sum is
+ * formed in f32 and then multiplied by its f32 scale, and y is rounded once, after the epilogue. */
+int forge_linear_int4(const void* x, int64_t ldx, const int32_t* packed, const float* scale,
+                      int64_t gs, const void* bias, const void* residual, int64_t ldr, int64_t M,
+                      int64_t C, int64_t R, int act, void* y, forge_stream_t stream);
 
 #ifdef __cplusplus
 }
