@@ -7,6 +7,7 @@
 // Three products over one ragged batch.  All run on the bf16 matrix instruction with f32 sums.
 #include "act.h"
 #include "common.h"
+#include "mfma_tile.h"
 #include "ragged.h"
 
 namespace {
@@ -155,6 +156,162 @@ __global__ __launch_bounds__(256) void gated_any_kernel(GatedArgs a, int p_tiles
     }
 }
 
+// ---------------------------------------------------------------- 16-byte aligned rows
+// 256 x 256 outputs per workgroup (mfma_tile.h); roles of P and Q as above, with
+//   FORWARD   P = 128 features: tile rows 128 w .. + 63 are Wg's rows 64 w .., the next 64 Wu's, so
+//             that wavefront w of P holds g and u of the same features in the same lanes and the
+//             activation and the product need no exchange
+//   DROWS     P and Q of the gate, then of the up projection, into the same sums
+// The inner dimension's tail and rows or columns outside are zeros that the loads themselves write.
+// One barrier per stage: what a wavefront has waited for it publishes there, and everybody has then
+// finished reading the buffer that the loads issued next will overwrite.  The two buffers are
+// separate arrays and the loop is unrolled by two because the compiler otherwise has to assume that
+// a load on its way to LDS may hit what is being read, and waits for it.
+template <int MODE>
+__global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tiles, int q_tiles) {
+    using namespace forge;
+    __shared__ __attribute__((aligned(1024))) char P0[kStageBytes], Q0[kStageBytes], P1[kStageBytes], Q1[kStageBytes];
+    __shared__ int slot[4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wp = wave >> 2, wq = wave & 3;
+    int b = xcd_tile(blockIdx.x, gridDim.x);
+    const int pt = b % p_tiles;
+    b /= p_tiles;
+
+    RaggedTile r;
+    int q0 = 0, inner = 0, which = 0;
+    if constexpr (MODE == DWEIGHTS) {
+        q0 = (b % q_tiles) * kTile;
+        b /= q_tiles;
+        r.expert = b % a.E;
+        which = b / a.E;
+        r.row0 = clamp_offset(a.offsets, r.expert, 0, a.N);
+        r.rows = clamp_offset(a.offsets, r.expert + 1, r.row0, a.N) - r.row0;
+        inner = r.rows;
+    } else {
+        if (!find_tile(a.offsets, a.E, a.N, kTile, b, r, slot)) return;
+        inner = r.expert < 0 ? 0 : MODE == FORWARD ? a.H : a.I;
+    }
+    const int p0 = pt * (MODE == FORWARD ? kTile / 2 : kTile);
+    const int per_phase = (inner + kStage - 1) / kStage;
+    const int stages = MODE == DROWS ? 2 * per_phase : per_phase;
+    const int64_t we = (int64_t)(r.expert < 0 ? 0 : r.expert) * a.ws;
+
+    // loaders
+    InnerLoader lp_in, lq_in;
+    OuterLoader lp_out, lq_out;
+    __amdgpu_buffer_rsrc_t dp, dq;
+    if constexpr (MODE == FORWARD) {
+        const bool up = (wave & 3) >= 2;                       // this wavefront loads rows of Wu
+        const int rows = a.I - p0 < kTile / 2 ? a.I - p0 : kTile / 2;
+        lp_in.init(wave, lane, a.ldw, rows, [](int t) { return (t >> 7) * 64 + (t & 63); });
+        dp = descriptor((up ? a.wu : a.wg) + we + (int64_t)p0 * a.ldw, (uint32_t)(((rows - 1) * a.ldw + a.H) * 2));
+        lq_in.init(wave, lane, a.ldx, r.rows, [](int t) { return t; });
+        dq = descriptor(a.x + (int64_t)r.row0 * a.ldx, (uint32_t)(((r.rows - 1) * a.ldx + a.H) * 2));
+    } else if constexpr (MODE == DROWS) {
+        lp_out.init(wave, lane, a.ldw, a.H - p0);
+        lq_in.init(wave, lane, a.I, r.rows, [](int t) { return t; });
+    } else {
+        lp_out.init(wave, lane, a.ldx, a.H - p0);
+        lq_out.init(wave, lane, a.I, a.I - q0);
+    }
+    auto stage = [&](int s, char* P, char* Q) {
+        if constexpr (MODE == FORWARD) {
+            lp_in.stage(dp, P, wave, s * kStage, a.H);
+            lq_in.stage(dq, Q, wave, s * kStage, a.H);
+        } else if constexpr (MODE == DROWS) {
+            const bool up = s >= per_phase;
+            const int k0 = (up ? s - per_phase : s) * kStage;
+            lp_out.stage((up ? a.wu : a.wg) + we + (int64_t)k0 * a.ldw + p0, a.ldw, a.I - k0, a.H - p0, P, wave);
+            const __amdgpu_buffer_rsrc_t d = descriptor((up ? a.du : a.dg) + (int64_t)r.row0 * a.I, (uint32_t)(r.rows * a.I * 2));
+            lq_in.stage(d, Q, wave, k0, a.I);
+        } else {
+            const int64_t k0 = (int64_t)r.row0 + s * kStage;
+            lp_out.stage(a.x + k0 * a.ldx + p0, a.ldx, r.rows - s * kStage, a.H - p0, P, wave);
+            lq_out.stage((which ? a.du : a.dg) + k0 * a.I + q0, a.I, r.rows - s * kStage, a.I - q0, Q, wave);
+        }
+        // the compiler knows of no use of these loads before the next wait and would sink them there
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    InnerFragment fp_in, fq_in;
+    OuterFragment<4> fp_out;
+    OuterFragment<2> fq_out;
+    if constexpr (MODE == FORWARD) fp_in.init(lane, wp * 4); else fp_out.init(lane, wp * 4);
+    if constexpr (MODE == DWEIGHTS) fq_out.init(lane, wq * 2); else fq_in.init(lane, wq * 2);
+
+    f32x16_t acc[4][2];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) acc[t][n][v] = 0.0f;
+    auto multiply = [&](const char* P, const char* Q) {
+        if constexpr (MODE == FORWARD) multiply_stage(P, Q, fp_in, fq_in, acc);
+        else if constexpr (MODE == DROWS) multiply_stage(P, Q, fp_out, fq_in, acc);
+        else multiply_stage(P, Q, fp_out, fq_out, acc);
+    };
+    if (stages > 0) stage(0, P0, Q0);
+    // the loop's body has no way out in its middle: with one the accumulators change registers
+    int s = 0;
+    for (; s + 1 < stages; s += 2) {
+        wait_loads();
+        __syncthreads();
+        stage(s + 1, P1, Q1);
+        multiply(P0, Q0);
+        wait_loads();
+        __syncthreads();
+        if (s + 2 < stages) stage(s + 2, P0, Q0);
+        multiply(P1, Q1);
+    }
+    if (s < stages) {
+        wait_loads();
+        __syncthreads();
+        multiply(P0, Q0);
+    }
+    // registers 4 j .. 4 j + 3 of a tile: rows 8 j + 4 (lane / 32) .. + 3 of P, column lane & 31 of Q
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const int q = (wq * 2 + n) * 32 + (lane & 31);
+        if (MODE == DWEIGHTS ? q0 + q >= a.I : q >= r.rows) continue;
+        if constexpr (MODE == FORWARD) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int i = p0 + wp * 64 + t * 32 + 8 * j + 4 * (lane >> 5);
+                    if (i >= a.I) continue;
+                    const int64_t at = (int64_t)(r.row0 + q) * a.I + i;
+                    f32x4_t g, u;
+                    float h[4];
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                        g[v] = acc[t][n][4 * j + v];
+                        u[v] = acc[t + 2][n][4 * j + v];
+                        h[v] = act_f32(a.act, g[v]) * u[v];
+                    }
+                    *reinterpret_cast<uint2*>(a.h + at) = make_uint2(pack_bf16(h[0], h[1]), pack_bf16(h[2], h[3]));
+                    if (a.g) {
+                        *reinterpret_cast<f32x4_t*>(a.g + at) = g;
+                        *reinterpret_cast<f32x4_t*>(a.u + at) = u;
+                    }
+                }
+        } else {
+            uint16_t* out = MODE == DROWS ? a.dx + (int64_t)(r.row0 + q) * a.H
+                                          : (which ? a.dwu : a.dwg) + ((int64_t)r.expert * a.I + q0 + q) * a.H;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int c = p0 + (wp * 4 + t) * 32 + 8 * j + 4 * (lane >> 5);
+                    if (c >= a.H) continue;
+                    *reinterpret_cast<uint2*>(out + c) = make_uint2(pack_bf16(acc[t][n][4 * j], acc[t][n][4 * j + 1]),
+                                                                   pack_bf16(acc[t][n][4 * j + 2], acc[t][n][4 * j + 3]));
+                }
+        }
+    }
+}
+
 // dg and du from g, u and dh, rounded to bf16 once (they are operands of the two products);
 // one element per thread
 __global__ __launch_bounds__(256) void gated_grad_kernel(const uint16_t* __restrict__ dh,
@@ -169,6 +326,44 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(const uint16_t* __restr
     const float d = forge::bf16_bits_to_f32(dh[i]);
     dg[i] = f32_to_bf16_bits(d * u[i] * vd);
     du[i] = f32_to_bf16_bits(d * va);
+}
+
+// the same for runs of 8 (N * I a multiple of 8, 16-byte aligned): 14 bytes moved per element
+__global__ __launch_bounds__(256) void gated_grad8_kernel(const uint4* __restrict__ dh,
+                                                          const f32x4_t* __restrict__ g,
+                                                          const f32x4_t* __restrict__ u, uint4* __restrict__ dg,
+                                                          uint4* __restrict__ du, int64_t n8, int act) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n8) return;
+    const uint4 d4 = dh[i];
+    const f32x4_t gv[2] = {g[2 * i], g[2 * i + 1]}, uv[2] = {u[2 * i], u[2 * i + 1]};
+    const uint32_t dw[4] = {d4.x, d4.y, d4.z, d4.w};
+    uint32_t og[4], ou[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float x[2], y[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const float d = __uint_as_float(k ? dw[j] & 0xFFFF0000u : dw[j] << 16);
+            float va, vd;
+            act_grad_f32(act, gv[j / 2][2 * (j & 1) + k], va, vd);
+            x[k] = d * uv[j / 2][2 * (j & 1) + k] * vd;
+            y[k] = d * va;
+        }
+        og[j] = pack_bf16(x[0], x[1]);
+        ou[j] = pack_bf16(y[0], y[1]);
+    }
+    dg[i] = make_uint4(og[0], og[1], og[2], og[3]);
+    du[i] = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// what gated_tile_kernel takes: 16-byte pieces everywhere, row offsets of a tile within 31 bits
+bool tiles_fit(const GatedArgs& a) {
+    return a.H % 8 == 0 && a.I % 8 == 0 && a.ldx % 8 == 0 && a.ldw % 8 == 0 && (a.E == 1 || a.ws % 8 == 0) &&
+           a.ldx < (1 << 21) && a.ldw < (1 << 21) && a.I < (1 << 21) && aligned16(a.x) && aligned16(a.wg) &&
+           aligned16(a.wu);
 }
 
 int64_t grad_bytes(int64_t N, int64_t I) { return forge::ceil_div(2 * N * I, 256) * 256; }
@@ -204,9 +399,12 @@ extern "C" int forge_gated_rows(const void* rows, int64_t ldx, const int32_t* of
     a.h = (uint16_t*)h; a.g = gate_out; a.u = up_out;
     hipStream_t st = (hipStream_t)stream;
     forge::KernelTiming timing("gated_rows", st, 4.0 * N * H * I, forge::WORK_FLOPS);
-    const int64_t p_tiles = forge::ceil_div(I, 32), blocks = p_tiles * forge::ragged_tiles(N, E, 64);
+    const bool fast = tiles_fit(a) && aligned16(h) && aligned16(gate_out) && aligned16(up_out);
+    const int64_t p_tiles = forge::ceil_div(I, fast ? 128 : 32);
+    const int64_t blocks = p_tiles * forge::ragged_tiles(N, E, fast ? 256 : 64);
     FORGE_REQUIRE(blocks <= INT32_MAX, "forge_gated_rows: %lld workgroups", (long long)blocks);
-    gated_any_kernel<FORWARD><<<dim3((unsigned)blocks), 256, 0, st>>>(a, (int)p_tiles);
+    if (fast) gated_tile_kernel<FORWARD><<<dim3((unsigned)blocks), 512, 0, st>>>(a, (int)p_tiles, 1);
+    else gated_any_kernel<FORWARD><<<dim3((unsigned)blocks), 256, 0, st>>>(a, (int)p_tiles);
     FORGE_LAUNCH_CHECK();
     return FORGE_OK;
 }
@@ -236,26 +434,39 @@ extern "C" int forge_gated_rows_backward(const void* dh, const float* g, const f
     a.N = (int)N; a.E = (int)E; a.H = (int)H; a.I = (int)I; a.act = act;
     a.dg = dg; a.du = du;
     a.dx = (uint16_t*)drows; a.dwg = (uint16_t*)dWg; a.dwu = (uint16_t*)dWu;
-    const int64_t h_tiles = forge::ceil_div(H, 64), i_tiles = forge::ceil_div(I, 64);
-    const int64_t blocks = h_tiles * forge::ragged_tiles(N, E, 64);
-    FORGE_REQUIRE(blocks <= INT32_MAX && h_tiles * i_tiles <= INT32_MAX, "%s: too many workgroups", name);
+    const bool fast = tiles_fit(a) && aligned16(dh) && aligned16(g) && aligned16(u) && aligned16(drows) &&
+                      aligned16(dWg) && aligned16(dWu);
+    const int tile = fast ? 256 : 64;
+    const int64_t h_tiles = forge::ceil_div(H, tile), i_tiles = forge::ceil_div(I, tile);
+    const int64_t blocks = h_tiles * forge::ragged_tiles(N, E, tile);
+    FORGE_REQUIRE(blocks <= INT32_MAX && h_tiles * i_tiles * 2 * E <= INT32_MAX, "%s: too many workgroups", name);
     if (N > 0) {
         forge::KernelTiming timing("gated_grad", st, 14.0 * N * I, forge::WORK_BYTES);
-        gated_grad_kernel<<<dim3((unsigned)forge::ceil_div(N * I, 256)), 256, 0, st>>>(
-            (const uint16_t*)dh, g, u, dg, du, N * I, act);
+        if (fast)
+            gated_grad8_kernel<<<dim3((unsigned)forge::ceil_div(N * I / 8, 256)), 256, 0, st>>>(
+                (const uint4*)dh, (const f32x4_t*)g, (const f32x4_t*)u, (uint4*)dg, (uint4*)du, N * I / 8, act);
+        else
+            gated_grad_kernel<<<dim3((unsigned)forge::ceil_div(N * I, 256)), 256, 0, st>>>(
+                (const uint16_t*)dh, g, u, dg, du, N * I, act);
         FORGE_LAUNCH_CHECK();
     }
     if (drows && N > 0) {
         forge::KernelTiming timing("gated_drows", st, 4.0 * N * H * I, forge::WORK_FLOPS);
-        gated_any_kernel<DROWS><<<dim3((unsigned)blocks), 256, 0, st>>>(a, (int)h_tiles);
+        if (fast) gated_tile_kernel<DROWS><<<dim3((unsigned)blocks), 512, 0, st>>>(a, (int)h_tiles, 1);
+        else gated_any_kernel<DROWS><<<dim3((unsigned)blocks), 256, 0, st>>>(a, (int)h_tiles);
         FORGE_LAUNCH_CHECK();
     }
     if (dWg || dWu) {
         forge::KernelTiming timing("gated_dweights", st, 2.0 * N * H * I * ((dWg ? 1 : 0) + (dWu ? 1 : 0)), forge::WORK_FLOPS);
-        // blockIdx.z picks the gate (0) or the up weights (1); one alone is passed as both
+        // gate weights first, then up weights; one alone is passed as the first
+        const int both = dWg && dWu ? 2 : 1;
         if (!dWg) { a.dg = du; a.dwg = a.dwu; }
-        gated_any_kernel<DWEIGHTS><<<dim3((unsigned)(h_tiles * i_tiles), (unsigned)E, dWg && dWu ? 2u : 1u), 256, 0, st>>>(
-            a, (int)h_tiles);
+        if (fast)
+            gated_tile_kernel<DWEIGHTS><<<dim3((unsigned)(h_tiles * i_tiles * E * both)), 512, 0, st>>>(
+                a, (int)h_tiles, (int)i_tiles);
+        else
+            gated_any_kernel<DWEIGHTS><<<dim3((unsigned)(h_tiles * i_tiles), (unsigned)E, both), 256, 0, st>>>(
+                a, (int)h_tiles);
         FORGE_LAUNCH_CHECK();
     }
     return FORGE_OK;
