@@ -180,17 +180,23 @@ def _act_code(activation) -> int:
 def _unit_rows(t):
     """A tensor whose rows the kernels can read as they are (unit column stride, rows that follow one
     another without overlapping); anything else is copied."""
-    if t.stride(-1) == 1 and all(a >= b * n for a, b, n in
-                                 zip(t.stride()[:-1], t.stride()[1:], t.shape[1:])):
+    stride, shape = t.stride(), t.shape
+    if stride[-1] == 1:
+        for i in range(len(shape) - 1):
+            if stride[i] < stride[i + 1] * shape[i + 1]:
+                return t.contiguous()
         return t
     return t.contiguous()
 
 
-def _need_one_device(*tensors):
-    _need_cuda(*tensors)
-    devs = {t.device for t in tensors if t is not None}
-    if len(devs) > 1:
-        raise RuntimeError(f"tensors on different devices: {sorted(map(str, devs))}")
+def _need_one_device(first, *tensors):
+    """All on one GPU; returns it."""
+    dev = first.device
+    if dev.type != "cuda" or any(t is not None and t.device != dev for t in tensors):
+        _need_cuda(first, *tensors)
+        raise RuntimeError("tensors on different devices: "
+                           f"{sorted({str(t.device) for t in (first, *tensors) if t is not None})}")
+    return dev
 
 
 def _need_cuda(*tensors):
@@ -207,6 +213,18 @@ class _HipKernels:
         self._lib = lib
 
     def _check(self, rc: int):
+        if rc != 0:
+            raise RuntimeError(self._lib.forge_last_error().decode())
+
+    def _launch(self, dev, fn, *args):
+        """fn(*args, current stream of dev), with dev as the current device.  The operators that also
+        serve single tokens go through here: a device guard and a Stream object cost several times what
+        the launch does."""
+        if dev.index == torch.cuda.current_device():
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+        else:
+            with torch.cuda.device(dev):
+                rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
         if rc != 0:
             raise RuntimeError(self._lib.forge_last_error().decode())
 
@@ -916,104 +934,106 @@ class _HipKernels:
     def rms_norm(self, x, weight, eps, residual=None):
         """x, residual [T,C] bf16/f32 (unit column stride), weight [C] -> y, residual out (None
         without residual), both [T,C] of x's dtype."""
-        _need_one_device(x, weight, residual)
+        dev = _need_one_device(x, weight, residual)
         T, C = x.shape
+        ldx, ldr, rp, out, op = x.stride(0), 0, 0, None, 0
         assert x.stride(1) == 1 and weight.is_contiguous() and weight.numel() == C
-        assert residual is None or (residual.dtype == x.dtype and residual.shape == x.shape
-                                    and residual.stride(1) == 1)
-        y = torch.empty((T, C), dtype=x.dtype, device=x.device)
-        out = None if residual is None else torch.empty_like(y)
-        with torch.cuda.device(x.device):
-            self._check(self._lib.forge_rms_norm(
-                _ptr(x), _dtype_code(x), max(x.stride(0), C), _ptr(residual),
-                0 if residual is None else max(residual.stride(0), C), _ptr(weight), _dtype_code(weight), T, C,
-                float(eps), _ptr(y), _ptr(out), _stream()))
+        y = torch.empty((T, C), dtype=x.dtype, device=dev)
+        if residual is not None:
+            assert residual.dtype == x.dtype and residual.shape == x.shape and residual.stride(1) == 1
+            out = torch.empty((T, C), dtype=x.dtype, device=dev)
+            ldr, rp, op = max(residual.stride(0), C), residual.data_ptr(), out.data_ptr()
+        self._launch(dev, self._lib.forge_rms_norm, x.data_ptr(), _dtype_code(x), max(ldx, C), rp, ldr,
+                     weight.data_ptr(), _dtype_code(weight), T, C, float(eps), y.data_ptr(), op)
         return y, out
 
     def rms_norm_fp8(self, x, weight, eps, residual=None):
         """The same with codes [T,C] float8_e4m3fn and scale_inv [T,ceil(C/128)] f32 in y's place."""
-        _need_one_device(x, weight, residual)
+        dev = _need_one_device(x, weight, residual)
         T, C = x.shape
+        ldx, ldr, rp, out, op = x.stride(0), 0, 0, None, 0
         assert x.stride(1) == 1 and weight.is_contiguous() and weight.numel() == C
-        assert residual is None or (residual.dtype == x.dtype and residual.shape == x.shape
-                                    and residual.stride(1) == 1)
-        codes = torch.empty((T, C), dtype=torch.float8_e4m3fn, device=x.device)
-        scale_inv = torch.empty((T, (C + 127) // 128), dtype=torch.float32, device=x.device)
-        out = None if residual is None else torch.empty((T, C), dtype=x.dtype, device=x.device)
-        with torch.cuda.device(x.device):
-            self._check(self._lib.forge_rms_norm_fp8(
-                _ptr(x), _dtype_code(x), max(x.stride(0), C), _ptr(residual),
-                0 if residual is None else max(residual.stride(0), C), _ptr(weight), _dtype_code(weight), T, C,
-                float(eps), _ptr(codes), _ptr(scale_inv), _ptr(out), _stream()))
+        codes = torch.empty((T, C), dtype=torch.float8_e4m3fn, device=dev)
+        scale_inv = torch.empty((T, (C + 127) // 128), dtype=torch.float32, device=dev)
+        if residual is not None:
+            assert residual.dtype == x.dtype and residual.shape == x.shape and residual.stride(1) == 1
+            out = torch.empty((T, C), dtype=x.dtype, device=dev)
+            ldr, rp, op = max(residual.stride(0), C), residual.data_ptr(), out.data_ptr()
+        self._launch(dev, self._lib.forge_rms_norm_fp8, x.data_ptr(), _dtype_code(x), max(ldx, C), rp, ldr,
+                     weight.data_ptr(), _dtype_code(weight), T, C, float(eps), codes.data_ptr(),
+                     scale_inv.data_ptr(), op)
         return codes, scale_inv, out
 
     def gated_rows(self, rows, offsets, w_gate, w_up, activation="silu", keep=False):
         """rows [N,H] bf16 grouped by expert, offsets [E+1] int32 on the device, w_gate / w_up
         [E,I,H] bf16 with equal strides -> h [N,I] bf16; keep: also g and u [N,I] f32, for
         gated_rows_backward.  Allocates its results and nothing else; nothing waits for the GPU."""
-        _need_one_device(rows, offsets, w_gate, w_up)
+        dev = _need_one_device(rows, offsets, w_gate, w_up)
         E, I, H = w_gate.shape
         N = rows.shape[0]
+        ws, ldw, one = w_gate.stride()
         assert rows.dtype == w_gate.dtype == w_up.dtype == torch.bfloat16 and rows.shape[1] == H
         assert offsets.dtype == torch.int32 and offsets.is_contiguous() and offsets.numel() == E + 1
-        assert rows.stride(1) == w_gate.stride(2) == 1 and w_gate.stride() == w_up.stride()
+        assert rows.stride(1) == one == 1 and w_gate.stride() == w_up.stride()
         assert w_up.shape == w_gate.shape
-        h = torch.empty((N, I), dtype=torch.bfloat16, device=rows.device)
+        h = torch.empty((N, I), dtype=torch.bfloat16, device=dev)
         g = u = None
         if keep:
-            g = torch.empty((N, I), dtype=torch.float32, device=rows.device)
-            u = torch.empty_like(g)
-        with torch.cuda.device(rows.device):
-            self._check(self._lib.forge_gated_rows(
-                _ptr(rows), max(rows.stride(0), H), _ptr(offsets), _ptr(w_gate), _ptr(w_up),
-                max(w_gate.stride(1), H), w_gate.stride(0), N, E, H, I, _act_code(activation), _ptr(h), _ptr(g),
-                _ptr(u), _stream()))
+            g, u = torch.empty((2, N, I), dtype=torch.float32, device=dev)
+        self._launch(dev, self._lib.forge_gated_rows, rows.data_ptr(), max(rows.stride(0), H),
+                     offsets.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), max(ldw, H), ws, N, E, H, I,
+                     _act_code(activation), h.data_ptr(), g.data_ptr() if keep else 0,
+                     u.data_ptr() if keep else 0)
         return (h, g, u) if keep else h
 
     def gated_rows_backward(self, dh, g, u, rows, offsets, w_gate, w_up, activation="silu",
                             need=(True, True, True)):
         """Gradients of gated_rows for dh [N,I] bf16 contiguous: (d rows [N,H], d w_gate, d w_up
         [E,I,H]) in bf16, None where `need` says so."""
-        _need_one_device(dh, g, u, rows, offsets, w_gate, w_up)
+        dev = _need_one_device(dh, g, u, rows, offsets, w_gate, w_up)
         E, I, H = w_gate.shape
         N = rows.shape[0]
+        ws, ldw, one = w_gate.stride()
         assert dh.dtype == rows.dtype == w_gate.dtype == w_up.dtype == torch.bfloat16
         assert tuple(dh.shape) == tuple(g.shape) == tuple(u.shape) == (N, I) and dh.is_contiguous()
         assert g.dtype == u.dtype == torch.float32 and g.is_contiguous() and u.is_contiguous()
         assert offsets.dtype == torch.int32 and offsets.is_contiguous() and offsets.numel() == E + 1
-        assert rows.stride(1) == w_gate.stride(2) == 1 and w_gate.stride() == w_up.stride()
-        dev = rows.device
+        assert rows.stride(1) == one == 1 and w_gate.stride() == w_up.stride()
+        assert w_up.shape == w_gate.shape and tuple(rows.shape) == (N, H)
         dx = torch.empty((N, H), dtype=torch.bfloat16, device=dev) if need[0] else None
         dwg = torch.empty((E, I, H), dtype=torch.bfloat16, device=dev) if need[1] else None
         dwu = torch.empty((E, I, H), dtype=torch.bfloat16, device=dev) if need[2] else None
         nbytes = int(self._lib.forge_gated_rows_backward_workspace_bytes(N, I))
-        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            self._check(self._lib.forge_gated_rows_backward(
-                _ptr(dh), _ptr(g), _ptr(u), _ptr(rows), max(rows.stride(0), H), _ptr(offsets), _ptr(w_gate),
-                _ptr(w_up), max(w_gate.stride(1), H), w_gate.stride(0), N, E, H, I, _act_code(activation),
-                _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(ws), ws.numel(), _stream()))
+        work = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+        ptr = lambda t: 0 if t is None else t.data_ptr()   # noqa: E731
+        self._launch(dev, self._lib.forge_gated_rows_backward, dh.data_ptr(), g.data_ptr(), u.data_ptr(),
+                     rows.data_ptr(), max(rows.stride(0), H), offsets.data_ptr(), w_gate.data_ptr(),
+                     w_up.data_ptr(), max(ldw, H), ws, N, E, H, I, _act_code(activation), ptr(dx), ptr(dwg),
+                     ptr(dwu), work.data_ptr(), nbytes)
         return dx, dwg, dwu
 
     def linear_int4(self, x, packed, scale, group_size, bias=None, activation=None, residual=None):
         """x [M,C] bf16, packed [R,ceil(C/8)] int32, scale [R,G] f32 (pack_int4's words and its
         groups' scales) -> act(x W^T + bias) + residual [M,R] bf16."""
-        _need_one_device(x, packed, scale, bias, residual)
+        dev = _need_one_device(x, packed, scale, bias, residual)
         M, C = x.shape
-        R = packed.shape[0]
+        R, words = packed.shape
+        ldx, ldr, bp, rp = x.stride(0), 0, 0, 0
         assert x.dtype == torch.bfloat16 and x.stride(1) == 1
-        assert packed.dtype == torch.int32 and packed.is_contiguous() and packed.shape[1] == (C + 7) // 8
+        assert packed.dtype == torch.int32 and packed.is_contiguous() and words == (C + 7) // 8
         assert scale.dtype == torch.float32 and scale.is_contiguous()
-        assert tuple(scale.shape) == (R, (C + group_size - 1) // group_size)
-        assert bias is None or (bias.dtype == torch.bfloat16 and bias.is_contiguous() and bias.numel() == R)
-        assert residual is None or (residual.dtype == torch.bfloat16 and residual.stride(1) == 1
-                                    and tuple(residual.shape) == (M, R))
-        y = torch.empty((M, R), dtype=torch.bfloat16, device=x.device)
-        with torch.cuda.device(x.device):
-            self._check(self._lib.forge_linear_int4(
-                _ptr(x), max(x.stride(0), C), _ptr(packed), _ptr(scale), int(group_size), _ptr(bias),
-                _ptr(residual), 0 if residual is None else max(residual.stride(0), R), M, C, R,
-                _act_code(activation), _ptr(y), _stream()))
+        assert scale.shape[0] == R and scale.shape[1] == (C + group_size - 1) // group_size
+        if bias is not None:
+            assert bias.dtype == torch.bfloat16 and bias.is_contiguous() and bias.numel() == R
+            bp = bias.data_ptr()
+        if residual is not None:
+            assert residual.dtype == torch.bfloat16 and residual.stride(1) == 1
+            assert residual.shape[0] == M and residual.shape[1] == R
+            ldr, rp = max(residual.stride(0), R), residual.data_ptr()
+        y = torch.empty((M, R), dtype=torch.bfloat16, device=dev)
+        self._launch(dev, self._lib.forge_linear_int4, x.data_ptr(), max(ldx, C), packed.data_ptr(),
+                     scale.data_ptr(), int(group_size), bp, rp, ldr, M, C, R, _act_code(activation),
+                     y.data_ptr())
         return y
 
 

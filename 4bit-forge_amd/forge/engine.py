@@ -62,9 +62,18 @@ def routed_rows(x: torch.Tensor, router_indices: torch.Tensor,
 
 
 def _no_gradient(name: str, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if not torch.is_grad_enabled():
+        return
+    for t in tensors:
+        if t is None or not t.requires_grad:
+            continue
         raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached "
                            "tensors")
+
+
+def _rows_of(t: torch.Tensor) -> torch.Tensor:
+    """[..., C] as [rows, C] with unit column stride"""
+    return _unit_rows(t if t.dim() == 2 else t.reshape(-1, t.shape[-1]))
 
 
 def _norm_arguments(name, x, weight, eps, residual):
@@ -73,16 +82,14 @@ def _norm_arguments(name, x, weight, eps, residual):
         raise ValueError(f"{name}: x is {x.dtype}, expected float32 or bfloat16")
     if weight.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"{name}: weight is {weight.dtype}, expected float32 or bfloat16")
-    if x.dim() < 1 or x.shape[-1] == 0 or tuple(weight.shape) != (x.shape[-1],):
+    if x.dim() < 1 or x.shape[-1] == 0 or weight.dim() != 1 or weight.shape[0] != x.shape[-1]:
         raise ValueError(f"{name}: weight {tuple(weight.shape)} does not fit rows of x {tuple(x.shape)}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError(f"{name}: residual {tuple(residual.shape)} {residual.dtype}, "
                          f"x {tuple(x.shape)} {x.dtype}")
     if not eps >= 0:
         raise ValueError(f"{name}: eps={eps}")
-    C = x.shape[-1]
-    flat = lambda t: None if t is None else _unit_rows(t.reshape(-1, C))   # noqa: E731
-    return flat(x), weight.contiguous(), flat(residual)
+    return _rows_of(x), weight.contiguous(), None if residual is None else _rows_of(residual)
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
@@ -94,7 +101,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     weight [C] bf16 or f32.  New tensors; no backward pass (refused where one is asked for)."""
     x2, w, r2 = _norm_arguments("rms_norm", x, weight, eps, residual)
     y, out = kernels.rms_norm(x2, w, eps, r2)
-    return y.view(x.shape) if residual is None else (y.view(x.shape), out.view(x.shape))
+    if x.dim() != 2:
+        y, out = y.view(x.shape), None if out is None else out.view(x.shape)
+    return y if residual is None else (y, out)
 
 
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
@@ -104,8 +113,10 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     ``kernels.fp8_block_dequant`` reads block-scaled weights."""
     x2, w, r2 = _norm_arguments("rms_norm_fp8", x, weight, eps, residual)
     codes, scale_inv, out = kernels.rms_norm_fp8(x2, w, eps, r2)
-    codes, scale_inv = codes.view(x.shape), scale_inv.view(*x.shape[:-1], scale_inv.shape[1])
-    return (codes, scale_inv) if residual is None else (codes, scale_inv, out.view(x.shape))
+    if x.dim() != 2:
+        codes, scale_inv = codes.view(x.shape), scale_inv.view(*x.shape[:-1], scale_inv.shape[1])
+        out = None if out is None else out.view(x.shape)
+    return (codes, scale_inv) if residual is None else (codes, scale_inv, out)
 
 
 class _GatedRows(torch.autograd.Function):
@@ -195,14 +206,14 @@ def linear_int4(x: torch.Tensor, packed: Dict[str, torch.Tensor], bias: Optional
     for)."""
     w, scale = packed["weight_packed"], packed["weight_scale"]
     _no_gradient("linear_int4", x, scale, bias, residual)
-    R, C = (int(v) for v in packed["weight_shape"])
+    R, C = packed["weight_shape"].tolist()
     if activation not in ACTIVATIONS:
         raise ValueError(f"linear_int4: unknown activation {activation!r} (one of {list(ACTIVATIONS)})")
     if x.dtype != torch.bfloat16:
         raise ValueError(f"linear_int4: x is {x.dtype}, expected bfloat16")
     if x.dim() < 1 or x.shape[-1] != C:
         raise ValueError(f"linear_int4: x {tuple(x.shape)} does not fit a weight of {R} x {C}")
-    if w.dtype != torch.int32 or tuple(w.shape) != (R, (C + 7) // 8):
+    if w.dtype != torch.int32 or w.shape != (R, (C + 7) // 8):
         raise ValueError(f"linear_int4: weight_packed {tuple(w.shape)} {w.dtype}, expected "
                          f"[{R}, {(C + 7) // 8}] int32")
     if scale.dim() != 2 or scale.shape[0] != R or not 1 <= scale.shape[1] <= C:
@@ -214,13 +225,13 @@ def linear_int4(x: torch.Tensor, packed: Dict[str, torch.Tensor], bias: Optional
         group_size = C // G
     if group_size < 1 or (C + group_size - 1) // group_size != G:
         raise ValueError(f"linear_int4: group_size={group_size} does not give {G} groups of {C} columns")
-    if bias is not None and (bias.dtype != torch.bfloat16 or tuple(bias.shape) != (R,)):
+    if bias is not None and (bias.dtype != torch.bfloat16 or bias.shape != (R,)):
         raise ValueError(f"linear_int4: bias {tuple(bias.shape)} {bias.dtype}, expected [{R}] bfloat16")
     shape = (*x.shape[:-1], R)
-    if residual is not None and (residual.dtype != torch.bfloat16 or tuple(residual.shape) != shape):
+    if residual is not None and (residual.dtype != torch.bfloat16 or residual.shape != shape):
         raise ValueError(f"linear_int4: residual {tuple(residual.shape)} {residual.dtype}, expected "
                          f"{shape} bfloat16")
-    y = kernels.linear_int4(_unit_rows(x.reshape(-1, C)), w.contiguous(), scale.float().contiguous(), group_size,
+    y = kernels.linear_int4(_rows_of(x), w.contiguous(), scale.float().contiguous(), group_size,
                             None if bias is None else bias.contiguous(), activation,
-                            None if residual is None else _unit_rows(residual.reshape(-1, R)))
-    return y.view(shape)
+                            None if residual is None else _rows_of(residual))
+    return y if len(shape) == 2 else y.view(shape)

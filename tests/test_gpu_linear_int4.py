@@ -32,6 +32,8 @@ CASES = [
     (33, 768, 2048, 32), (64, 1536, 96, 128), (65, 2048, 768, 128), (100, 264, 130, 128), (129, 4096, 300, 64),
     (256, 1024, 513, 256), (300, 2048, 768, 128), (513, 1504, 257, 32), (1000, 7168, 384, 128), (40, 7, 9, 128),
     (7, 320, 17, 64), (9, 8200, 24, 128), (260, 200, 131, 40), (1, 30000, 48, 128), (12, 640, 16, 96),
+    (300, 1000, 70, 1000), (270, 672, 40, 96), (400, 104, 129, 32), (290, 72, 20, 128), (700, 2048, 130, 2048),
+    (20, 1000, 70, 1000), (50, 72, 20, 128), (300, 320, 64, 64),
 ]
 
 
