@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256) void gated_any_kernel(GatedArgs a, int p_tiles
         dgu = which ? a.du : a.dg;
         dw = which ? a.dwu : a.dwg;
     } else {
-        if (!find_tile(a.offsets, a.E, a.N, T, qt, r, slot)) return;
+        if (!find_tile(a.offsets, a.E, a.N, T, [=](int) { return qt; }, r, slot)) return;
         expert = r.expert;
         inner = expert < 0 ? 0 : (MODE == FORWARD ? a.H : a.I);
         phases = MODE == DROWS ? 2 : 1;
@@ -163,38 +163,48 @@ __global__ __launch_bounds__(256) void gated_any_kernel(GatedArgs a, int p_tiles
 //             activation and the product need no exchange
 //   DROWS     P and Q of the gate, then of the up projection, into the same sums
 // The inner dimension's tail and rows or columns outside are zeros that the loads themselves write.
-// One barrier per stage: what a wavefront has waited for it publishes there, and everybody has then
-// finished reading the buffer that the loads issued next will overwrite.  The two buffers are
-// separate arrays and the loop is unrolled by two because the compiler otherwise has to assume that
-// a load on its way to LDS may hit what is being read, and waits for it.
 template <int MODE>
 __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tiles, int q_tiles) {
     using namespace forge;
     __shared__ __attribute__((aligned(1024))) char P0[kStageBytes], Q0[kStageBytes], P1[kStageBytes], Q1[kStageBytes];
     __shared__ int slot[4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wp = wave >> 2, wq = wave & 3;
-    int b = xcd_tile(blockIdx.x, gridDim.x);
-    const int pt = b % p_tiles;
-    b /= p_tiles;
+    // wavefronts i and i + 4 share a SIMD; they get different quarters of Q, so that a tile with few rows
+    // keeps one wavefront busy on every SIMD instead of two on some
+    const int wp = wave >> 2, wq = (wave & 3) ^ (wp << 1);
 
     RaggedTile r;
-    int q0 = 0, inner = 0, which = 0;
+    int q0 = 0, inner = 0, which = 0, pt;
     if constexpr (MODE == DWEIGHTS) {
-        q0 = (b % q_tiles) * kTile;
-        b /= q_tiles;
-        r.expert = b % a.E;
-        which = b / a.E;
+        // experts differ in rows, so every XCD takes an eighth of every expert's tiles
+        const int tiles = p_tiles * q_tiles, per = (tiles + 7) / 8;
+        const int i = blockIdx.x / 8, t = (blockIdx.x % 8) * per + i % per;
+        if (t >= tiles) return;
+        r.expert = (i / per) % a.E;
+        which = (i / per) / a.E;
+        pt = t % p_tiles;
+        q0 = (t / p_tiles) * kTile;
         r.row0 = clamp_offset(a.offsets, r.expert, 0, a.N);
         r.rows = clamp_offset(a.offsets, r.expert + 1, r.row0, a.N) - r.row0;
         inner = r.rows;
     } else {
-        if (!find_tile(a.offsets, a.E, a.N, kTile, b, r, slot)) return;
+        // runs of 4 tiles of Q by all tiles of P: the 32 workgroups that an XCD runs at a time are
+        // then 4 x 8 tiles, 12 panels through its L2 where 2 x 16 would be 18
+        if (!find_tile(a.offsets, a.E, a.N, kTile, [&](int q_count) {
+                const int t = xcd_tile(blockIdx.x, q_count * p_tiles);
+                if (t >= q_count * p_tiles) return -1;
+                const int run = t / (4 * p_tiles), in_run = t - run * 4 * p_tiles;
+                const int wide = min(q_count - run * 4, 4);
+                slot[3] = in_run / wide;
+                return run * 4 + in_run % wide;
+            }, r, slot)) return;
+        pt = __builtin_amdgcn_readfirstlane(slot[3]);
         inner = r.expert < 0 ? 0 : MODE == FORWARD ? a.H : a.I;
     }
     const int p0 = pt * (MODE == FORWARD ? kTile / 2 : kTile);
     const int per_phase = (inner + kStage - 1) / kStage;
-    const int stages = MODE == DROWS ? 2 * per_phase : per_phase;
+    // nothing to sum (rows of no expert, an expert without rows): one stage of zeros
+    const int stages = max(MODE == DROWS ? 2 * per_phase : per_phase, 1);
     const int64_t we = (int64_t)(r.expert < 0 ? 0 : r.expert) * a.ws;
 
     // loaders
@@ -204,34 +214,32 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
     if constexpr (MODE == FORWARD) {
         const bool up = (wave & 3) >= 2;                       // this wavefront loads rows of Wu
         const int rows = a.I - p0 < kTile / 2 ? a.I - p0 : kTile / 2;
-        lp_in.init(wave, lane, a.ldw, rows, [](int t) { return (t >> 7) * 64 + (t & 63); });
+        lp_in.init(lane, a.ldw, (wave >> 2) * 64 + (wave & 1) * 32);
         dp = descriptor((up ? a.wu : a.wg) + we + (int64_t)p0 * a.ldw, (uint32_t)(((rows - 1) * a.ldw + a.H) * 2));
-        lq_in.init(wave, lane, a.ldx, r.rows, [](int t) { return t; });
+        lq_in.init(lane, a.ldx, wave * 32);
         dq = descriptor(a.x + (int64_t)r.row0 * a.ldx, (uint32_t)(((r.rows - 1) * a.ldx + a.H) * 2));
     } else if constexpr (MODE == DROWS) {
         lp_out.init(wave, lane, a.ldw, a.H - p0);
-        lq_in.init(wave, lane, a.I, r.rows, [](int t) { return t; });
+        lq_in.init(lane, a.I, wave * 32);
     } else {
         lp_out.init(wave, lane, a.ldx, a.H - p0);
         lq_out.init(wave, lane, a.I, a.I - q0);
     }
-    auto stage = [&](int s, char* P, char* Q) {
+    auto load = [&](int s, char* P, char* Q) {
         if constexpr (MODE == FORWARD) {
-            lp_in.stage(dp, P, wave, s * kStage, a.H);
-            lq_in.stage(dq, Q, wave, s * kStage, a.H);
+            lp_in.stage(dp, P, wave, a.ldw, s * kStage, inner);
+            lq_in.stage(dq, Q, wave, a.ldx, s * kStage, inner);
         } else if constexpr (MODE == DROWS) {
             const bool up = s >= per_phase;
             const int k0 = (up ? s - per_phase : s) * kStage;
-            lp_out.stage((up ? a.wu : a.wg) + we + (int64_t)k0 * a.ldw + p0, a.ldw, a.I - k0, a.H - p0, P, wave);
+            lp_out.stage((up ? a.wu : a.wg) + we + (int64_t)k0 * a.ldw + p0, a.ldw, inner - k0, a.H - p0, P, wave);
             const __amdgpu_buffer_rsrc_t d = descriptor((up ? a.du : a.dg) + (int64_t)r.row0 * a.I, (uint32_t)(r.rows * a.I * 2));
-            lq_in.stage(d, Q, wave, k0, a.I);
+            lq_in.stage(d, Q, wave, a.I, k0, inner);
         } else {
             const int64_t k0 = (int64_t)r.row0 + s * kStage;
             lp_out.stage(a.x + k0 * a.ldx + p0, a.ldx, r.rows - s * kStage, a.H - p0, P, wave);
             lq_out.stage((which ? a.du : a.dg) + k0 * a.I + q0, a.I, r.rows - s * kStage, a.I - q0, Q, wave);
         }
-        // the compiler knows of no use of these loads before the next wait and would sink them there
-        __builtin_amdgcn_sched_barrier(0);
     };
     InnerFragment fp_in, fq_in;
     OuterFragment<4> fp_out;
@@ -239,75 +247,179 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
     if constexpr (MODE == FORWARD) fp_in.init(lane, wp * 4); else fp_out.init(lane, wp * 4);
     if constexpr (MODE == DWEIGHTS) fq_out.init(lane, wq * 2); else fq_in.init(lane, wq * 2);
 
-    f32x16_t acc[4][2];
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) acc[t][n][v] = 0.0f;
-    auto multiply = [&](const char* P, const char* Q) {
-        if constexpr (MODE == FORWARD) multiply_stage(P, Q, fp_in, fq_in, acc);
-        else if constexpr (MODE == DROWS) multiply_stage(P, Q, fp_out, fq_in, acc);
-        else multiply_stage(P, Q, fp_out, fq_out, acc);
+    // Registers 4 j .. 4 j + 3 of a tile: rows 8 j + 4 (lane / 32) .. + 3 of P, column lane & 31 of Q, i.e.
+    // 8 bytes of 32 rows of the output at a time.  The tile goes through LDS, [row of Q][column of P] with
+    // 16-byte piece c of row q at c ^ (q % 32), and leaves in runs of a whole row.
+    // (32 KB of the tile per buffer: 64 rows of 512 bytes, or 128 of FORWARD's 256 bytes.)
+    constexpr int kCols = MODE == FORWARD ? kTile / 2 : kTile, kPieces = kCols / 8, kRows = kStageBytes / (kCols * 2);
+    auto buffer = [&](int i) {
+        lds_char *b0 = (lds_char*)P0, *b1 = (lds_char*)Q0, *b2 = (lds_char*)P1, *b3 = (lds_char*)Q1;
+        return i == 0 ? b0 : i == 1 ? b1 : i == 2 ? b2 : b3;
     };
-    if (stages > 0) stage(0, P0, Q0);
-    // the loop's body has no way out in its middle: with one the accumulators change registers
-    int s = 0;
-    for (; s + 1 < stages; s += 2) {
-        wait_loads();
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    if (wq * 64 < (MODE == DWEIGHTS ? a.I - q0 : r.rows)) {
+        f32x16_t acc[4][2];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) acc[t][n][v] = 0.0f;
+        if constexpr (MODE == FORWARD) multiply_stages(stages, P0, Q0, P1, Q1, load, fp_in, fq_in, acc);
+        else if constexpr (MODE == DROWS) multiply_stages(stages, P0, Q0, P1, Q1, load, fp_out, fq_in, acc);
+        else multiply_stages(stages, P0, Q0, P1, Q1, load, fp_out, fq_out, acc);
         __syncthreads();
-        stage(s + 1, P1, Q1);
-        multiply(P0, Q0);
-        wait_loads();
-        __syncthreads();
-        if (s + 2 < stages) stage(s + 2, P0, Q0);
-        multiply(P1, Q1);
-    }
-    if (s < stages) {
-        wait_loads();
-        __syncthreads();
-        multiply(P0, Q0);
-    }
-    // registers 4 j .. 4 j + 3 of a tile: rows 8 j + 4 (lane / 32) .. + 3 of P, column lane & 31 of Q
+        // an opaque copy: addresses made from it are not formed before the inner loop, where they would
+        // cost registers
+        int lane_e = lane;
+        asm volatile("" : "+v"(lane_e));
+        lds_char* to = buffer(wq * 64 / kRows);
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        const int q = (wq * 2 + n) * 32 + (lane & 31);
-        if (MODE == DWEIGHTS ? q0 + q >= a.I : q >= r.rows) continue;
-        if constexpr (MODE == FORWARD) {
+        for (int n = 0; n < 2; ++n) {
+            const int q = wq * 64 + n * 32 + (lane_e & 31);
+            lds_char* row = to + (q % kRows) * (kCols * 2) + (lane_e >> 5) * 8;
+            if constexpr (MODE == FORWARD) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int i = p0 + wp * 64 + t * 32 + 8 * j + 4 * (lane >> 5);
-                    if (i >= a.I) continue;
-                    const int64_t at = (int64_t)(r.row0 + q) * a.I + i;
-                    f32x4_t g, u;
-                    float h[4];
+                    for (int j = 0; j < 4; ++j) {
+                        f32x4_t g, u;
+                        float h[4];
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        g[v] = acc[t][n][4 * j + v];
-                        u[v] = acc[t + 2][n][4 * j + v];
-                        h[v] = act_f32(a.act, g[v]) * u[v];
+                        for (int v = 0; v < 4; ++v) {
+                            g[v] = acc[t][n][4 * j + v];
+                            u[v] = acc[t + 2][n][4 * j + v];
+                            h[v] = act_f32(a.act, g[v]) * u[v];
+                        }
+                        *(__attribute__((address_space(3))) u32x2*)(row + (((wp * 8 + t * 4 + j) ^ (q % kPieces)) * 16)) =
+                            u32x2{pack_bf16(h[0], h[1]), pack_bf16(h[2], h[3])};
+                        const int i = p0 + wp * 64 + t * 32 + 8 * j + 4 * (lane_e >> 5);
+                        if (a.g && q < r.rows && i < a.I) {
+                            const int64_t at = (int64_t)(r.row0 + q) * a.I + i;
+                            *reinterpret_cast<f32x4_t*>(a.g + at) = g;
+                            *reinterpret_cast<f32x4_t*>(a.u + at) = u;
+                        }
                     }
-                    *reinterpret_cast<uint2*>(a.h + at) = make_uint2(pack_bf16(h[0], h[1]), pack_bf16(h[2], h[3]));
-                    if (a.g) {
-                        *reinterpret_cast<f32x4_t*>(a.g + at) = g;
-                        *reinterpret_cast<f32x4_t*>(a.u + at) = u;
-                    }
-                }
-        } else {
-            uint16_t* out = MODE == DROWS ? a.dx + (int64_t)(r.row0 + q) * a.H
-                                          : (which ? a.dwu : a.dwg) + ((int64_t)r.expert * a.I + q0 + q) * a.H;
+            } else {
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+                for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int c = p0 + (wp * 4 + t) * 32 + 8 * j + 4 * (lane >> 5);
-                    if (c >= a.H) continue;
-                    *reinterpret_cast<uint2*>(out + c) = make_uint2(pack_bf16(acc[t][n][4 * j], acc[t][n][4 * j + 1]),
-                                                                   pack_bf16(acc[t][n][4 * j + 2], acc[t][n][4 * j + 3]));
+                    for (int j = 0; j < 4; ++j)
+                        *(__attribute__((address_space(3))) u32x2*)(row + (((wp * 16 + t * 4 + j) ^ (q % kPieces)) * 16)) =
+                            u32x2{pack_bf16(acc[t][n][4 * j], acc[t][n][4 * j + 1]),
+                                  pack_bf16(acc[t][n][4 * j + 2], acc[t][n][4 * j + 3])};
+            }
+        }
+    } else {
+        load_stages(stages, P0, Q0, P1, Q1, load);
+        __syncthreads();
+    }
+    __syncthreads();
+    uint16_t* out;
+    int64_t pitch;
+    int rows, cols;
+    if constexpr (MODE == FORWARD) {
+        out = a.h + (int64_t)r.row0 * a.I + p0;
+        pitch = a.I; rows = r.rows; cols = a.I - p0;
+    } else if constexpr (MODE == DROWS) {
+        out = a.dx + (int64_t)r.row0 * a.H + p0;
+        pitch = a.H; rows = r.rows; cols = a.H - p0;
+    } else {
+        out = (which ? a.dwu : a.dwg) + ((int64_t)r.expert * a.I + q0) * a.H + p0;
+        pitch = a.H; rows = a.I - q0; cols = a.H - p0;
+    }
+    // wavefront w writes rows 32 w .. 32 w + 31
+    lds_char* from = buffer(wave * 32 / kRows);
+    const int piece = lane % kPieces;
+    if (piece * 8 < cols) {
+#pragma unroll 4
+        for (int i = 0; i < 32 * kPieces / 64; ++i) {
+            const int q = wave * 32 + i * (64 / kPieces) + lane / kPieces;
+            if (q >= rows) break;
+            const u32x4 v = *(__attribute__((address_space(3))) u32x4*)(from + (q % kRows) * (kCols * 2) +
+                                                                        ((piece ^ (q % kPieces)) * 16));
+            *reinterpret_cast<u32x4*>(out + q * pitch + piece * 8) = v;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- few rows: FORWARD alone
+// Bound by the weights of the experts that have rows, which stream through once.  A workgroup takes 16
+// features (their rows of Wg and of Wu) and all of H; its 8 wavefronts take every eighth run of 128
+// columns, straight into registers, and their sums meet in LDS in a fixed order.  That is
+// 8 I / 16 wavefronts per expert where the tiles above have 8 I / 128, and nothing waits for a
+// barrier before the end.  MT blocks of 16 rows; the rows come from the caches.
+template <int MT>
+__global__ __launch_bounds__(512) void gated_few_kernel(GatedArgs a, int p_tiles) {
+    using namespace forge;
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    constexpr int U = MT == 1 ? 2 : 1;                          // runs in flight per wavefront
+    __shared__ __attribute__((aligned(16))) float part[8][MT][2][16][16];    // [.., row, feature]
+    __shared__ int slot[4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 15, kb = lane >> 4;
+    const int i0 = (blockIdx.x % p_tiles) * 16, qt = blockIdx.x / p_tiles;
+    RaggedTile r;
+    if (!find_tile(a.offsets, a.E, a.N, 16 * MT, [=](int) { return qt; }, r, slot)) return;
+    const int inner = r.expert < 0 ? 0 : a.H;
+    const int64_t we = (int64_t)(r.expert < 0 ? 0 : r.expert) * a.ws + (int64_t)i0 * a.ldw;
+    const uint32_t wbytes = (uint32_t)(((min(a.I - i0, 16) - 1) * a.ldw + a.H) * 2);
+    const __amdgpu_buffer_rsrc_t dg = descriptor(a.wg + we, wbytes), du = descriptor(a.wu + we, wbytes);
+    const __amdgpu_buffer_rsrc_t dx = descriptor(a.x + (int64_t)r.row0 * a.ldx, (uint32_t)(((r.rows - 1) * a.ldx + a.H) * 2));
+    f32x4_t g[MT], u[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) g[t] = u[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    const int runs = (inner + 127) / 128;
+    for (int c0 = wave; c0 < runs; c0 += 8 * U) {
+        u32x4 wg[U][4], wu[U][4], x[U][MT][4];
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const int k = (c0 + 8 * i) * 128 + d * 32 + kb * 8;
+                const bool in = k < inner;
+                // (weight rows and rows behind the last are beyond their descriptors)
+                const int at = in ? (int)((n * a.ldw + k) * 2) : (int)kOutside;
+                wg[i][d] = __builtin_amdgcn_raw_buffer_load_b128(dg, at, 0, 0);
+                wu[i][d] = __builtin_amdgcn_raw_buffer_load_b128(du, at, 0, 0);
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+                    x[i][t][d] = __builtin_amdgcn_raw_buffer_load_b128(
+                        dx, in ? (int)(((t * 16 + n) * a.ldx + k) * 2) : (int)kOutside, 0, 0);
+            }
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    const bf16x8_t xv = __builtin_bit_cast(bf16x8_t, x[i][t][d]);
+                    g[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, wg[i][d]), xv, g[t], 0, 0, 0);
+                    u[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, wu[i][d]), xv, u[t], 0, 0, 0);
                 }
+    }
+    // register v: feature 4 (lane / 16) + v, row lane & 15
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        *reinterpret_cast<f32x4_t*>(&part[wave][t][0][n][kb * 4]) = g[t];
+        *reinterpret_cast<f32x4_t*>(&part[wave][t][1][n][kb * 4]) = u[t];
+    }
+    __syncthreads();
+    for (int o = threadIdx.x; o < MT * 256; o += 512) {
+        const int q = o / 16, f = o % 16;
+        if (q >= r.rows || i0 + f >= a.I) continue;
+        float gs = 0.0f, us = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+            gs += part[w][q / 16][0][q % 16][f];
+            us += part[w][q / 16][1][q % 16][f];
+        }
+        const int64_t at = (int64_t)(r.row0 + q) * a.I + i0 + f;
+        a.h[at] = f32_to_bf16_bits(act_f32(a.act, gs) * us);
+        if (a.g) {
+            a.g[at] = gs;
+            a.u[at] = us;
         }
     }
 }
@@ -366,6 +478,8 @@ bool tiles_fit(const GatedArgs& a) {
            aligned16(a.wu);
 }
 
+constexpr int64_t kFewRows = 256;    // up to here gated_few_kernel
+
 int64_t grad_bytes(int64_t N, int64_t I) { return forge::ceil_div(2 * N * I, 256) * 256; }
 
 int check(const char* name, const void* rows, int64_t ldx, const int32_t* offsets, const void* Wg,
@@ -400,10 +514,16 @@ extern "C" int forge_gated_rows(const void* rows, int64_t ldx, const int32_t* of
     hipStream_t st = (hipStream_t)stream;
     forge::KernelTiming timing("gated_rows", st, 4.0 * N * H * I, forge::WORK_FLOPS);
     const bool fast = tiles_fit(a) && aligned16(h) && aligned16(gate_out) && aligned16(up_out);
-    const int64_t p_tiles = forge::ceil_div(I, fast ? 128 : 32);
-    const int64_t blocks = p_tiles * forge::ragged_tiles(N, E, fast ? 256 : 64);
+    const bool few = fast && N <= kFewRows;
+    const int64_t p_tiles = forge::ceil_div(I, few ? 16 : fast ? 128 : 32);
+    const int q_tile = few ? (N <= 16 ? 16 : N <= 32 ? 32 : 64) : fast ? 256 : 64;
+    const int64_t blocks = forge::ceil_div(p_tiles * forge::ragged_tiles(N, E, q_tile), 8) * 8;
     FORGE_REQUIRE(blocks <= INT32_MAX, "forge_gated_rows: %lld workgroups", (long long)blocks);
-    if (fast) gated_tile_kernel<FORWARD><<<dim3((unsigned)blocks), 512, 0, st>>>(a, (int)p_tiles, 1);
+    const dim3 grid((unsigned)blocks);
+    if (few && q_tile == 16) gated_few_kernel<1><<<grid, 512, 0, st>>>(a, (int)p_tiles);
+    else if (few && q_tile == 32) gated_few_kernel<2><<<grid, 512, 0, st>>>(a, (int)p_tiles);
+    else if (few) gated_few_kernel<4><<<grid, 512, 0, st>>>(a, (int)p_tiles);
+    else if (fast) gated_tile_kernel<FORWARD><<<dim3((unsigned)blocks), 512, 0, st>>>(a, (int)p_tiles, 1);
     else gated_any_kernel<FORWARD><<<dim3((unsigned)blocks), 256, 0, st>>>(a, (int)p_tiles);
     FORGE_LAUNCH_CHECK();
     return FORGE_OK;
@@ -438,8 +558,8 @@ extern "C" int forge_gated_rows_backward(const void* dh, const float* g, const f
                       aligned16(dWg) && aligned16(dWu);
     const int tile = fast ? 256 : 64;
     const int64_t h_tiles = forge::ceil_div(H, tile), i_tiles = forge::ceil_div(I, tile);
-    const int64_t blocks = h_tiles * forge::ragged_tiles(N, E, tile);
-    FORGE_REQUIRE(blocks <= INT32_MAX && h_tiles * i_tiles * 2 * E <= INT32_MAX, "%s: too many workgroups", name);
+    const int64_t blocks = forge::ceil_div(h_tiles * forge::ragged_tiles(N, E, tile), 8) * 8;
+    FORGE_REQUIRE(blocks <= INT32_MAX && (h_tiles * i_tiles + 8) * 2 * E <= INT32_MAX, "%s: too many workgroups", name);
     if (N > 0) {
         forge::KernelTiming timing("gated_grad", st, 14.0 * N * I, forge::WORK_BYTES);
         if (fast)
@@ -462,7 +582,7 @@ extern "C" int forge_gated_rows_backward(const void* dh, const float* g, const f
         const int both = dWg && dWu ? 2 : 1;
         if (!dWg) { a.dg = du; a.dwg = a.dwu; }
         if (fast)
-            gated_tile_kernel<DWEIGHTS><<<dim3((unsigned)(h_tiles * i_tiles * E * both)), 512, 0, st>>>(
+            gated_tile_kernel<DWEIGHTS><<<dim3((unsigned)(forge::ceil_div(h_tiles * i_tiles, 8) * 8 * E * both)), 512, 0, st>>>(
                 a, (int)h_tiles, (int)i_tiles);
         else
             gated_any_kernel<DWEIGHTS><<<dim3((unsigned)(h_tiles * i_tiles), (unsigned)E, both), 256, 0, st>>>(

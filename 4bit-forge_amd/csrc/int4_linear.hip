@@ -5,7 +5,7 @@
 // products are exact; the scale is applied to every group's f32 sum.
 #include "act.h"
 #include "common.h"
-#include "mfma_tile.h"
+#include "mfma_tile64.h"
 
 namespace {
 using forge::act_f32;

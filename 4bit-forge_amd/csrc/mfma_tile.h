@@ -7,15 +7,17 @@
 // bytes a clock, so the matrix pipe and not the LDS is the limit; 64 x 64 per wavefront (16
 // wavefronts) would need 256 KB and sit exactly on it.
 //
-// Stages go from memory to LDS without touching registers (buffer_load ... lds, 16 bytes a lane):
-// the next stage's loads are issued before the current stage is multiplied.  A lane whose element
-// lies outside the matrix gets an offset beyond the descriptor's range, for which the hardware
-// writes zeros.
+// A stage is 64 deep and there are two buffers.  Stages go from memory to LDS without touching
+// registers (buffer_load ... lds, 16 bytes a lane), issued as soon as their buffer has been read,
+// seven eighths of two stages before their use.  A lane whose element lies outside the matrix gets an
+// offset beyond the descriptor's range, for which the hardware writes zeros; stages behind the last
+// are fetched like that too.
 //
 // The lanes of one such load write 1 KiB of consecutive LDS, so the layout that keeps the reads free of
 // bank conflicts is made by choosing which 16 bytes each lane fetches:
 //   K_INNER (the inner dimension is contiguous in memory): 256 rows of 128 bytes; 16-byte piece c of
 //     row r lies at piece c ^ (r / 2 % 8), so 16 consecutive rows of one piece cover all 64 banks.
+//     (Stages of 32 with four buffers were slower: rows of 64 bytes are twice the L2 requests.)
 //   K_OUTER (the inner dimension is the row): 64 rows of 512 bytes, read transposed by
 //     ds_read_b64_tr_b16 (16 lanes fetch 4 rows x 16 columns, lane i receives column i); piece c of
 //     row k lies at c ^ 4 (k % 4), so that the four rows of one read are in different banks.
@@ -39,57 +41,64 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor(const void* p, uint
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t d, char* lds, uint32_t offset) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (__attribute__((address_space(3))) void*)lds, 16, (int)offset, 0, 0, 0);
 }
-// everything this wavefront has on its way to LDS has arrived
-__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }   // vmcnt(0)
+// all but the last N of this wavefront's loads have arrived, and all of its LDS reads (vmcnt(N), lgkmcnt(0))
+template <int N>
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15)); }
+// the same, then the workgroup's barrier; nothing the compiler knows of moves across it
+template <int N>
+__device__ __forceinline__ void wait_loads_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    wait_loads<N>();
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+}
 
-// ---- K_INNER: rows `row0 ..` of a matrix with pitch ld, inner dimension `inner`
+// ---- K_INNER: the descriptor covers exactly the valid rows of pitch ld, so that rows behind them are
+// outside its range; the columns from `inner` on are sorted out here.  Load j of a wavefront takes
+// 8 rows, 8 j rows behind its first; its lanes' pieces are those of load 0 for even j, and the
+// others of their 128 bytes (piece ^ 4) for odd j.
 struct InnerLoader {
-    uint32_t off[4];     // byte offset of this lane's 16 bytes of the four loads of its wavefront
-    uint32_t piece[4];   // and their place in the stage (columns)
-    // `rows` valid rows (others read as zero); row_of(r): which row of the descriptor tile row r is
-    template <typename F>
-    __device__ __forceinline__ void init(int wave, int lane, int64_t ld, int rows, F row_of) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int r = (wave * 4 + j) * 8 + lane / 8;
-            const int c = (lane & 7) ^ ((r >> 1) & 7);
-            const int m = row_of(r);
-            piece[j] = c * 8;
-            off[j] = m < rows ? (uint32_t)(m * ld * 2) + c * 16 : kOutside;
-        }
+    uint32_t off;        // byte offset of this lane's row, load 0
+    int piece;           // columns into the stage, load 0
+    // first_row: which row of the descriptor the wavefront's first row is
+    __device__ __forceinline__ void init(int lane, int64_t ld, int first_row) {
+        off = (uint32_t)((first_row + lane / 8) * ld * 2);
+        piece = ((lane & 7) ^ (lane >> 4)) * 8;
     }
-    __device__ __forceinline__ void stage(__amdgpu_buffer_rsrc_t d, char* lds, int wave, int k0, int inner) const {
+    __device__ __forceinline__ void stage(__amdgpu_buffer_rsrc_t d, char* lds, int wave, int64_t ld, int k0, int inner) const {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const uint32_t o = k0 + (int)piece[j] < inner ? off[j] + (uint32_t)k0 * 2 : kOutside;
-            load_to_lds(d, lds + (wave * 4 + j) * 1024, o);
+            const int k = k0 + ((j & 1) ? piece ^ 32 : piece);
+            load_to_lds(d, lds + (wave * 4 + j) * 1024, k < inner ? off + (uint32_t)(k * 2) + (uint32_t)(j * 16 * ld) : kOutside);
         }
     }
 };
 // ---- K_OUTER: columns `col0 ..` of a matrix whose rows are the inner dimension.  The descriptor is
 // made per stage (base at the stage's first row), so row offsets never pass 32 bits.
 struct OuterLoader {
-    uint32_t off[4];
+    uint32_t even, odd;  // byte offsets of loads 0 and 1; 2 and 3 are 4 rows behind
     __device__ __forceinline__ void init(int wave, int lane, int64_t ld, int cols) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int k = (wave * 4 + j) * 2 + lane / 32;
-            const int c = (lane & 31) ^ ((k & 3) << 2);
-            off[j] = c * 8 < cols ? (uint32_t)(k * ld * 2) + c * 16 : kOutside;
-        }
+        const int k = wave * 8 + lane / 32, c = (lane & 31) ^ ((lane / 32) << 2);
+        even = c * 8 < cols ? (uint32_t)(k * ld * 2) + c * 16 : kOutside;
+        odd = (c ^ 8) * 8 < cols ? (uint32_t)((k + 2) * ld * 2) + (c ^ 8) * 16 : kOutside;
     }
     // base: first row of the stage at the tile's first column; rows left in the matrix from there
     __device__ __forceinline__ void stage(const uint16_t* base, int64_t ld, int left, int cols, char* lds, int wave) const {
-        const int rows = left < kStage ? left : kStage;
-        const int width = cols < kTile ? cols : kTile;
-        const __amdgpu_buffer_rsrc_t d = descriptor(base, (uint32_t)(((rows - 1) * ld + width) * 2));
+        const int rows = min(left, kStage), width = min(cols, kTile);
+        const int size = max((rows - 1) * (int)ld + width, 0);           // 0 rows or fewer: nothing
+        const __amdgpu_buffer_rsrc_t d = descriptor(base, (uint32_t)size * 2);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) load_to_lds(d, lds + (wave * 4 + j) * 1024, off[j]);
+        for (int j = 0; j < 4; ++j)
+            // (kOutside plus a few rows is still outside)
+            load_to_lds(d, lds + (wave * 4 + j) * 1024, ((j & 1) ? odd : even) + (uint32_t)((j >> 1) * 8 * ld));
     }
 };
 
 // ---- fragments: 32 rows (tile t of the operand) x 16 of the inner dimension (step s of the stage)
 struct InnerFragment {
+    static constexpr int kReads = 1;     // LDS instructions per fragment
     uint32_t at[4];
     __device__ __forceinline__ void init(int lane, int tile0) {
         const int r = lane & 31;
@@ -103,6 +112,7 @@ struct InnerFragment {
 };
 template <int TILES>
 struct OuterFragment {
+    static constexpr int kReads = 2;
     uint32_t at[TILES];
     __device__ __forceinline__ void init(int lane, int tile0) {
         const int g = lane >> 4, i = lane & 15;
@@ -122,30 +132,115 @@ struct OuterFragment {
     }
 };
 
-// One stage: 4 steps of 16, 4 x 2 matrix instructions each.
-template <typename FP, typename FQ>
-__device__ __forceinline__ void multiply_stage(const char* P, const char* Q, const FP& fp, const FQ& fq,
-                                               f32x16_t (&acc)[4][2]) {
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        bf16x8_t p[4], q[2];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) p[t] = fp.read(P, t, s);
+// The fragments of one step: 4 of P, 2 of Q
+struct Fragments {
+    bf16x8_t p[4], q[2];
+    template <typename FP, typename FQ>
+    __device__ __forceinline__ void read(const char* P, const char* Q, const FP& fp, const FQ& fq, int s) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) q[t] = fq.read(Q, t, s);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) p[t] = fp.read(P, t, s);
+    }
+    __device__ __forceinline__ void multiply(f32x16_t (&acc)[4][2]) const {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int n = 0; n < 2; ++n)
                 acc[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[t], q[n], acc[t][n], 0, 0, 0);
     }
+};
+
+// The order in which a step issues: after every matrix instruction its share of the next step's LDS
+// reads and (LOADS) of the loads to LDS.  Left alone the compiler sinks the reads to the step's end.
+template <int READS, int LOADS>
+__device__ __forceinline__ void order_step() {
+    constexpr int kPer = (READS + 5) / 6;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                       // matrix instruction
+        if (i < LOADS) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);        // load to LDS
+        if (i < 6) __builtin_amdgcn_sched_group_barrier(0x100, kPer, 0);         // LDS read
+    }
 }
 
-// Workgroup b of a launch runs on XCD b % 8 (each has its own L2): gives every XCD a run of
-// consecutive tiles, so that tiles that share an operand share an L2.
-__device__ __forceinline__ int xcd_tile(int b, int blocks) {
-    const int q = blocks / 8, r = blocks % 8, x = b % 8;
-    return x * q + (x < r ? x : r) + b / 8;
+// The inner loop.  load(s, P, Q) issues stage s's loads (8 per wavefront).  A stage is four steps;
+// while a step's 8 matrix instructions run, the next step's fragments are read.  The one barrier of
+// a stage sits before its last step, whose fragments are in registers by then: nothing waits behind
+// it.  It publishes that the next stage has arrived and that this stage's buffer has been read, which
+// the loads of the stage after next then fill.
+// The buffers are separate arrays and the loop is unrolled over them because the compiler otherwise
+// has to assume that a load on its way to LDS may hit what is being read, and waits for it.
+template <typename LOAD, typename FP, typename FQ>
+__device__ __forceinline__ void one_stage(int s, char* P, char* Q, const char* Pn, const char* Qn, LOAD& load,
+                                          const FP& fp, const FQ& fq, Fragments& f, f32x16_t (&acc)[4][2]) {
+    constexpr int kReads = 4 * FP::kReads + 2 * FQ::kReads;
+    Fragments g;
+    g.read(P, Q, fp, fq, 1);
+    f.multiply(acc);
+    order_step<kReads, 0>();
+    __builtin_amdgcn_sched_barrier(0);
+    f.read(P, Q, fp, fq, 2);
+    g.multiply(acc);
+    order_step<kReads, 0>();
+    __builtin_amdgcn_sched_barrier(0);
+    g.read(P, Q, fp, fq, 3);
+    f.multiply(acc);
+    order_step<kReads, 0>();
+    wait_loads_barrier<0>();
+    load(s + 2, P, Q);
+    f.read(Pn, Qn, fp, fq, 0);
+    g.multiply(acc);
+    order_step<kReads, 8>();
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// stages >= 1
+template <typename LOAD, typename FP, typename FQ>
+__device__ __forceinline__ void multiply_stages(int stages, char* P0, char* Q0, char* P1, char* Q1, LOAD& load,
+                                                const FP& fp, const FQ& fq, f32x16_t (&acc)[4][2]) {
+    load(0, P0, Q0);
+    load(1, P1, Q1);
+    wait_loads_barrier<8>();
+    Fragments f;
+    f.read(P0, Q0, fp, fq, 0);
+    int s = 0;
+    for (; s + 2 <= stages; s += 2) {
+        one_stage(s, P0, Q0, P1, Q1, load, fp, fq, f, acc);
+        one_stage(s + 1, P1, Q1, P0, Q0, load, fp, fq, f, acc);
+    }
+    if (s < stages) one_stage(s, P0, Q0, P1, Q1, load, fp, fq, f, acc);
+    // loads of stages behind the last (zeros) are still on their way to LDS: a workgroup that ends
+    // gives its LDS away
+    wait_loads<0>();
+}
+
+// What a wavefront without outputs of its own does meanwhile: its share of the loads, and the barriers
+template <typename LOAD>
+__device__ __forceinline__ void load_stages(int stages, char* P0, char* Q0, char* P1, char* Q1, LOAD& load) {
+    load(0, P0, Q0);
+    load(1, P1, Q1);
+    wait_loads_barrier<8>();
+    int s = 0;
+    for (; s + 2 <= stages; s += 2) {
+        wait_loads_barrier<0>();
+        load(s + 2, P0, Q0);
+        wait_loads_barrier<0>();
+        load(s + 3, P1, Q1);
+    }
+    if (s < stages) {
+        wait_loads_barrier<0>();
+        load(s + 2, P0, Q0);
+    }
+    wait_loads<0>();
+}
+
+// Workgroup b of a launch runs on XCD b % 8 (each has its own L2).  Of `tiles` tiles every XCD takes
+// a run of consecutive ones, so that tiles that share an operand share an L2; the tile of b's, or
+// `tiles` or more if there is none.
+__device__ __forceinline__ int xcd_tile(int b, int tiles) {
+    const int per = (tiles + 7) / 8, i = b / 8;
+    return i < per ? (b % 8) * per + i : tiles;
 }
 
 }  // namespace forge
