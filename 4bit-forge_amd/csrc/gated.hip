@@ -345,82 +345,248 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
 }
 
 // ---------------------------------------------------------------- few rows: FORWARD alone
-// Bound by the weights of the experts that have rows, which stream through once.  A workgroup takes 16
-// features (their rows of Wg and of Wu) and all of H; its 8 wavefronts take every eighth run of 128
-// columns, straight into registers, and their sums meet in LDS in a fixed order.  That is
-// 8 I / 16 wavefronts per expert where the tiles above have 8 I / 128, and nothing waits for a
-// barrier before the end.  MT blocks of 16 rows; the rows come from the caches.
+// Bound by the weights of the experts that have rows, which stream through once.  A wavefront takes 16
+// features (their rows of Wg and of Wu) and every `split`-th run of 128 columns, and no barrier
+// before the end; the split wavefronts that share their features add up in LDS in a fixed order.
+// A workgroup's 8 wavefronts cover 128 / split features: the host splits as far as it takes to fill
+// the GPU, and no further, since a wavefront with few runs spends its time on its beginning and end.
+// Every wavefront has two LDS buffers of its own, one run each.  Runs go there by loads of 256
+// consecutive bytes of 4 rows (straight into registers the matrix instruction's layout would fetch 64
+// bytes of 16 rows at a time, which HBM serves a third slower); 16-byte piece c of row n lies at c ^ n.
+// MT blocks of 16 rows, which come from the caches.
+constexpr int kRunBytes = 32 * 256;                              // 16 rows of Wg, 16 of Wu, 128 columns
 template <int MT>
-__global__ __launch_bounds__(512) void gated_few_kernel(GatedArgs a, int p_tiles) {
+__global__ __launch_bounds__(512) void gated_few_kernel(GatedArgs a, int p_tiles, int split) {
     using namespace forge;
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    constexpr int U = MT == 1 ? 2 : 1;                          // runs in flight per wavefront
-    __shared__ __attribute__((aligned(16))) float part[8][MT][2][16][16];    // [.., row, feature]
+    __shared__ __attribute__((aligned(1024))) char S0[8 * kRunBytes], S1[8 * kRunBytes];
     __shared__ int slot[4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, kb = lane >> 4;
-    const int i0 = (blockIdx.x % p_tiles) * 16, qt = blockIdx.x / p_tiles;
+    const int share = wave % split;                              // which of its features' runs
+    const int f0 = (blockIdx.x % p_tiles) * (128 / split), qt = blockIdx.x / p_tiles;
+    const int i0 = f0 + wave / split * 16;
     RaggedTile r;
     if (!find_tile(a.offsets, a.E, a.N, 16 * MT, [=](int) { return qt; }, r, slot)) return;
     const int inner = r.expert < 0 ? 0 : a.H;
-    const int64_t we = (int64_t)(r.expert < 0 ? 0 : r.expert) * a.ws + (int64_t)i0 * a.ldw;
-    const uint32_t wbytes = (uint32_t)(((min(a.I - i0, 16) - 1) * a.ldw + a.H) * 2);
+    const int wrows = min(a.I - i0, 16);                          // none for a wavefront behind the last feature
+    const int64_t we = (int64_t)(r.expert < 0 ? 0 : r.expert) * a.ws + (wrows > 0 ? (int64_t)i0 * a.ldw : 0);
+    const uint32_t wbytes = wrows > 0 ? (uint32_t)(((wrows - 1) * a.ldw + a.H) * 2) : 0u;
     const __amdgpu_buffer_rsrc_t dg = descriptor(a.wg + we, wbytes), du = descriptor(a.wu + we, wbytes);
     const __amdgpu_buffer_rsrc_t dx = descriptor(a.x + (int64_t)r.row0 * a.ldx, (uint32_t)(((r.rows - 1) * a.ldx + a.H) * 2));
     f32x4_t g[MT], u[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) g[t] = u[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     const int runs = (inner + 127) / 128;
-    for (int c0 = wave; c0 < runs; c0 += 8 * U) {
-        u32x4 wg[U][4], wu[U][4], x[U][MT][4];
+    // (weight rows and rows behind the last are beyond their descriptors)
+    auto fetch = [&](int c, char* S, u32x4 (&x)[MT][4]) {
+        char* to = S + wave * kRunBytes;
 #pragma unroll
-        for (int i = 0; i < U; ++i)
+        for (int j = 0; j < 4; ++j) {
+            const int row = j * 4 + kb, k = c * 128 + (n ^ row) * 8;
+            const uint32_t at = k < inner ? (uint32_t)((row * a.ldw + k) * 2) : kOutside;
+            load_to_lds(dg, to + j * 1024, at);
+            load_to_lds(du, to + 4096 + j * 1024, at);
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
-                const int k = (c0 + 8 * i) * 128 + d * 32 + kb * 8;
-                const bool in = k < inner;
-                // (weight rows and rows behind the last are beyond their descriptors)
-                const int at = in ? (int)((n * a.ldw + k) * 2) : (int)kOutside;
-                wg[i][d] = __builtin_amdgcn_raw_buffer_load_b128(dg, at, 0, 0);
-                wu[i][d] = __builtin_amdgcn_raw_buffer_load_b128(du, at, 0, 0);
-#pragma unroll
-                for (int t = 0; t < MT; ++t)
-                    x[i][t][d] = __builtin_amdgcn_raw_buffer_load_b128(
-                        dx, in ? (int)(((t * 16 + n) * a.ldx + k) * 2) : (int)kOutside, 0, 0);
+                const int k = c * 128 + d * 32 + kb * 8;
+                x[t][d] = __builtin_amdgcn_raw_buffer_load_b128(
+                    dx, k < inner ? (int)(((t * 16 + n) * a.ldx + k) * 2) : (int)kOutside, 0, 0);
             }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto multiply = [&](const char* S, const u32x4 (&x)[MT][4]) {
+        const char* from = S + wave * kRunBytes + n * 256;
+        bf16x8_t wg[4], wu[4];
 #pragma unroll
-        for (int i = 0; i < U; ++i)
+        for (int d = 0; d < 4; ++d) {
+            wg[d] = *reinterpret_cast<const bf16x8_t*>(from + (((d * 4 + kb) ^ n) * 16));
+            wu[d] = *reinterpret_cast<const bf16x8_t*>(from + 4096 + (((d * 4 + kb) ^ n) * 16));
+        }
 #pragma unroll
-            for (int d = 0; d < 4; ++d)
+        for (int d = 0; d < 4; ++d)
 #pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    const bf16x8_t xv = __builtin_bit_cast(bf16x8_t, x[i][t][d]);
-                    g[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, wg[i][d]), xv, g[t], 0, 0, 0);
-                    u[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, wu[i][d]), xv, u[t], 0, 0, 0);
-                }
+            for (int t = 0; t < MT; ++t) {
+                const bf16x8_t xv = __builtin_bit_cast(bf16x8_t, x[t][d]);
+                g[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wg[d], xv, g[t], 0, 0, 0);
+                u[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wu[d], xv, u[t], 0, 0, 0);
+            }
+        // the buffer is free once the reads are back
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0xC07F);                       // lgkmcnt(0)
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // all but the last run's loads (8 to LDS, 4 MT to registers) have arrived
+    auto arrived = [] {
+        constexpr int kLater = 8 + 4 * MT;
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0x0F70 | (kLater & 15) | ((kLater >> 4) << 14));
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+    };
+    u32x4 x0[MT][4], x1[MT][4];
+    // runs behind the last are fetched as zeros, so that every wavefront always has two on their way
+    fetch(share, S0, x0);
+    fetch(share + split, S1, x1);
+    for (int c = share; c < runs; c += 2 * split) {
+        arrived();
+        multiply(S0, x0);
+        fetch(c + 2 * split, S0, x0);
+        arrived();
+        multiply(S1, x1);
+        fetch(c + 3 * split, S1, x1);
     }
-    // register v: feature 4 (lane / 16) + v, row lane & 15
+    __builtin_amdgcn_s_waitcnt(0x0F70);                           // vmcnt(0): the zeros behind the last run
+    __syncthreads();
+    // [wavefront][block of rows][gate, up][row][feature]; register v: feature 4 (lane / 16) + v, row lane & 15
+    float* part = reinterpret_cast<float*>(S0);
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-        *reinterpret_cast<f32x4_t*>(&part[wave][t][0][n][kb * 4]) = g[t];
-        *reinterpret_cast<f32x4_t*>(&part[wave][t][1][n][kb * 4]) = u[t];
+        *reinterpret_cast<f32x4_t*>(part + ((wave * MT + t) * 2 + 0) * 256 + n * 16 + kb * 4) = g[t];
+        *reinterpret_cast<f32x4_t*>(part + ((wave * MT + t) * 2 + 1) * 256 + n * 16 + kb * 4) = u[t];
     }
     __syncthreads();
-    for (int o = threadIdx.x; o < MT * 256; o += 512) {
-        const int q = o / 16, f = o % 16;
-        if (q >= r.rows || i0 + f >= a.I) continue;
+    const int features = 128 / split;
+    for (int o = threadIdx.x; o < MT * 16 * features; o += 512) {
+        const int q = o / features, f = o % features;
+        if (q >= r.rows || f0 + f >= a.I) continue;
+        const float* p = part + ((f / 16 * split * MT + q / 16) * 2) * 256 + (q % 16) * 16 + f % 16;
         float gs = 0.0f, us = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) {
-            gs += part[w][q / 16][0][q % 16][f];
-            us += part[w][q / 16][1][q % 16][f];
+        for (int w = 0; w < split; ++w, p += MT * 512) {
+            gs += p[0];
+            us += p[256];
         }
-        const int64_t at = (int64_t)(r.row0 + q) * a.I + i0 + f;
+        const int64_t at = (int64_t)(r.row0 + q) * a.I + f0 + f;
         a.h[at] = f32_to_bf16_bits(act_f32(a.act, gs) * us);
         if (a.g) {
             a.g[at] = gs;
             a.u[at] = us;
         }
+    }
+}
+
+// ---------------------------------------------------------------- few rows: DROWS
+// The same idea with W's rows as the inner dimension: a workgroup takes 128 columns of X and one tile
+// of 32 rows, its 8 wavefronts every eighth run of 32 of W's rows (the gate's, then the up
+// projection's), 256 consecutive bytes of each, and their sums meet in LDS in a fixed order.  H / 128
+// workgroups of 2 I / 256 runs per expert where the tiles above have H / 256 of 2 I / 64 stages.
+// A run's row k lies at 256 k, its 16-byte piece c at c ^ 4 (k % 4): transposed reads as in mfma_tile.h.
+__global__ __launch_bounds__(512) void gated_drows_few_kernel(GatedArgs a, int p_tiles) {
+    using namespace forge;
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    constexpr int kRun = 32 * 256;
+    __shared__ __attribute__((aligned(1024))) char S0[8 * kRun], S1[8 * kRun];
+    __shared__ int slot[4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int p0 = (blockIdx.x % p_tiles) * 128, qt = blockIdx.x / p_tiles;
+    RaggedTile r;
+    if (!find_tile(a.offsets, a.E, a.N, 32, [=](int) { return qt; }, r, slot)) return;
+    const int per_phase = r.expert < 0 ? 0 : (a.I + 31) / 32, runs = 2 * per_phase;
+    const int64_t we = (int64_t)(r.expert < 0 ? 0 : r.expert) * a.ws + p0;
+    const int cols = min(a.H - p0, 128);
+    // this lane's place in a load of 4 rows
+    const int row = lane >> 4, piece = (lane & 15) ^ (row << 2);
+    const uint32_t at0 = piece * 8 < cols ? (uint32_t)((row * a.ldw + piece * 8) * 2) : kOutside;
+    auto fetch = [&](int c, char* S, u32x4 (&q)[2]) {
+        const bool up = c >= per_phase;
+        const int k0 = (up ? c - per_phase : c) * 32;
+        // runs behind the last have no rows: zeros
+        const int rows = c < runs ? min(a.I - k0, 32) : 0;
+        const int size = max((rows - 1) * (int)a.ldw + cols, 0);
+        const __amdgpu_buffer_rsrc_t dw = descriptor((up ? a.wu : a.wg) + we + (c < runs ? k0 * a.ldw : 0), (uint32_t)size * 2);
+        const __amdgpu_buffer_rsrc_t dd = descriptor((up ? a.du : a.dg) + (int64_t)r.row0 * a.I, (uint32_t)(r.rows * a.I * 2));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) load_to_lds(dw, S + wave * kRun + j * 1024, at0 + (uint32_t)(j * 8 * a.ldw));
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int k = k0 + s * 16 + (lane >> 5) * 8;
+            q[s] = __builtin_amdgcn_raw_buffer_load_b128(
+                dd, c < runs && k < a.I ? (int)(((lane & 31) * a.I + k) * 2) : (int)kOutside, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    f32x16_t acc[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) acc[t][v] = 0.0f;
+    uint32_t from[4];
+    {
+        const int g = lane >> 4, i = lane & 15, k = 8 * (g >> 1) + (i >> 2), col = 16 * (g & 1) + 4 * (i & 3);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) from[t] = wave * kRun + k * 256 + ((((col >> 3) + t * 4) ^ ((i >> 2) << 2)) * 16) + (col & 7) * 2;
+    }
+    auto multiply = [&](const char* S, const u32x4 (&q)[2]) {
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        bf16x8_t p[2][4];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const char* f = S + from[t] + s * 4096;
+                const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)f);
+                const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(f + 1024));
+                const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                p[s][t] = __builtin_bit_cast(bf16x8_t, v);
+            }
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[s][t], __builtin_bit_cast(bf16x8_t, q[s]), acc[t], 0, 0, 0);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0xC07F);                       // lgkmcnt(0): the buffer is free
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto arrived = [] {                                           // all but the last run's 10 loads
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0x0F7A);
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+    };
+    u32x4 q0[2], q1[2];
+    fetch(wave, S0, q0);
+    fetch(wave + 8, S1, q1);
+    for (int c = wave; c < runs; c += 16) {
+        arrived();
+        multiply(S0, q0);
+        fetch(c + 16, S0, q0);
+        arrived();
+        multiply(S1, q1);
+        fetch(c + 24, S1, q1);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    __syncthreads();
+    // [wavefront][row][128 columns] f32, 16 KB a wavefront: four in either buffer.  Registers 4 j .. 4 j + 3
+    // of tile t: columns 32 t + 8 j + 4 (lane / 32) .. + 3, row lane & 31; 16-byte piece c of row q at c ^ q.
+    {
+        char* part = (wave < 4 ? S0 : S1) + (wave & 3) * 16384 + (lane & 31) * 512;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                f32x4_t v;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = acc[t][4 * j + i];
+                *reinterpret_cast<f32x4_t*>(part + (((t * 8 + j * 2 + (lane >> 5)) ^ (lane & 31)) * 16)) = v;
+            }
+    }
+    __syncthreads();
+    // a thread sums 4 columns of one row, twice
+    for (int o = threadIdx.x; o < 32 * 32; o += 512) {
+        const int q = o >> 5, c = o & 31;
+        if (q >= r.rows || c * 4 >= cols) continue;
+        f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+            v += *reinterpret_cast<const f32x4_t*>((w < 4 ? S0 : S1) + (w & 3) * 16384 + q * 512 + ((c ^ q) * 16));
+        *reinterpret_cast<uint2*>(a.dx + (int64_t)(r.row0 + q) * a.H + p0 + c * 4) =
+            make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
     }
 }
 
@@ -478,7 +644,15 @@ bool tiles_fit(const GatedArgs& a) {
            aligned16(a.wu);
 }
 
-constexpr int64_t kFewRows = 256;    // up to here gated_few_kernel
+constexpr int64_t kFillWorkgroups = 256;
+// The kernels for few rows rather than the tiles (7168 x 2048, weights from HBM, us, few against tiles:
+// forward 8 experts of 8 rows 96 / 166, of 32 116 / 175, of 64 152 / 181, one expert of 256 79 / 126, of 512
+// 153 / 127; d rows 8 experts of 32 rows 102 / 110, of 64 146 / 114, one of 256 49 / 80, of 512 93 / 82;
+// 128 experts at 2048 x 768 forward of 4 rows 183 / 222, of 64 269 / 219).
+bool few_rows(int64_t N, int64_t E) { return N <= 256 || N <= 32 * E; }
+// and how many rows of x per workgroup (8 experts of 16 rows: 98 with 16, 101 with 32, 116 with 64;
+// of 64 rows: 238, 178, 152)
+int few_tile(int64_t N, int64_t E) { return N <= 32 || N <= 16 * E ? 16 : N <= 64 || N <= 48 * E ? 32 : 64; }
 
 int64_t grad_bytes(int64_t N, int64_t I) { return forge::ceil_div(2 * N * I, 256) * 256; }
 
@@ -514,15 +688,18 @@ extern "C" int forge_gated_rows(const void* rows, int64_t ldx, const int32_t* of
     hipStream_t st = (hipStream_t)stream;
     forge::KernelTiming timing("gated_rows", st, 4.0 * N * H * I, forge::WORK_FLOPS);
     const bool fast = tiles_fit(a) && aligned16(h) && aligned16(gate_out) && aligned16(up_out);
-    const bool few = fast && N <= kFewRows;
-    const int64_t p_tiles = forge::ceil_div(I, few ? 16 : fast ? 128 : 32);
-    const int q_tile = few ? (N <= 16 ? 16 : N <= 32 ? 32 : 64) : fast ? 256 : 64;
+    const bool few = fast && few_rows(N, E);
+    const int64_t live = N < E ? N : E;                           // experts with rows, at most
+    int split = 1;
+    while (few && split < 8 && forge::ceil_div(I, 128 / split) * live < kFillWorkgroups) split *= 2;
+    const int64_t p_tiles = forge::ceil_div(I, few ? 128 / split : fast ? 128 : 32);
+    const int q_tile = few ? few_tile(N, E) : fast ? 256 : 64;
     const int64_t blocks = forge::ceil_div(p_tiles * forge::ragged_tiles(N, E, q_tile), 8) * 8;
     FORGE_REQUIRE(blocks <= INT32_MAX, "forge_gated_rows: %lld workgroups", (long long)blocks);
     const dim3 grid((unsigned)blocks);
-    if (few && q_tile == 16) gated_few_kernel<1><<<grid, 512, 0, st>>>(a, (int)p_tiles);
-    else if (few && q_tile == 32) gated_few_kernel<2><<<grid, 512, 0, st>>>(a, (int)p_tiles);
-    else if (few) gated_few_kernel<4><<<grid, 512, 0, st>>>(a, (int)p_tiles);
+    if (few && q_tile == 16) gated_few_kernel<1><<<grid, 512, 0, st>>>(a, (int)p_tiles, split);
+    else if (few && q_tile == 32) gated_few_kernel<2><<<grid, 512, 0, st>>>(a, (int)p_tiles, split);
+    else if (few) gated_few_kernel<4><<<grid, 512, 0, st>>>(a, (int)p_tiles, split);
     else if (fast) gated_tile_kernel<FORWARD><<<dim3((unsigned)blocks), 512, 0, st>>>(a, (int)p_tiles, 1);
     else gated_any_kernel<FORWARD><<<dim3((unsigned)blocks), 256, 0, st>>>(a, (int)p_tiles);
     FORGE_LAUNCH_CHECK();
@@ -572,7 +749,10 @@ extern "C" int forge_gated_rows_backward(const void* dh, const float* g, const f
     }
     if (drows && N > 0) {
         forge::KernelTiming timing("gated_drows", st, 4.0 * N * H * I, forge::WORK_FLOPS);
-        if (fast) gated_tile_kernel<DROWS><<<dim3((unsigned)blocks), 512, 0, st>>>(a, (int)h_tiles, 1);
+        if (fast && few_rows(N, E)) {
+            const int64_t p_tiles = forge::ceil_div(H, 128);
+            gated_drows_few_kernel<<<dim3((unsigned)(p_tiles * forge::ragged_tiles(N, E, 32))), 512, 0, st>>>(a, (int)p_tiles);
+        } else if (fast) gated_tile_kernel<DROWS><<<dim3((unsigned)blocks), 512, 0, st>>>(a, (int)h_tiles, 1);
         else gated_any_kernel<DROWS><<<dim3((unsigned)blocks), 256, 0, st>>>(a, (int)h_tiles);
         FORGE_LAUNCH_CHECK();
     }
