@@ -208,7 +208,7 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
     const int64_t we = (int64_t)(r.expert < 0 ? 0 : r.expert) * a.ws;
 
     // loaders
-    InnerLoader lp_in, lq_in;
+    InnerLoader<4> lp_in, lq_in;
     OuterLoader lp_out, lq_out;
     __amdgpu_buffer_rsrc_t dp, dq;
     if constexpr (MODE == FORWARD) {

@@ -5,7 +5,9 @@
 // products are exact; the scale is applied to every group's f32 sum.
 #include "act.h"
 #include "common.h"
-#include "mfma_tile64.h"
+#include "mfma_tile.h"
+
+#include <type_traits>
 
 namespace {
 using forge::act_f32;
@@ -32,21 +34,28 @@ __device__ __forceinline__ void store_y(const Int4Args& a, int m, int r, float v
     a.y[(int64_t)m * a.R + r] = f32_to_bf16_bits(v);
 }
 
+// The low nibble of byte B as a signed 4-bit integer / 16, f32: the instruction's operand is the byte
+// itself (left to itself the compiler shifts every nibble down first)
+template <int B>
+__device__ __forceinline__ uint32_t nibble_of_byte(uint32_t v) {
+    uint32_t r;
+    if constexpr (B == 0) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(r) : "v"(v));
+    else if constexpr (B == 1) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(r) : "v"(v));
+    else if constexpr (B == 2) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(r) : "v"(v));
+    else asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(r) : "v"(v));
+    return r;
+}
 // Eight nibbles of a packed word as bf16 integers -8 .. 7 divided by 16, lowest first.
 // v_cvt_off_f32_i4 gives a signed 4-bit integer / 16 as f32 (the top bit's flip turns offset binary into
 // two's complement), exact in the upper 16 bits: 14 instructions for 8 values.  The factor 16 goes
 // into the scale.
 __device__ __forceinline__ bf16x8_t nibbles(uint32_t word) {
     const uint32_t a = word ^ 0x88888888u, b = a >> 4;
-    uint32_t out[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint32_t lo = __float_as_uint(__builtin_amdgcn_cvt_off_f32_i4((int)(a >> (8 * j))));
-        const uint32_t hi = __float_as_uint(__builtin_amdgcn_cvt_off_f32_i4((int)(b >> (8 * j))));
-        out[j] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
-    }
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    const u32x4 v = {out[0], out[1], out[2], out[3]};
+    const u32x4 v = {__builtin_amdgcn_perm(nibble_of_byte<0>(b), nibble_of_byte<0>(a), 0x07060302u),
+                     __builtin_amdgcn_perm(nibble_of_byte<1>(b), nibble_of_byte<1>(a), 0x07060302u),
+                     __builtin_amdgcn_perm(nibble_of_byte<2>(b), nibble_of_byte<2>(a), 0x07060302u),
+                     __builtin_amdgcn_perm(nibble_of_byte<3>(b), nibble_of_byte<3>(a), 0x07060302u)};
     return __builtin_bit_cast(bf16x8_t, v);
 }
 constexpr float kNibbleUnit = 16.0f;
@@ -163,139 +172,239 @@ __global__ __launch_bounds__(512) void int4_few_kernel(Int4Args a) {
 }
 
 // ---------------------------------------------------------------- many rows of x
-// 256 rows of x by 128 weight rows per workgroup, 64 columns a stage (mfma_tile.h), 8 wavefronts of
-// 64 x 64.  x goes to LDS without registers; the packed words (two per thread and stage) are
-// converted once per workgroup on their way to LDS, a stage ahead of their use.  Every group's sum
-// is formed by itself and folded into the totals with its scale, one fma per output and group:
-// that needs two sets of sums, which is why a wavefront has 64 x 64 outputs and not 128 x 64.
-// FOLD: steps of 16 columns between folds within a stage (4: groups of 64 or more; 2: of 32).
-template <int FOLD>
-__global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles) {
+// 128 rows of x by 256 weight rows per workgroup, 64 columns a stage (mfma_tile.h), 8 wavefronts (2 along
+// x, 4 along the weights) of 64 x 64.  Every group's sum is formed by itself and folded into the totals
+// with its scale, one fma per output and group: that needs two sets of sums, which is why a wavefront
+// has 64 x 64 outputs and not 128 x 64.
+// x and the packed words go to LDS without registers, four stages ahead, the words in runs of 64 bytes
+// (two stages: a lane's own 16 bytes of its weight row, straight into registers, are a request each, and
+// 16 such loads a stage keep the address unit busy longer than the matrix pipe).  A 32 x 16 fragment
+// of W is one word per lane, converted by the wavefront that multiplies by it, a step ahead.  Both
+// wavefronts along x convert the same words; converted once, into LDS, they would cost 16 KB of writes
+// and 64 KB of reads a stage beside x's 64 KB, and the LDS was then the limit.
+// Where groups end is fixed at compile time: 128 columns (two stages) hold FOLDS folds (1: groups of
+// 128 k or a single one; 2: of 64 k; 4: of 32 k).  The first product of a group starts from the
+// constant zero.
+template <int FOLDS>
+__global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles, int m_tiles, bool vec) {
     using namespace forge;
-    constexpr int kWBytes = 128 * kStage * 2;
-    __shared__ __attribute__((aligned(1024))) char X0[kStageBytes], W0[kWBytes], X1[kStageBytes], W1[kWBytes];
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    constexpr int kRows = 128, kXBytes = kRows * kStage * 2;
+    // (the epilogue takes half of the tile's 128 KB in f32 at a time)
+    __shared__ __attribute__((aligned(1024))) char X0[kXBytes], X1[kXBytes], X2[kXBytes], X3[kXBytes], W0[256 * 64], W1[256 * 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wp = wave >> 1, wq = wave & 1;
-    const int b = xcd_tile(blockIdx.x, gridDim.x);
-    const int r0 = (b % r_tiles) * 128, m0 = (b / r_tiles) * kTile;
-    const int rows = a.R - r0 < 128 ? a.R - r0 : 128;
-    const int xrows = a.M - m0 < kTile ? a.M - m0 : kTile;
+    const int wp = wave >> 2, wq = wave & 3;
+    const int tile = xcd_tile(blockIdx.x, r_tiles * m_tiles);
+    if (tile >= r_tiles * m_tiles) return;
+    // runs of 8 tiles of x by all weight tiles
+    const int run = tile / (8 * r_tiles), in_run = tile - run * 8 * r_tiles, wide = min(m_tiles - run * 8, 8);
+    const int r0 = in_run / wide * 256, m0 = (run * 8 + in_run % wide) * kRows;
+    const int rows = min(a.R - r0, 256), xrows = min(a.M - m0, kRows);
     const __amdgpu_buffer_rsrc_t dx = descriptor(a.x + (int64_t)m0 * a.ldx, (uint32_t)(((xrows - 1) * a.ldx + a.C) * 2));
     const __amdgpu_buffer_rsrc_t dw = descriptor(a.w + (int64_t)r0 * a.words, (uint32_t)(rows * a.words * 4));
-    InnerLoader lx;
-    lx.init(wave, lane, a.ldx, xrows, [](int t) { return t; });
-    // this thread's two words of a stage: row threadIdx.x / 4, words 2 (threadIdx.x % 4) and the next
-    const int wrow = threadIdx.x >> 2, wcol = (threadIdx.x & 3) * 2;
-    const uint32_t wat = (uint32_t)((wrow * a.words + wcol) * 4);
-    uint32_t wlds[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) wlds[i] = wrow * 128 + (((wcol + i) ^ ((wrow >> 1) & 7)) * 16);
-    uint32_t word[2];
-    auto fetch = [&](int s) {
-        // words behind the row are a neighbour's (their x is zero) or outside the array (read as zero)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) word[i] = __builtin_amdgcn_raw_buffer_load_b32(dw, (int)(wat + s * 32 + i * 4), 0, 0);
-    };
-    auto convert = [&](char* W) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) *reinterpret_cast<bf16x8_t*>(W + wlds[i]) = nibbles(word[i]);
-    };
-    InnerFragment fx, fw;
+    const __amdgpu_buffer_rsrc_t ds = descriptor(a.scale + (int64_t)r0 * a.G, (uint32_t)(rows * a.G * 4));
+    InnerLoader<2> lx;
+    lx.init(lane, a.ldx, wave * 16);
+    InnerFragment fx;
     fx.init(lane, wp * 2);
-    fw.init(lane, wq * 2);
+
+    const uint32_t sat = (uint32_t)((wq * 64 + lane) * a.G * 4); // lanes 0 .. 31: the first 32 weight rows' scales, 32 .. 63: the others'
+    // Words of two stages: row r at 64 r, its 16-byte piece c (2 (stage % 2) + lane / 32 of the reader) at
+    // c ^ (r / 4 % 4).  What lies behind the row is a neighbour's (its x is zero) or outside the array: the
+    // range check is per word, so a load across the array's end still gets the words inside.
+    const uint32_t wat = (uint32_t)((wave * 32 + lane / 4) * a.words * 4 + (((lane & 3) ^ ((lane >> 4) & 3)) * 16));
+    auto load_words = [&](char* W, int pair) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) load_to_lds(dw, W + (wave * 2 + j) * 1024, wat + (uint32_t)(j * 64 * a.words) + pair * 64);
+    };
+    const uint32_t wfrom = (uint32_t)((wq * 64 + (lane & 31)) * 64);
+    auto read_words = [&](u32x4 (&w)[2], const char* W, int odd) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+            w[n] = *reinterpret_cast<const u32x4*>(W + wfrom + n * 2048 + (((odd * 2 + (lane >> 5)) ^ ((lane >> 2) & 3)) * 16));
+    };
+    // words 0 .. 3 | 4 .. 7 of the two lanes to 0 2 4 6 | 1 3 5 7: word of step s is then 2 s + lane / 32
+    auto spread = [&](u32x4 (&w)[2]) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            auto p = __builtin_amdgcn_permlane32_swap(w[n][0], w[n][1], false, false);
+            auto q = __builtin_amdgcn_permlane32_swap(w[n][2], w[n][3], false, false);
+            w[n][0] = p[0]; w[n][2] = p[1];
+            w[n][1] = q[0]; w[n][3] = q[1];
+        }
+    };
+
     f32x16_t total[2][2], acc[2][2];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) total[t][n][v] = acc[t][n][v] = 0.0f;
-    const float* sp[2];
+            for (int v = 0; v < 16; ++v) total[t][n][v] = 0.0f;
+    // The scales of the four stages of a turn's folds, each asked for when the turn before has used its
+    // place: loads come back in order, so a wait for a young one is a wait for all x and words before it
+    // (asked for two stages ahead they cost half of the kernel's time).
+    constexpr int kFolds = 2 * FOLDS;
+    uint32_t sc[kFolds];
+    int g = 0, k_next = 0, k_end = a.gs;                        // of the group whose scales are asked for next
+    auto scales = [&](int i) {
+        sc[i] = __builtin_amdgcn_raw_buffer_load_b32(ds, (int)(sat + g * 4), 0, 0);
+        k_next += 128 / FOLDS;
+        if (k_next >= k_end && g + 1 < a.G) {                   // (the last group's again behind C)
+            ++g;
+            k_end += a.gs;
+        }
+    };
+    auto fold = [&](int i) {
+        const auto both = __builtin_amdgcn_permlane32_swap(sc[i], sc[i], false, false);
+        const float s2[2] = {__uint_as_float(both[0]), __uint_as_float(both[1])};
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        const int r = r0 + (wq * 2 + n) * 32 + (lane & 31);
-        sp[n] = a.scale + (int64_t)(r < a.R ? r : 0) * a.G;
-    }
-    int g = 0, pos = 0, end = a.gs;                             // group, columns done, where the group ends
-    float sc[2] = {sp[0][0], sp[1][0]};
-    auto fold = [&]() {
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) total[t][n][v] = __builtin_fmaf(s2[n], acc[t][n][v], total[t][n][v]);
+                // here and now: put off, several groups' sums would be alive at once, 64 registers each
+                asm volatile("" : "+v"(total[t][n]));
+            }
+        scales(i);
+    };
+    struct Step {
+        bf16x8_t p[2], q[2];
+    };
+    auto prepare = [&](Step& f, const char* X, int s, const u32x4 (&w)[2]) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) f.p[t] = fx.read(X, t, s);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) f.q[n] = nibbles(w[n][s]);
+    };
+    auto multiply = [&](auto first, const Step& f) {
+        const f32x16_t zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int n = 0; n < 2; ++n)
+                acc[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.p[t], f.q[n], decltype(first)::value ? zero : acc[t][n], 0, 0, 0);
+        // a step's matrix instructions among the next step's reads (and conversions, as the compiler likes)
 #pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    total[t][n][v] = __builtin_fmaf(sc[n], acc[t][n][v], total[t][n][v]);
-                    acc[t][n][v] = 0.0f;
-                }
-    };
-    auto next_group = [&]() {
-        if (++g < a.G) {
-            end = a.C - end < a.gs ? a.C : end + a.gs;
-            sc[0] = sp[0][g];
-            sc[1] = sp[1][g];
+        for (int i = 0; i < 4; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
     };
-    auto multiply = [&](const char* X, const char* W) {
+    Step f, h;
+    // Stage s, the I-th of its turn; the next one's x in Xn.  w: its words (spread), wn: the next stage's;
+    // W: this pair of stages' words, Wn: the next pair's
+    auto one_stage = [&](auto i, int s, char* X, const char* Xn, char* W, const char* Wn, u32x4 (&w)[2], u32x4 (&wn)[2]) {
+        constexpr int I = decltype(i)::value;
+        constexpr bool kFirst = I % 2 == 0 || FOLDS > 1, kLast = I % 2 == 1 || FOLDS > 1;
+        prepare(h, X, 1, w);
+        multiply(std::integral_constant<bool, kFirst>{}, f);
+        prepare(f, X, 2, w);
+        multiply(std::false_type{}, h);
+        if (FOLDS == 4) fold(2 * I);
+        prepare(h, X, 3, w);
+        multiply(std::integral_constant<bool, FOLDS == 4>{}, f);
+        // The next stage's x (and words, if a pair begins) have arrived once no more loads are on their way
+        // than were issued behind them: x of two stages, one pair's words, and the scales of three stages
+        // (FOLDS 1: of every other).
+        constexpr int kScales = FOLDS == 1 ? (I % 2 == 0 ? 2 : 1) : FOLDS == 2 ? 3 : 6;
+        wait_loads_barrier<2 * 2 + 2 + kScales>();
+        lx.stage(dx, X, wave, a.ldx, (s + 4) * kStage, a.C);
+        __builtin_amdgcn_sched_barrier(0);
+        if (I % 2 == 0) {
+            load_words(W, s / 2 + 2);                           // everybody has this pair's in registers
+            __builtin_amdgcn_sched_barrier(0);
+        } else {
+            read_words(wn, Wn, 0);
+            read_words(w, Wn, 1);
+        }
+        spread(wn);
+        prepare(f, Xn, 0, wn);
+        multiply(std::false_type{}, h);
+        if (kLast) fold(FOLDS == 1 ? I / 2 : FOLDS == 2 ? I : 2 * I + 1);
+    };
+    u32x4 w0[2], w1[2];                                         // words of even and odd stages
+    // in the loop's own order
+    lx.stage(dx, X0, wave, a.ldx, 0, a.C);
+    __builtin_amdgcn_sched_barrier(0);
+    load_words(W0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    lx.stage(dx, X1, wave, a.ldx, kStage, a.C);
+    lx.stage(dx, X2, wave, a.ldx, 2 * kStage, a.C);
+    __builtin_amdgcn_sched_barrier(0);
+    load_words(W1, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    lx.stage(dx, X3, wave, a.ldx, 3 * kStage, a.C);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            bf16x8_t p[2], q[2];
+    for (int i = 0; i < kFolds; ++i) scales(i);
+    wait_loads_barrier<8 + kFolds>();
+    read_words(w0, W0, 0);
+    read_words(w1, W0, 1);
+    spread(w0);
+    prepare(f, X0, 0, w0);
+    // (columns behind C are zeros of x times a neighbour's words)
+    const int stages = (a.C + 2 * kStage - 1) / (2 * kStage) * 2;
+    int s = 0;
+    for (; s + 4 <= stages; s += 4) {
+        one_stage(std::integral_constant<int, 0>{}, s, X0, X1, W0, W1, w0, w1);
+        one_stage(std::integral_constant<int, 1>{}, s + 1, X1, X2, W0, W1, w1, w0);
+        one_stage(std::integral_constant<int, 2>{}, s + 2, X2, X3, W1, W0, w0, w1);
+        one_stage(std::integral_constant<int, 3>{}, s + 3, X3, X0, W1, W0, w1, w0);
+    }
+    if (s < stages) {
+        one_stage(std::integral_constant<int, 0>{}, s, X0, X1, W0, W1, w0, w1);
+        one_stage(std::integral_constant<int, 1>{}, s + 1, X1, X2, W0, W1, w1, w0);
+    }
+    wait_loads<0>();
+    __syncthreads();
+    // The tile goes through LDS as f32, 64 rows of x (one row of wavefronts) at a time, so that bias,
+    // residual and y are read and written in runs of 8 columns.  16 rows of 1 KB a buffer.
+    // Register v of a tile: row 8 (v / 4) + 4 (lane / 32) + v % 4 of x, weight row lane & 31.
+    auto quarter = [&](int i) { return reinterpret_cast<float*>(i == 0 ? X0 : i == 1 ? X1 : i == 2 ? X2 : X3); };
 #pragma unroll
-            for (int t = 0; t < 2; ++t) p[t] = fx.read(X, t, s);
-#pragma unroll
-            for (int t = 0; t < 2; ++t) q[t] = fw.read(W, t, s);
+    for (int pass = 0; pass < 2; ++pass) {
+        if (wp == pass) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
-                    acc[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[t], q[n], acc[t][n], 0, 0, 0);
-            if (s % FOLD == FOLD - 1) {
-                pos += 16 * FOLD;
-                if (pos >= end && g < a.G) {
-                    fold();
-                    next_group();
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        quarter(t * 2 + (v >> 3))[(8 * ((v >> 2) & 1) + 4 * (lane >> 5) + (v & 3)) * 256 + (wq * 2 + n) * 32 +
+                                                  (lane & 31)] = total[t][n][v] * kNibbleUnit;
+        }
+        __syncthreads();
+        // 32 threads a row, 16 rows at a time
+        const int c = (threadIdx.x & 31) * 8, r = r0 + c;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int m = m0 + pass * 64 + i * 16 + (threadIdx.x >> 5);
+            if (m >= a.M || r >= a.R) continue;
+            const float* from = quarter(i) + (threadIdx.x >> 5) * 256 + c;
+            if (vec) {
+                float v[8];
+                *reinterpret_cast<f32x4_t*>(v) = *reinterpret_cast<const f32x4_t*>(from);
+                *reinterpret_cast<f32x4_t*>(v + 4) = *reinterpret_cast<const f32x4_t*>(from + 4);
+                uint32_t b[4] = {0, 0, 0, 0}, e[4] = {0, 0, 0, 0};
+                if (a.bias) *reinterpret_cast<uint4*>(b) = *reinterpret_cast<const uint4*>(a.bias + r);
+                if (a.res) *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(a.res + (int64_t)m * a.ldr + r);
+                uint32_t y[4];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    if (a.bias) v[k] += __uint_as_float(k & 1 ? b[k / 2] & 0xFFFF0000u : b[k / 2] << 16);
+                    v[k] = act_f32(a.act, v[k]);
+                    if (a.res) v[k] += __uint_as_float(k & 1 ? e[k / 2] & 0xFFFF0000u : e[k / 2] << 16);
+                    if (k & 1) y[k / 2] = forge::pack_bf16(v[k - 1], v[k]);
                 }
+                *reinterpret_cast<uint4*>(a.y + (int64_t)m * a.R + r) = make_uint4(y[0], y[1], y[2], y[3]);
+            } else {
+                for (int k = 0; k < 8 && r + k < a.R; ++k) store_y(a, m, r + k, from[k]);
             }
         }
-    };
-    const int stages = (a.C + kStage - 1) / kStage;
-    fetch(0);
-    lx.stage(dx, X0, wave, 0, a.C);
-    convert(W0);
-    fetch(1);
-    int s = 0;
-    for (; s + 1 < stages; s += 2) {
-        wait_loads();
         __syncthreads();
-        lx.stage(dx, X1, wave, (s + 1) * kStage, a.C);
-        convert(W1);
-        fetch(s + 2);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(X0, W0);
-        wait_loads();
-        __syncthreads();
-        if (s + 2 < stages) lx.stage(dx, X0, wave, (s + 2) * kStage, a.C);
-        convert(W0);
-        fetch(s + 3);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(X1, W1);
-    }
-    if (s < stages) {
-        wait_loads();
-        __syncthreads();
-        multiply(X0, W0);
-    }
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        const int r = r0 + (wq * 2 + n) * 32 + (lane & 31);
-        if (r >= a.R) continue;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const int m = m0 + (wp * 2 + t) * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3);
-                if (m < a.M) store_y(a, m, r, total[t][n][v] * kNibbleUnit);
-            }
     }
 }
 
@@ -351,6 +460,8 @@ __global__ __launch_bounds__(256) void int4_any_kernel(Int4Args a, int r_tiles) 
     }
 }
 
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
 constexpr int64_t kFewRows = 256;    // up to here int4_few_kernel
 
 template <int MT, int NT>
@@ -387,7 +498,7 @@ extern "C" int forge_linear_int4(const void* x, int64_t ldx, const int32_t* pack
     hipStream_t st = (hipStream_t)stream;
     forge::KernelTiming timing("linear_int4", st, 2.0 * M * C * R, forge::WORK_FLOPS);
     const bool one_group = a.G == 1;
-    const bool pieces = C % 8 == 0 && ldx % 8 == 0 && ldx < (1 << 21) && (reinterpret_cast<uintptr_t>(x) & 15) == 0 &&
+    const bool pieces = C % 8 == 0 && ldx % 8 == 0 && ldx < (1 << 21) && aligned16(x) &&
                         (gs % 32 == 0 || one_group);
     if (!pieces) {
         const int64_t r_tiles = forge::ceil_div(R, 64), blocks = r_tiles * forge::ceil_div(M, 64);
@@ -396,10 +507,14 @@ extern "C" int forge_linear_int4(const void* x, int64_t ldx, const int32_t* pack
     } else if (M <= kFewRows) {
         launch_few(a, one_group, st);
     } else {
-        const int64_t r_tiles = forge::ceil_div(R, 128), blocks = r_tiles * forge::ceil_div(M, 256);
+        const int64_t r_tiles = forge::ceil_div(R, 256), m_tiles = forge::ceil_div(M, 128);
+        const int64_t blocks = forge::ceil_div(r_tiles * m_tiles, 8) * 8;
         FORGE_REQUIRE(blocks <= INT32_MAX, "%s: %lld workgroups", name, (long long)blocks);
-        if (gs % 64 == 0 || one_group) int4_tile_kernel<4><<<dim3((unsigned)blocks), 512, 0, st>>>(a, (int)r_tiles);
-        else int4_tile_kernel<2><<<dim3((unsigned)blocks), 512, 0, st>>>(a, (int)r_tiles);
+        const dim3 grid((unsigned)blocks);
+        const bool vec = R % 8 == 0 && aligned16(y) && aligned16(bias) && aligned16(residual) && (!residual || ldr % 8 == 0);
+        if (gs % 128 == 0 || one_group) int4_tile_kernel<1><<<grid, 512, 0, st>>>(a, (int)r_tiles, (int)m_tiles, vec);
+        else if (gs % 64 == 0) int4_tile_kernel<2><<<grid, 512, 0, st>>>(a, (int)r_tiles, (int)m_tiles, vec);
+        else int4_tile_kernel<4><<<grid, 512, 0, st>>>(a, (int)r_tiles, (int)m_tiles, vec);
     }
     FORGE_LAUNCH_CHECK();
     return FORGE_OK;

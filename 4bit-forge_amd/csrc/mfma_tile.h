@@ -43,7 +43,7 @@ __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t d, char* lds,
 }
 // all but the last N of this wavefront's loads have arrived, and all of its LDS reads (vmcnt(N), lgkmcnt(0))
 template <int N>
-__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15)); }
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14)); }
 // the same, then the workgroup's barrier; nothing the compiler knows of moves across it
 template <int N>
 __device__ __forceinline__ void wait_loads_barrier() {
@@ -56,9 +56,10 @@ __device__ __forceinline__ void wait_loads_barrier() {
 }
 
 // ---- K_INNER: the descriptor covers exactly the valid rows of pitch ld, so that rows behind them are
-// outside its range; the columns from `inner` on are sorted out here.  Load j of a wavefront takes
-// 8 rows, 8 j rows behind its first; its lanes' pieces are those of load 0 for even j, and the
+// outside its range; the columns from `inner` on are sorted out here.  A wavefront has LOADS loads of 8
+// rows (an even number), load j 8 j rows behind its first; its lanes' pieces are those of load 0 for even j, and the
 // others of their 128 bytes (piece ^ 4) for odd j.
+template <int LOADS>
 struct InnerLoader {
     uint32_t off;        // byte offset of this lane's row, load 0
     int piece;           // columns into the stage, load 0
@@ -69,9 +70,9 @@ struct InnerLoader {
     }
     __device__ __forceinline__ void stage(__amdgpu_buffer_rsrc_t d, char* lds, int wave, int64_t ld, int k0, int inner) const {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < LOADS; ++j) {
             const int k = k0 + ((j & 1) ? piece ^ 32 : piece);
-            load_to_lds(d, lds + (wave * 4 + j) * 1024, k < inner ? off + (uint32_t)(k * 2) + (uint32_t)(j * 16 * ld) : kOutside);
+            load_to_lds(d, lds + (wave * LOADS + j) * 1024, k < inner ? off + (uint32_t)(k * 2) + (uint32_t)(j * 16 * ld) : kOutside);
         }
     }
 };
@@ -132,22 +133,26 @@ struct OuterFragment {
     }
 };
 
-// The fragments of one step: 4 of P, 2 of Q
+// The fragments of one step: NP of P, 2 of Q
+template <int NP>
 struct Fragments {
-    bf16x8_t p[4], q[2];
+    bf16x8_t p[NP], q[2];
     template <typename FP, typename FQ>
     __device__ __forceinline__ void read(const char* P, const char* Q, const FP& fp, const FQ& fq, int s) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) q[t] = fq.read(Q, t, s);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) p[t] = fp.read(P, t, s);
+        for (int t = 0; t < NP; ++t) p[t] = fp.read(P, t, s);
     }
-    __device__ __forceinline__ void multiply(f32x16_t (&acc)[4][2]) const {
+    // FIRST: the sums start from zero, which the matrix instruction takes as a constant
+    template <bool FIRST = false>
+    __device__ __forceinline__ void multiply(f32x16_t (&acc)[NP][2]) const {
+        const f32x16_t zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < NP; ++t)
 #pragma unroll
             for (int n = 0; n < 2; ++n)
-                acc[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[t], q[n], acc[t][n], 0, 0, 0);
+                acc[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[t], q[n], FIRST ? zero : acc[t][n], 0, 0, 0);
     }
 };
 
@@ -173,9 +178,9 @@ __device__ __forceinline__ void order_step() {
 // has to assume that a load on its way to LDS may hit what is being read, and waits for it.
 template <typename LOAD, typename FP, typename FQ>
 __device__ __forceinline__ void one_stage(int s, char* P, char* Q, const char* Pn, const char* Qn, LOAD& load,
-                                          const FP& fp, const FQ& fq, Fragments& f, f32x16_t (&acc)[4][2]) {
+                                          const FP& fp, const FQ& fq, Fragments<4>& f, f32x16_t (&acc)[4][2]) {
     constexpr int kReads = 4 * FP::kReads + 2 * FQ::kReads;
-    Fragments g;
+    Fragments<4> g;
     g.read(P, Q, fp, fq, 1);
     f.multiply(acc);
     order_step<kReads, 0>();
@@ -202,7 +207,7 @@ __device__ __forceinline__ void multiply_stages(int stages, char* P0, char* Q0, 
     load(0, P0, Q0);
     load(1, P1, Q1);
     wait_loads_barrier<8>();
-    Fragments f;
+    Fragments<4> f;
     f.read(P0, Q0, fp, fq, 0);
     int s = 0;
     for (; s + 2 <= stages; s += 2) {
