@@ -34,6 +34,21 @@ __device__ __forceinline__ void store_y(const Int4Args& a, int m, int r, float v
     a.y[(int64_t)m * a.R + r] = f32_to_bf16_bits(v);
 }
 
+// the same for 8 columns (R, ldr and the pointers allow 16-byte accesses)
+__device__ __forceinline__ void store_y8(const Int4Args& a, int m, int r, float (&v)[8]) {
+    uint32_t b[4] = {0, 0, 0, 0}, e[4] = {0, 0, 0, 0}, y[4];
+    if (a.bias) *reinterpret_cast<uint4*>(b) = *reinterpret_cast<const uint4*>(a.bias + r);
+    if (a.res) *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(a.res + (int64_t)m * a.ldr + r);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        if (a.bias) v[k] += __uint_as_float(k & 1 ? b[k / 2] & 0xFFFF0000u : b[k / 2] << 16);
+        v[k] = act_f32(a.act, v[k]);
+        if (a.res) v[k] += __uint_as_float(k & 1 ? e[k / 2] & 0xFFFF0000u : e[k / 2] << 16);
+        if (k & 1) y[k / 2] = forge::pack_bf16(v[k - 1], v[k]);
+    }
+    *reinterpret_cast<uint4*>(a.y + (int64_t)m * a.R + r) = make_uint4(y[0], y[1], y[2], y[3]);
+}
+
 // The low nibble of byte B as a signed 4-bit integer / 16, f32: the instruction's operand is the byte
 // itself (left to itself the compiler shifts every nibble down first)
 template <int B>
@@ -61,114 +76,83 @@ __device__ __forceinline__ bf16x8_t nibbles(uint32_t word) {
 constexpr float kNibbleUnit = 16.0f;
 
 // ---------------------------------------------------------------- few rows of x
-// Bound by the packed words, which are read once: a workgroup takes 16 NT weight rows and all of
-// C, its 8 wavefronts every eighth run of 128 columns, and their sums meet in LDS (in a fixed
-// order).  A lane fetches 16 bytes, 32 nibbles, of one weight row, so four lanes fetch 64
-// consecutive bytes of it; exchanging words between the four (two v_permlane32_swap, two
-// v_permlane16_swap) gives every lane the word that the matrix instruction wants of it when each
-// step takes 32 consecutive columns, and then x too is read in 64-byte runs and a step never
-// crosses a group (groups are multiples of 32).  STEPS steps of 32 columns share a scale.  x comes
-// from the caches: MT blocks of 16 rows; rows beyond M and columns beyond C read as zero.
-template <int MT, int NT, int STEPS>
+// Bound by the packed words, which are read once: a workgroup takes 16 weight rows, its 8 wavefronts every
+// eighth run of 128 columns, and their sums meet in LDS (in a fixed order; fewer wavefronts per row and
+// more rows per workgroup were slower at every size, 47 against 34 us at 7168 -> 18432).  A lane fetches
+// 16 bytes, 32 nibbles, of one weight row, so four lanes fetch 64 consecutive bytes of it; exchanging
+// words between the four (two
+// v_permlane32_swap, two v_permlane16_swap) gives every lane the word that the matrix instruction
+// wants of it when each step takes 32 consecutive columns, and then x too is read in 64-byte runs and
+// a step never crosses a group (groups are multiples of 32).  STEPS steps of 32 columns share a
+// scale.  The up to 16 rows of x come from the caches; rows beyond M and columns beyond C read as zero.
+template <int STEPS>
 __global__ __launch_bounds__(512) void int4_few_kernel(Int4Args a) {
     using namespace forge;
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    constexpr int U = MT * NT == 1 ? 4 : MT * NT == 2 ? 2 : 1;      // runs in flight per wavefront
-    constexpr int OUT = MT * NT * 256;
-    __shared__ float part[8][OUT];
+    constexpr int U = 4;                                        // runs in flight per wavefront
+    __shared__ float part[8][256];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, kb = lane >> 4;
-    const int r0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT;
-    const int rows = a.R - r0 < 16 * NT ? a.R - r0 : 16 * NT;
-    const int xrows = a.M - m0 < 16 * MT ? a.M - m0 : 16 * MT;
+    const int r0 = blockIdx.x * 16, rows = min(a.R - r0, 16);
     const __amdgpu_buffer_rsrc_t dw = descriptor(a.w + (int64_t)r0 * a.words, (uint32_t)(rows * a.words * 4));
     const __amdgpu_buffer_rsrc_t ds = descriptor(a.scale + (int64_t)r0 * a.G, (uint32_t)(rows * a.G * 4));
-    const __amdgpu_buffer_rsrc_t dx = descriptor(a.x + (int64_t)m0 * a.ldx, (uint32_t)(((xrows - 1) * a.ldx + a.C) * 2));
-    f32x4_t total[MT][NT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) total[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    const int runs = (a.C + 127) / 128, full = a.words / 16;
+    const __amdgpu_buffer_rsrc_t dx = descriptor(a.x, (uint32_t)(((a.M - 1) * a.ldx + a.C) * 2));
+    f32x4_t total = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int runs = (a.C + 127) / 128;
     for (int c0 = wave; c0 < runs; c0 += 8 * U) {
-        u32x4 w[U][NT], x[U][MT][4];
-        float sc[U][NT][4 / STEPS];
+        u32x4 w[U], x[U][4];
+        float sc[U][4 / STEPS];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int c = c0 + 8 * u;
+            // (words behind the row are a neighbour's, their x is zero, or outside the array)
+            w[u] = __builtin_amdgcn_raw_buffer_load_b128(dw, (n * a.words + c * 16 + kb * 4) * 4, 0, 0);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const uint32_t at = (uint32_t)(((j * 16 + n) * a.words + c * 16 + kb * 4) * 4);
-                if (c < full) {
-                    w[u][j] = __builtin_amdgcn_raw_buffer_load_b128(dw, (int)at, 0, 0);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        w[u][j][i] = __builtin_amdgcn_raw_buffer_load_b32(
-                            dw, c * 16 + kb * 4 + i < a.words ? (int)(at + 4 * i) : (int)kOutside, 0, 0);
-                }
-#pragma unroll
-                for (int i = 0; i < 4 / STEPS; ++i) {
-                    const int k = c * 128 + i * STEPS * 32;
-                    sc[u][j][i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
-                        ds, k < a.C ? ((j * 16 + n) * a.G + k / a.gs) * 4 : (int)kOutside, 0, 0));
-                }
+            for (int i = 0; i < 4 / STEPS; ++i) {
+                const int k = c * 128 + i * STEPS * 32;
+                sc[u][i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                    ds, k < a.C ? (n * a.G + k / a.gs) * 4 : (int)kOutside, 0, 0));
             }
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const int k = c * 128 + d * 32 + kb * 8, m = i * 16 + n;
-                    x[u][i][d] = __builtin_amdgcn_raw_buffer_load_b128(
-                        dx, k < a.C && m < xrows ? (int)((m * a.ldx + k) * 2) : (int)kOutside, 0, 0);
-                }
+            for (int d = 0; d < 4; ++d) {
+                const int k = c * 128 + d * 32 + kb * 8;
+                x[u][d] = __builtin_amdgcn_raw_buffer_load_b128(
+                    dx, k < a.C && n < a.M ? (int)((n * a.ldx + k) * 2) : (int)kOutside, 0, 0);
+            }
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) {
+            u32x4& q = w[u];
+            auto s = __builtin_amdgcn_permlane32_swap(q[0], q[2], false, false);
+            q[0] = s[0]; q[2] = s[1];
+            s = __builtin_amdgcn_permlane32_swap(q[1], q[3], false, false);
+            q[1] = s[0]; q[3] = s[1];
+            s = __builtin_amdgcn_permlane16_swap(q[0], q[1], false, false);
+            q[0] = s[0]; q[1] = s[1];
+            s = __builtin_amdgcn_permlane16_swap(q[2], q[3], false, false);
+            q[2] = s[0]; q[3] = s[1];
+            f32x4_t acc;
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                u32x4& q = w[u][j];
-                auto s = __builtin_amdgcn_permlane32_swap(q[0], q[2], false, false);
-                q[0] = s[0]; q[2] = s[1];
-                s = __builtin_amdgcn_permlane32_swap(q[1], q[3], false, false);
-                q[1] = s[0]; q[3] = s[1];
-                s = __builtin_amdgcn_permlane16_swap(q[0], q[1], false, false);
-                q[0] = s[0]; q[1] = s[1];
-                s = __builtin_amdgcn_permlane16_swap(q[2], q[3], false, false);
-                q[2] = s[0]; q[3] = s[1];
-                f32x4_t acc[MT];
+            for (int d = 0; d < 4; ++d) {
+                if (d % STEPS == 0) acc = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x[u][d]), nibbles(q[d]), acc, 0, 0, 0);
+                if (d % STEPS == STEPS - 1)
 #pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const bf16x8_t wv = nibbles(q[d]);
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        if (d % STEPS == 0) acc[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-                        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x[u][i][d]), wv,
-                                                                         acc[i], 0, 0, 0);
-                        if (d % STEPS == STEPS - 1)
-#pragma unroll
-                            for (int v = 0; v < 4; ++v)
-                                total[i][j][v] = __builtin_fmaf(sc[u][j][d / STEPS], acc[i][v], total[i][j][v]);
-                    }
-                }
+                    for (int v = 0; v < 4; ++v) total[v] = __builtin_fmaf(sc[u][d / STEPS], acc[v], total[v]);
             }
+        }
     }
-    // register v of a 16 x 16 block: row 4 (lane / 16) + v of x, weight row lane & 15
+    // register v: row 4 (lane / 16) + v of x, weight row lane & 15
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) part[wave][((i * 16 + kb * 4 + v) * NT + j) * 16 + n] = total[i][j][v];
+    for (int v = 0; v < 4; ++v) part[wave][(kb * 4 + v) * 16 + n] = total[v];
     __syncthreads();
-    for (int o = threadIdx.x; o < OUT; o += 512) {
-        const int m = m0 + o / (16 * NT), r = r0 + o % (16 * NT);
-        if (m >= a.M || r >= a.R) continue;
-        float v = 0.0f;
+    if (threadIdx.x >= 256) return;
+    const int m = threadIdx.x / 16, r = r0 + threadIdx.x % 16;
+    if (m >= a.M || r >= a.R) return;
+    float v = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v += part[i][o];
-        store_y(a, m, r, v * kNibbleUnit);
-    }
+    for (int w = 0; w < 8; ++w) v += part[w][threadIdx.x];
+    store_y(a, m, r, v * kNibbleUnit);
 }
 
 // ---------------------------------------------------------------- many rows of x
@@ -388,24 +372,215 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles,
                 float v[8];
                 *reinterpret_cast<f32x4_t*>(v) = *reinterpret_cast<const f32x4_t*>(from);
                 *reinterpret_cast<f32x4_t*>(v + 4) = *reinterpret_cast<const f32x4_t*>(from + 4);
-                uint32_t b[4] = {0, 0, 0, 0}, e[4] = {0, 0, 0, 0};
-                if (a.bias) *reinterpret_cast<uint4*>(b) = *reinterpret_cast<const uint4*>(a.bias + r);
-                if (a.res) *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(a.res + (int64_t)m * a.ldr + r);
-                uint32_t y[4];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    if (a.bias) v[k] += __uint_as_float(k & 1 ? b[k / 2] & 0xFFFF0000u : b[k / 2] << 16);
-                    v[k] = act_f32(a.act, v[k]);
-                    if (a.res) v[k] += __uint_as_float(k & 1 ? e[k / 2] & 0xFFFF0000u : e[k / 2] << 16);
-                    if (k & 1) y[k / 2] = forge::pack_bf16(v[k - 1], v[k]);
-                }
-                *reinterpret_cast<uint4*>(a.y + (int64_t)m * a.R + r) = make_uint4(y[0], y[1], y[2], y[3]);
+                store_y8(a, m, r, v);
             } else {
                 for (int k = 0; k < 8 && r + k < a.R; ++k) store_y(a, m, r + k, from[k]);
             }
         }
         __syncthreads();
     }
+}
+
+// ---------------------------------------------------------------- in between
+// Too many rows of x for the kernel above to read them from the caches for every 16 weight rows, too
+// few for 128 x 256 tiles to fill the GPU: 32 PT rows of x by 64 weight rows per workgroup, and each of its 8
+// wavefronts forms all of that tile over every eighth 128 columns (a pair of stages), on LDS buffers of
+// its own, without a barrier; their sums meet in LDS in a fixed order.  The wavefront's inner loop is
+// that of the tiles: x a stage ahead, words a pair ahead, fragments a step ahead.
+template <int PT, int FOLDS>
+__global__ __launch_bounds__(512) void int4_split_kernel(Int4Args a, int r_tiles, int m_tiles, bool vec) {
+    using namespace forge;
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    constexpr int kRows = 32 * PT, kXBytes = kRows * 128;
+    __shared__ __attribute__((aligned(1024))) char XA[8 * kXBytes], XB[8 * kXBytes], W[8 * 4096];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tile = xcd_tile(blockIdx.x, r_tiles * m_tiles);
+    if (tile >= r_tiles * m_tiles) return;
+    const int r0 = tile / m_tiles * 64, m0 = tile % m_tiles * kRows;
+    const int rows = min(a.R - r0, 64), xrows = min(a.M - m0, kRows);
+    const __amdgpu_buffer_rsrc_t dx = descriptor(a.x + (int64_t)m0 * a.ldx, (uint32_t)(((xrows - 1) * a.ldx + a.C) * 2));
+    const __amdgpu_buffer_rsrc_t dw = descriptor(a.w + (int64_t)r0 * a.words, (uint32_t)(rows * a.words * 4));
+    const __amdgpu_buffer_rsrc_t ds = descriptor(a.scale + (int64_t)r0 * a.G, (uint32_t)(rows * a.G * 4));
+    InnerLoader<4 * PT> lx;                                     // as wavefront 0 of a tile of its own
+    lx.init(lane, a.ldx, 0);
+    InnerFragment fx;
+    fx.init(lane, 0);
+    // words of a pair of stages: row r at 64 r, its piece c at c ^ (r / 4 % 4)
+    const uint32_t wat = (uint32_t)((lane / 4) * a.words * 4 + (((lane & 3) ^ ((lane >> 4) & 3)) * 16));
+    const uint32_t wfrom = (uint32_t)(wave * 4096 + (lane & 31) * 64);
+    char *const xa = XA + wave * kXBytes, *const xb = XB + wave * kXBytes;
+    auto load_x = [&](char* X, int k) { lx.stage(dx, X, 0, a.ldx, k, a.C); };
+    auto load_words = [&](int pair) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) load_to_lds(dw, W + wave * 4096 + j * 1024, wat + (uint32_t)(j * 64 * a.words) + pair * 64);
+    };
+    auto read_words = [&](u32x4 (&w)[2], int odd) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            w[n] = *reinterpret_cast<const u32x4*>(W + wfrom + n * 2048 + (((odd * 2 + (lane >> 5)) ^ ((lane >> 2) & 3)) * 16));
+        }
+    };
+    auto spread = [&](u32x4 (&w)[2]) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            auto p = __builtin_amdgcn_permlane32_swap(w[n][0], w[n][1], false, false);
+            auto q = __builtin_amdgcn_permlane32_swap(w[n][2], w[n][3], false, false);
+            w[n][0] = p[0]; w[n][2] = p[1];
+            w[n][1] = q[0]; w[n][3] = q[1];
+        }
+    };
+    f32x16_t total[PT][2], acc[PT][2];
+#pragma unroll
+    for (int t = 0; t < PT; ++t)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) total[t][n][v] = 0.0f;
+    const uint32_t sat = (uint32_t)(lane * a.G * 4);
+    auto scales = [&](uint32_t (&sc)[FOLDS], int pair) {
+        int g = pair * 128 / a.gs, into = pair * 128 - g * a.gs;
+#pragma unroll
+        for (int i = 0; i < FOLDS; ++i) {
+            sc[i] = __builtin_amdgcn_raw_buffer_load_b32(ds, (int)(sat + min(g, a.G - 1) * 4), 0, 0);
+            into += 128 / FOLDS;
+            if (into >= a.gs) {
+                into -= a.gs;
+                ++g;
+            }
+        }
+    };
+    auto fold = [&](uint32_t s) {
+        const auto both = __builtin_amdgcn_permlane32_swap(s, s, false, false);
+        const float s2[2] = {__uint_as_float(both[0]), __uint_as_float(both[1])};
+#pragma unroll
+        for (int t = 0; t < PT; ++t)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) total[t][n][v] = __builtin_fmaf(s2[n], acc[t][n][v], total[t][n][v]);
+                asm volatile("" : "+v"(total[t][n]));           // here and now, as above
+            }
+    };
+    struct Step {
+        bf16x8_t p[PT], q[2];
+    };
+    auto prepare = [&](Step& f, const char* X, int s, const u32x4 (&w)[2]) {
+#pragma unroll
+        for (int t = 0; t < PT; ++t) f.p[t] = fx.read(X, t, s);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) f.q[n] = nibbles(w[n][s]);
+    };
+    auto multiply = [&](auto first, const Step& f) {
+        const f32x16_t zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < PT; ++t)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+                acc[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.p[t], f.q[n], decltype(first)::value ? zero : acc[t][n], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // this wavefront's LDS reads are back, and all but the last N of its loads have arrived
+    auto arrived = [](auto n) {
+        constexpr int N = decltype(n)::value;
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        wait_loads<N>();
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+    };
+    Step f, h;
+    u32x4 w0[2], w1[2];
+    uint32_t sc[FOLDS], sn[FOLDS];
+    const int pairs = (a.C + 127) / 128;
+    if (wave < pairs) {
+        load_words(wave);
+        __builtin_amdgcn_sched_barrier(0);
+        scales(sc, wave);
+        __builtin_amdgcn_sched_barrier(0);
+        load_x(xa, wave * 128);
+        __builtin_amdgcn_sched_barrier(0);
+        load_x(xb, wave * 128 + 64);
+        arrived(std::integral_constant<int, 4 * PT>{});
+        read_words(w0, 0);
+        read_words(w1, 1);
+        spread(w0);
+        prepare(f, xa, 0, w0);
+        // (what lies behind the last pair is fetched as zeros of x)
+        for (int p = wave; p < pairs; p += 8) {
+            prepare(h, xa, 1, w0);
+            multiply(std::true_type{}, f);
+            prepare(f, xa, 2, w0);
+            multiply(std::false_type{}, h);
+            if (FOLDS == 4) fold(sc[0]);
+            prepare(h, xa, 3, w0);
+            multiply(std::integral_constant<bool, FOLDS == 4>{}, f);
+            arrived(std::integral_constant<int, 63>{});         // the reads: words and xa are free
+            load_words(p + 8);
+            __builtin_amdgcn_sched_barrier(0);
+            scales(sn, p + 8);
+            __builtin_amdgcn_sched_barrier(0);
+            load_x(xa, (p + 8) * 128);
+            arrived(std::integral_constant<int, 4 + FOLDS + 4 * PT>{});      // xb
+            spread(w1);
+            prepare(f, xb, 0, w1);
+            multiply(std::false_type{}, h);
+            if (FOLDS > 1) fold(sc[FOLDS == 2 ? 0 : 1]);
+            prepare(h, xb, 1, w1);
+            multiply(std::integral_constant<bool, (FOLDS > 1)>{}, f);
+            prepare(f, xb, 2, w1);
+            multiply(std::false_type{}, h);
+            if (FOLDS == 4) fold(sc[FOLDS / 2]);
+            prepare(h, xb, 3, w1);
+            multiply(std::integral_constant<bool, FOLDS == 4>{}, f);
+            arrived(std::integral_constant<int, 63>{});
+            load_x(xb, (p + 8) * 128 + 64);
+            arrived(std::integral_constant<int, 4 * PT>{});     // the next pair's words, scales and xa
+            read_words(w0, 0);
+            read_words(w1, 1);
+            spread(w0);
+            prepare(f, xa, 0, w0);
+            multiply(std::false_type{}, h);
+            fold(sc[FOLDS - 1]);
+#pragma unroll
+            for (int i = 0; i < FOLDS; ++i) sc[i] = sn[i];
+        }
+        wait_loads<0>();
+    }
+    // partial sums [row of x][64 weight rows], 256 bytes a row, half of the rows in either buffer of the
+    // wavefront's own.  Register v of a tile: row 8 (v / 4) + 4 (lane / 32) + v % 4 of x, weight row lane & 31.
+#pragma unroll
+    for (int t = 0; t < PT; ++t)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const int m = t * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3);
+                char* half = PT == 2 ? (t ? xb : xa) : (v >> 3 ? xb : xa);
+                reinterpret_cast<float*>(half)[m % (kRows / 2) * 64 + n * 32 + (lane & 31)] = total[t][n][v];
+            }
+    __syncthreads();
+    // 8 threads a row of x
+    const int m = threadIdx.x >> 3, c = (threadIdx.x & 7) * 8, r = r0 + c;
+    if (m >= xrows || r >= a.R) return;
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+    const char* from = (m < kRows / 2 ? XA : XB) + (m % (kRows / 2) * 64 + c) * 4;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+        const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(from + w * kXBytes);
+        const f32x4_t hi = *reinterpret_cast<const f32x4_t*>(from + w * kXBytes + 16);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            v[k] += lo[k];
+            v[k + 4] += hi[k];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] *= kNibbleUnit;
+    if (vec) store_y8(a, m0 + m, r, v);
+    else
+        for (int k = 0; k < 8 && r + k < a.R; ++k) store_y(a, m0 + m, r + k, v[k]);
 }
 
 // Any shape, alignment and group size: 64 x 64 outputs per workgroup, four wavefronts of 32 x 32,
@@ -462,19 +637,29 @@ __global__ __launch_bounds__(256) void int4_any_kernel(Int4Args a, int r_tiles) 
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-constexpr int64_t kFewRows = 256;    // up to here int4_few_kernel
+// Which kernel (us, C = 7168, R = 4096; 256 workgroups run at a time).  int4_few_kernel, for a few rows of x:
+// 1 row 12 against 20 of int4_split_kernel<1>, 16 rows 16 / 21.
+constexpr int64_t kFewRows = 16;
+// int4_split_kernel with 32 rows while its workgroups run at once: 128 rows 21 against 27 with 64 rows, 256
+// rows 39 / 29.  And int4_tile_kernel when that one's workgroups would take their turns: 512 rows (512
+// workgroups) 51 against 109, 1024 rows 100 / 118, 2048 rows 265 / 131; R = 7168, C = 2048 512 rows (896) 42 / 42.
+constexpr int64_t kAtOnce = 256, kSplitWorkgroups = 896;
+int64_t split_workgroups(int64_t M, int64_t R, int64_t rows) { return forge::ceil_div(R, 64) * forge::ceil_div(M, rows); }
 
-template <int MT, int NT>
-void launch_steps(const Int4Args& a, bool one_group, hipStream_t st) {
-    const dim3 grid((unsigned)forge::ceil_div(a.R, 16 * NT), (unsigned)forge::ceil_div(a.M, 16 * MT));
-    if (a.gs % 128 == 0 || one_group) int4_few_kernel<MT, NT, 4><<<grid, 512, 0, st>>>(a);
-    else if (a.gs % 64 == 0) int4_few_kernel<MT, NT, 2><<<grid, 512, 0, st>>>(a);
-    else int4_few_kernel<MT, NT, 1><<<grid, 512, 0, st>>>(a);
+template <int PT>
+void launch_split(const Int4Args& a, bool one_group, bool vec, hipStream_t st) {
+    const int r_tiles = (int)forge::ceil_div(a.R, 64), m_tiles = (int)forge::ceil_div(a.M, 32 * PT);
+    const dim3 grid((unsigned)(forge::ceil_div((int64_t)r_tiles * m_tiles, 8) * 8));
+    if (a.gs % 128 == 0 || one_group) int4_split_kernel<PT, 1><<<grid, 512, 0, st>>>(a, r_tiles, m_tiles, vec);
+    else if (a.gs % 64 == 0) int4_split_kernel<PT, 2><<<grid, 512, 0, st>>>(a, r_tiles, m_tiles, vec);
+    else int4_split_kernel<PT, 4><<<grid, 512, 0, st>>>(a, r_tiles, m_tiles, vec);
 }
+
 void launch_few(const Int4Args& a, bool one_group, hipStream_t st) {
-    if (a.M <= 16) launch_steps<1, 1>(a, one_group, st);
-    else if (a.M <= 32) launch_steps<2, 1>(a, one_group, st);
-    else launch_steps<4, 1>(a, one_group, st);
+    const dim3 grid((unsigned)forge::ceil_div(a.R, 16));
+    if (a.gs % 128 == 0 || one_group) int4_few_kernel<4><<<grid, 512, 0, st>>>(a);
+    else if (a.gs % 64 == 0) int4_few_kernel<2><<<grid, 512, 0, st>>>(a);
+    else int4_few_kernel<1><<<grid, 512, 0, st>>>(a);
 }
 }  // namespace
 
@@ -500,18 +685,22 @@ extern "C" int forge_linear_int4(const void* x, int64_t ldx, const int32_t* pack
     const bool one_group = a.G == 1;
     const bool pieces = C % 8 == 0 && ldx % 8 == 0 && ldx < (1 << 21) && aligned16(x) &&
                         (gs % 32 == 0 || one_group);
+    const bool vec = R % 8 == 0 && aligned16(y) && aligned16(bias) && aligned16(residual) && (!residual || ldr % 8 == 0);
     if (!pieces) {
         const int64_t r_tiles = forge::ceil_div(R, 64), blocks = r_tiles * forge::ceil_div(M, 64);
         FORGE_REQUIRE(blocks <= INT32_MAX, "%s: %lld workgroups", name, (long long)blocks);
         int4_any_kernel<<<dim3((unsigned)blocks), 256, 0, st>>>(a, (int)r_tiles);
     } else if (M <= kFewRows) {
         launch_few(a, one_group, st);
+    } else if (split_workgroups(M, R, 32) <= kAtOnce) {
+        launch_split<1>(a, one_group, vec, st);
+    } else if (split_workgroups(M, R, 64) <= kSplitWorkgroups) {
+        launch_split<2>(a, one_group, vec, st);
     } else {
         const int64_t r_tiles = forge::ceil_div(R, 256), m_tiles = forge::ceil_div(M, 128);
         const int64_t blocks = forge::ceil_div(r_tiles * m_tiles, 8) * 8;
         FORGE_REQUIRE(blocks <= INT32_MAX, "%s: %lld workgroups", name, (long long)blocks);
         const dim3 grid((unsigned)blocks);
-        const bool vec = R % 8 == 0 && aligned16(y) && aligned16(bias) && aligned16(residual) && (!residual || ldr % 8 == 0);
         if (gs % 128 == 0 || one_group) int4_tile_kernel<1><<<grid, 512, 0, st>>>(a, (int)r_tiles, (int)m_tiles, vec);
         else if (gs % 64 == 0) int4_tile_kernel<2><<<grid, 512, 0, st>>>(a, (int)r_tiles, (int)m_tiles, vec);
         else int4_tile_kernel<4><<<grid, 512, 0, st>>>(a, (int)r_tiles, (int)m_tiles, vec);
