@@ -40,124 +40,13 @@ struct GatedArgs {
 
 enum { FORWARD = 0, DROWS = 1, DWEIGHTS = 2 };
 
-// ---------------------------------------------------------------- any shape, any alignment
-// 64 x 64 outputs per workgroup, four wavefronts of 32 x 32, 32 of the inner dimension a step
-// through LDS, every element loaded by itself under its own bounds: what takes the calls whose
-// rows are not 16-byte aligned.
-//   FORWARD   P = weight rows (32 of Wg above the same 32 of Wu), Q = rows,         inner H
-//   DROWS     P = columns of X, Q = rows,                                           inner I, twice
-//   DWEIGHTS  P = columns of X, Q = rows of dW,                                     inner the expert's rows
-// P runs along the registers of the accumulator, i.e. along the output's contiguous dimension.
-template <int MODE>
-__global__ __launch_bounds__(256) void gated_any_kernel(GatedArgs a, int p_tiles) {
-    constexpr int T = 64, K = 32, LD = K + 8;
-    __shared__ uint16_t P[T][LD], Q[T][LD];
-    __shared__ int slot[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wp = wave >> 1, wq = wave & 1;
-    const int pt = blockIdx.x % p_tiles, qt = blockIdx.x / p_tiles;
-
-    RaggedTile r;
-    int q0 = 0, expert, inner, phases = 1;
-    const uint16_t* dgu = nullptr;
-    uint16_t* dw = nullptr;
-    if constexpr (MODE == DWEIGHTS) {
-        const int i_tiles = (a.I + T - 1) / T;
-        const int which = blockIdx.z;
-        expert = blockIdx.y;
-        q0 = qt * T;
-        if (qt >= i_tiles) return;
-        r.expert = expert;
-        r.row0 = forge::clamp_offset(a.offsets, expert, 0, a.N);
-        r.rows = forge::clamp_offset(a.offsets, expert + 1, r.row0, a.N) - r.row0;
-        inner = r.rows;
-        dgu = which ? a.du : a.dg;
-        dw = which ? a.dwu : a.dwg;
-    } else {
-        if (!find_tile(a.offsets, a.E, a.N, T, [=](int) { return qt; }, r, slot)) return;
-        expert = r.expert;
-        inner = expert < 0 ? 0 : (MODE == FORWARD ? a.H : a.I);
-        phases = MODE == DROWS ? 2 : 1;
-    }
-    const int64_t wbase = (int64_t)(expert < 0 ? 0 : expert) * a.ws;
-    const int p0 = pt * (MODE == FORWARD ? T / 2 : T);
-
-    f32x16_t acc;
-#pragma unroll
-    for (int v = 0; v < 16; ++v) acc[v] = 0.0f;
-    for (int ph = 0; ph < phases; ++ph)
-        for (int k0 = 0; k0 < inner; k0 += K) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < T * K; i += 256) {
-                // neighbouring threads along whichever index is contiguous in memory
-                int row, k;
-                if (MODE == FORWARD) { k = i % K; row = i / K; } else { row = i % T; k = i / T; }
-                uint16_t v = 0;
-                if (k0 + k < inner) {
-                    if constexpr (MODE == FORWARD) {
-                        const int w = p0 + (row & 31);
-                        if (w < a.I) v = (row < 32 ? a.wg : a.wu)[wbase + (int64_t)w * a.ldw + k0 + k];
-                    } else if constexpr (MODE == DROWS) {
-                        if (p0 + row < a.H) v = (ph ? a.wu : a.wg)[wbase + (int64_t)(k0 + k) * a.ldw + p0 + row];
-                    } else {
-                        if (p0 + row < a.H) v = a.x[(int64_t)(r.row0 + k0 + k) * a.ldx + p0 + row];
-                    }
-                }
-                P[row][k] = v;
-                int qr, qk;
-                if (MODE != DWEIGHTS) { qk = i % K; qr = i / K; } else { qr = i % T; qk = i / T; }
-                v = 0;
-                if (k0 + qk < inner) {
-                    if constexpr (MODE == FORWARD) {
-                        if (qr < r.rows) v = a.x[(int64_t)(r.row0 + qr) * a.ldx + k0 + qk];
-                    } else if constexpr (MODE == DROWS) {
-                        if (qr < r.rows) v = (ph ? a.du : a.dg)[(int64_t)(r.row0 + qr) * a.I + k0 + qk];
-                    } else {
-                        if (q0 + qr < a.I) v = dgu[(int64_t)(r.row0 + k0 + qk) * a.I + q0 + qr];
-                    }
-                }
-                Q[qr][qk] = v;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int s = 0; s < K; s += 16) {
-                // FORWARD: this wavefront's 32 P rows are 16 of Wg and the same 16 of Wu
-                const int pr = MODE == FORWARD ? ((lane & 31) < 16 ? wp * 16 + (lane & 15) : 32 + wp * 16 + (lane & 15))
-                                               : wp * 32 + (lane & 31);
-                const bf16x8_t pv = *reinterpret_cast<const bf16x8_t*>(&P[pr][s + 8 * (lane >> 5)]);
-                const bf16x8_t qv = *reinterpret_cast<const bf16x8_t*>(&Q[wq * 32 + (lane & 31)][s + 8 * (lane >> 5)]);
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(pv, qv, acc, 0, 0, 0);
-            }
-        }
-    // register v of the accumulator: row 8 (v >> 2) + 4 (lane >> 5) + (v & 3) of P, column lane & 31 of Q
-    const int q = wq * 32 + (lane & 31);
-    if constexpr (MODE == FORWARD) {
-        if (q >= r.rows) return;
-#pragma unroll
-        for (int v = 0; v < 8; ++v) {                  // rows 0..15: gate, 16..31: up (registers v and v + 8)
-            const int i = p0 + wp * 16 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3);
-            if (i >= a.I) continue;
-            const int64_t at = (int64_t)(r.row0 + q) * a.I + i;
-            a.h[at] = f32_to_bf16_bits(act_f32(a.act, acc[v]) * acc[v + 8]);
-            if (a.g) {
-                a.g[at] = acc[v];
-                a.u[at] = acc[v + 8];
-            }
-        }
-    } else {
-        if (MODE == DROWS ? q >= r.rows : q0 + q >= a.I) return;
-        uint16_t* out = MODE == DROWS ? a.dx + (int64_t)(r.row0 + q) * a.H
-                                      : dw + ((int64_t)expert * a.I + q0 + q) * a.H;
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-            const int c = p0 + wp * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3);
-            if (c < a.H) out[c] = f32_to_bf16_bits(acc[v]);
-        }
-    }
-}
-
-// ---------------------------------------------------------------- 16-byte aligned rows
-// 256 x 256 outputs per workgroup (mfma_tile.h); roles of P and Q as above, with
+// ---------------------------------------------------------------- many rows
+// 256 x 256 outputs per workgroup (mfma_tile.h).  P runs along the registers of the accumulator, i.e. along
+// the output's contiguous dimension, Q across the lanes:
+//   FORWARD   P = weight rows, Q = rows of X,              inner dimension H
+//   DROWS     P = columns of X, Q = rows of X,             inner I, twice
+//   DWEIGHTS  P = columns of X, Q = rows of dW,            inner the expert's rows
+// with
 //   FORWARD   P = 128 features: tile rows 128 w .. + 63 are Wg's rows 64 w .., the next 64 Wu's, so
 //             that wavefront w of P holds g and u of the same features in the same lanes and the
 //             activation and the product need no exchange
@@ -590,24 +479,9 @@ __global__ __launch_bounds__(512) void gated_drows_few_kernel(GatedArgs a, int p
     }
 }
 
-// dg and du from g, u and dh, rounded to bf16 once (they are operands of the two products);
-// one element per thread
-__global__ __launch_bounds__(256) void gated_grad_kernel(const uint16_t* __restrict__ dh,
-                                                         const float* __restrict__ g,
-                                                         const float* __restrict__ u,
-                                                         uint16_t* __restrict__ dg,
-                                                         uint16_t* __restrict__ du, int64_t n, int act) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    float va, vd;
-    act_grad_f32(act, g[i], va, vd);
-    const float d = forge::bf16_bits_to_f32(dh[i]);
-    dg[i] = f32_to_bf16_bits(d * u[i] * vd);
-    du[i] = f32_to_bf16_bits(d * va);
-}
-
-// the same for runs of 8 (N * I a multiple of 8, 16-byte aligned): 14 bytes moved per element
-__global__ __launch_bounds__(256) void gated_grad8_kernel(const uint4* __restrict__ dh,
+// dg and du from g, u and dh, rounded to bf16 once (they are operands of the two products), 8 elements
+// per thread: 14 bytes moved per element
+__global__ __launch_bounds__(256) void gated_grad_kernel(const uint4* __restrict__ dh,
                                                           const f32x4_t* __restrict__ g,
                                                           const f32x4_t* __restrict__ u, uint4* __restrict__ dg,
                                                           uint4* __restrict__ du, int64_t n8, int act) {
@@ -637,13 +511,6 @@ __global__ __launch_bounds__(256) void gated_grad8_kernel(const uint4* __restric
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// what gated_tile_kernel takes: 16-byte pieces everywhere, row offsets of a tile within 31 bits
-bool tiles_fit(const GatedArgs& a) {
-    return a.H % 8 == 0 && a.I % 8 == 0 && a.ldx % 8 == 0 && a.ldw % 8 == 0 && (a.E == 1 || a.ws % 8 == 0) &&
-           a.ldx < (1 << 21) && a.ldw < (1 << 21) && a.I < (1 << 21) && aligned16(a.x) && aligned16(a.wg) &&
-           aligned16(a.wu);
-}
-
 constexpr int64_t kFillWorkgroups = 256;
 // The kernels for few rows rather than the tiles (7168 x 2048, weights from HBM, us, few against tiles:
 // forward 8 experts of 8 rows 96 / 166, of 32 116 / 175, of 64 152 / 181, one expert of 256 79 / 126, of 512
@@ -656,30 +523,91 @@ int few_tile(int64_t N, int64_t E) { return N <= 32 || N <= 16 * E ? 16 : N <= 6
 
 int64_t grad_bytes(int64_t N, int64_t I) { return forge::ceil_div(2 * N * I, 256) * 256; }
 
+// out[b][r][c] = in[b][r][c], zeros behind the last row and column; 8 elements per thread.  Rows start
+// anywhere: an odd element's 16 bytes are put together from the five 4-byte words they lie across.
+__global__ __launch_bounds__(256) void pad_rows_kernel(const uint16_t* __restrict__ in, int64_t stride, int64_t ld,
+                                                       uint4* __restrict__ out, int R, int C, int Rp, int Cp8,
+                                                       const int32_t* __restrict__ offsets) {
+    const int b = blockIdx.y;
+    if (offsets && offsets[b] >= offsets[b + 1]) return;         // nobody reads this one
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (int64_t)Rp * Cp8) return;
+    const int r = (int)(i / Cp8), c = (int)(i - (int64_t)r * Cp8) * 8;
+    uint32_t v[4] = {0, 0, 0, 0};
+    if (r < R && c < C) {
+        const uint16_t* p = in + b * stride + (int64_t)r * ld + c;
+        const bool odd = (reinterpret_cast<uintptr_t>(p) & 2) != 0;
+        if (c + 8 <= C && !odd) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = reinterpret_cast<const uint32_t*>(p)[j];
+        } else if (c > 0 && c + 8 < C) {                          // the words' other halves are the row's own
+            const uint32_t* q = reinterpret_cast<const uint32_t*>(p - 1);
+            uint32_t w = q[0];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t next = q[j + 1];
+                v[j] = w >> 16 | next << 16;
+                w = next;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c + j < C) v[j / 2] |= (uint32_t)p[j] << (16 * (j & 1));
+        }
+    }
+    out[(int64_t)b * Rp * Cp8 + i] = make_uint4(v[0], v[1], v[2], v[3]);
+}
+
 int check(const char* name, const void* rows, int64_t ldx, const int32_t* offsets, const void* Wg,
           const void* Wu, int64_t ldw, int64_t w_stride, int64_t N, int64_t E, int64_t H, int64_t I, int act) {
     FORGE_REQUIRE(N >= 0 && E >= 1 && H >= 1 && I >= 1, "%s: N=%lld E=%lld H=%lld I=%lld", name, (long long)N,
                   (long long)E, (long long)H, (long long)I);
-    FORGE_REQUIRE(N <= (1 << 30) && E <= 65535 && H <= (1 << 22) && I <= (1 << 22),
-                  "%s: N=%lld E=%lld H=%lld I=%lld: too large (N < 2^30, E < 2^16, H and I up to 2^22)", name,
-                  (long long)N, (long long)E, (long long)H, (long long)I);
+    FORGE_REQUIRE(N <= (1 << 30) && E <= 65535 && H < (1 << 21) && I < (1 << 21) && ldx < (1 << 21) && ldw < (1 << 21),
+                  "%s: N=%lld E=%lld H=%lld I=%lld: too large (N up to 2^30, E below 2^16, H, I and the row pitches below 2^21)",
+                  name, (long long)N, (long long)E, (long long)H, (long long)I);
     FORGE_REQUIRE(act >= FORGE_ACT_NONE && act <= FORGE_ACT_RELU, "%s: act=%d", name, act);
     FORGE_REQUIRE(offsets && Wg && Wu && (rows || N == 0), "%s: null pointer", name);
     FORGE_REQUIRE(ldx >= H && ldw >= H && (E == 1 || w_stride >= I * ldw),
                   "%s: row pitch %lld / %lld below H=%lld or expert stride %lld below I rows", name,
                   (long long)ldx, (long long)ldw, (long long)H, (long long)w_stride);
+    FORGE_REQUIRE(H % 8 == 0 && I % 8 == 0 && ldx % 8 == 0 && ldw % 8 == 0 && (E == 1 || w_stride % 8 == 0) &&
+                      aligned16(rows) && aligned16(Wg) && aligned16(Wu),
+                  "%s: H=%lld, I=%lld, pitches and strides must be multiples of 8 elements and pointers 16-byte aligned "
+                  "(forge_pad_rows makes such copies)", name, (long long)H, (long long)I);
     return FORGE_OK;
 }
 }  // namespace
+
+extern "C" int forge_pad_rows(const void* in, int64_t stride, int64_t ld, void* out, int64_t batch, int64_t R,
+                              int64_t C, int64_t Rp, int64_t Cp, const int32_t* offsets, forge_stream_t stream) {
+    const char* name = "forge_pad_rows";
+    FORGE_REQUIRE(batch >= 0 && R >= 0 && C >= 1 && Rp >= R && Cp >= C && Cp % 8 == 0,
+                  "%s: batch=%lld R=%lld C=%lld Rp=%lld Cp=%lld", name, (long long)batch, (long long)R, (long long)C,
+                  (long long)Rp, (long long)Cp);
+    FORGE_REQUIRE(batch <= 65535 && Rp < (1 << 30) && Cp < (1 << 24) && Rp * Cp / 8 <= (int64_t)INT32_MAX * 256,
+                  "%s: batch=%lld Rp=%lld Cp=%lld: too large", name, (long long)batch, (long long)Rp, (long long)Cp);
+    if (batch == 0 || Rp == 0) return FORGE_OK;
+    FORGE_REQUIRE(in && out, "%s: null pointer", name);
+    FORGE_REQUIRE(aligned16(out) && (reinterpret_cast<uintptr_t>(in) & 1) == 0, "%s: out not 16-byte aligned", name);
+    FORGE_REQUIRE(ld >= C, "%s: row pitch %lld below C=%lld", name, (long long)ld, (long long)C);
+    hipStream_t st = (hipStream_t)stream;
+    forge::KernelTiming timing("pad_rows", st, 2.0 * batch * (R * C + Rp * Cp), forge::WORK_BYTES);
+    pad_rows_kernel<<<dim3((unsigned)forge::ceil_div(Rp * Cp / 8, 256), (unsigned)batch), 256, 0, st>>>(
+        (const uint16_t*)in, stride, ld, (uint4*)out, (int)R, (int)C, (int)Rp, (int)(Cp / 8), offsets);
+    FORGE_LAUNCH_CHECK();
+    return FORGE_OK;
+}
 
 extern "C" int forge_gated_rows(const void* rows, int64_t ldx, const int32_t* offsets, const void* Wg,
                                 const void* Wu, int64_t ldw, int64_t w_stride, int64_t N, int64_t E,
                                 int64_t H, int64_t I, int act, void* h, float* gate_out, float* up_out,
                                 forge_stream_t stream) {
-    if (int rc = check("forge_gated_rows", rows, ldx, offsets, Wg, Wu, ldw, w_stride, N, E, H, I, act)) return rc;
+    const char* name = "forge_gated_rows";
+    if (int rc = check(name, rows, ldx, offsets, Wg, Wu, ldw, w_stride, N, E, H, I, act)) return rc;
     if (N == 0) return FORGE_OK;
-    FORGE_REQUIRE(h, "forge_gated_rows: null pointer");
-    FORGE_REQUIRE((gate_out == nullptr) == (up_out == nullptr), "forge_gated_rows: gate_out and up_out go together");
+    FORGE_REQUIRE(h, "%s: null pointer", name);
+    FORGE_REQUIRE((gate_out == nullptr) == (up_out == nullptr), "%s: gate_out and up_out go together", name);
+    FORGE_REQUIRE(aligned16(h) && aligned16(gate_out) && aligned16(up_out), "%s: outputs not 16-byte aligned", name);
     GatedArgs a{};
     a.x = (const uint16_t*)rows; a.offsets = offsets; a.wg = (const uint16_t*)Wg; a.wu = (const uint16_t*)Wu;
     a.ldx = ldx; a.ldw = ldw; a.ws = w_stride;
@@ -687,21 +615,19 @@ extern "C" int forge_gated_rows(const void* rows, int64_t ldx, const int32_t* of
     a.h = (uint16_t*)h; a.g = gate_out; a.u = up_out;
     hipStream_t st = (hipStream_t)stream;
     forge::KernelTiming timing("gated_rows", st, 4.0 * N * H * I, forge::WORK_FLOPS);
-    const bool fast = tiles_fit(a) && aligned16(h) && aligned16(gate_out) && aligned16(up_out);
-    const bool few = fast && few_rows(N, E);
+    const bool few = few_rows(N, E);
     const int64_t live = N < E ? N : E;                           // experts with rows, at most
     int split = 1;
     while (few && split < 8 && forge::ceil_div(I, 128 / split) * live < kFillWorkgroups) split *= 2;
-    const int64_t p_tiles = forge::ceil_div(I, few ? 128 / split : fast ? 128 : 32);
-    const int q_tile = few ? few_tile(N, E) : fast ? 256 : 64;
+    const int64_t p_tiles = forge::ceil_div(I, few ? 128 / split : 128);
+    const int q_tile = few ? few_tile(N, E) : 256;
     const int64_t blocks = forge::ceil_div(p_tiles * forge::ragged_tiles(N, E, q_tile), 8) * 8;
-    FORGE_REQUIRE(blocks <= INT32_MAX, "forge_gated_rows: %lld workgroups", (long long)blocks);
+    FORGE_REQUIRE(blocks <= INT32_MAX, "%s: %lld workgroups", name, (long long)blocks);
     const dim3 grid((unsigned)blocks);
-    if (few && q_tile == 16) gated_few_kernel<1><<<grid, 512, 0, st>>>(a, (int)p_tiles, split);
-    else if (few && q_tile == 32) gated_few_kernel<2><<<grid, 512, 0, st>>>(a, (int)p_tiles, split);
-    else if (few) gated_few_kernel<4><<<grid, 512, 0, st>>>(a, (int)p_tiles, split);
-    else if (fast) gated_tile_kernel<FORWARD><<<dim3((unsigned)blocks), 512, 0, st>>>(a, (int)p_tiles, 1);
-    else gated_any_kernel<FORWARD><<<dim3((unsigned)blocks), 256, 0, st>>>(a, (int)p_tiles);
+    if (!few) gated_tile_kernel<FORWARD><<<grid, 512, 0, st>>>(a, (int)p_tiles, 1);
+    else if (q_tile == 16) gated_few_kernel<1><<<grid, 512, 0, st>>>(a, (int)p_tiles, split);
+    else if (q_tile == 32) gated_few_kernel<2><<<grid, 512, 0, st>>>(a, (int)p_tiles, split);
+    else gated_few_kernel<4><<<grid, 512, 0, st>>>(a, (int)p_tiles, split);
     FORGE_LAUNCH_CHECK();
     return FORGE_OK;
 }
@@ -721,7 +647,8 @@ extern "C" int forge_gated_rows_backward(const void* dh, const float* g, const f
     FORGE_REQUIRE(N == 0 || ws_bytes >= forge_gated_rows_backward_workspace_bytes(N, I),
                   "%s: workspace of %lld bytes, %lld needed", name, (long long)ws_bytes,
                   (long long)forge_gated_rows_backward_workspace_bytes(N, I));
-    FORGE_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 15) == 0, "%s: workspace not 16-byte aligned", name);
+    FORGE_REQUIRE(aligned16(ws) && aligned16(dh) && aligned16(g) && aligned16(u) && aligned16(drows) && aligned16(dWg) &&
+                      aligned16(dWu), "%s: workspace, gradients, g and u must be 16-byte aligned", name);
     uint16_t* dg = (uint16_t*)ws;
     uint16_t* du = (uint16_t*)((char*)ws + grad_bytes(N, I));
     hipStream_t st = (hipStream_t)stream;
@@ -731,29 +658,21 @@ extern "C" int forge_gated_rows_backward(const void* dh, const float* g, const f
     a.N = (int)N; a.E = (int)E; a.H = (int)H; a.I = (int)I; a.act = act;
     a.dg = dg; a.du = du;
     a.dx = (uint16_t*)drows; a.dwg = (uint16_t*)dWg; a.dwu = (uint16_t*)dWu;
-    const bool fast = tiles_fit(a) && aligned16(dh) && aligned16(g) && aligned16(u) && aligned16(drows) &&
-                      aligned16(dWg) && aligned16(dWu);
-    const int tile = fast ? 256 : 64;
-    const int64_t h_tiles = forge::ceil_div(H, tile), i_tiles = forge::ceil_div(I, tile);
-    const int64_t blocks = forge::ceil_div(h_tiles * forge::ragged_tiles(N, E, tile), 8) * 8;
-    FORGE_REQUIRE(blocks <= INT32_MAX && (h_tiles * i_tiles + 8) * 2 * E <= INT32_MAX, "%s: too many workgroups", name);
+    const bool few = few_rows(N, E);
+    const int64_t h_tiles = forge::ceil_div(H, 256), i_tiles = forge::ceil_div(I, 256), p_tiles = few ? forge::ceil_div(H, 128) : h_tiles;
+    const int64_t row_blocks = forge::ceil_div(p_tiles * forge::ragged_tiles(N, E, few ? 32 : 256), 8) * 8;
+    const int64_t weight_blocks = forge::ceil_div(h_tiles * i_tiles, 8) * 8 * E;
+    FORGE_REQUIRE(row_blocks <= INT32_MAX && 2 * weight_blocks <= INT32_MAX && N * I / 8 / 256 < INT32_MAX, "%s: too many workgroups", name);
     if (N > 0) {
         forge::KernelTiming timing("gated_grad", st, 14.0 * N * I, forge::WORK_BYTES);
-        if (fast)
-            gated_grad8_kernel<<<dim3((unsigned)forge::ceil_div(N * I / 8, 256)), 256, 0, st>>>(
-                (const uint4*)dh, (const f32x4_t*)g, (const f32x4_t*)u, (uint4*)dg, (uint4*)du, N * I / 8, act);
-        else
-            gated_grad_kernel<<<dim3((unsigned)forge::ceil_div(N * I, 256)), 256, 0, st>>>(
-                (const uint16_t*)dh, g, u, dg, du, N * I, act);
+        gated_grad_kernel<<<dim3((unsigned)forge::ceil_div(N * I / 8, 256)), 256, 0, st>>>(
+            (const uint4*)dh, (const f32x4_t*)g, (const f32x4_t*)u, (uint4*)dg, (uint4*)du, N * I / 8, act);
         FORGE_LAUNCH_CHECK();
     }
     if (drows && N > 0) {
         forge::KernelTiming timing("gated_drows", st, 4.0 * N * H * I, forge::WORK_FLOPS);
-        if (fast && few_rows(N, E)) {
-            const int64_t p_tiles = forge::ceil_div(H, 128);
-            gated_drows_few_kernel<<<dim3((unsigned)(p_tiles * forge::ragged_tiles(N, E, 32))), 512, 0, st>>>(a, (int)p_tiles);
-        } else if (fast) gated_tile_kernel<DROWS><<<dim3((unsigned)blocks), 512, 0, st>>>(a, (int)h_tiles, 1);
-        else gated_any_kernel<DROWS><<<dim3((unsigned)blocks), 256, 0, st>>>(a, (int)h_tiles);
+        if (few) gated_drows_few_kernel<<<dim3((unsigned)row_blocks), 512, 0, st>>>(a, (int)p_tiles);
+        else gated_tile_kernel<DROWS><<<dim3((unsigned)row_blocks), 512, 0, st>>>(a, (int)p_tiles, 1);
         FORGE_LAUNCH_CHECK();
     }
     if (dWg || dWu) {
@@ -761,12 +680,7 @@ extern "C" int forge_gated_rows_backward(const void* dh, const float* g, const f
         // gate weights first, then up weights; one alone is passed as the first
         const int both = dWg && dWu ? 2 : 1;
         if (!dWg) { a.dg = du; a.dwg = a.dwu; }
-        if (fast)
-            gated_tile_kernel<DWEIGHTS><<<dim3((unsigned)(forge::ceil_div(h_tiles * i_tiles, 8) * 8 * E * both)), 512, 0, st>>>(
-                a, (int)h_tiles, (int)i_tiles);
-        else
-            gated_any_kernel<DWEIGHTS><<<dim3((unsigned)(h_tiles * i_tiles), (unsigned)E, both), 256, 0, st>>>(
-                a, (int)h_tiles);
+        gated_tile_kernel<DWEIGHTS><<<dim3((unsigned)(weight_blocks * both)), 512, 0, st>>>(a, (int)h_tiles, (int)i_tiles);
         FORGE_LAUNCH_CHECK();
     }
     return FORGE_OK;

@@ -583,7 +583,7 @@ __global__ __launch_bounds__(512) void int4_split_kernel(Int4Args a, int r_tiles
         for (int k = 0; k < 8 && r + k < a.R; ++k) store_y(a, m0 + m, r + k, v[k]);
 }
 
-// Any shape, alignment and group size: 64 x 64 outputs per workgroup, four wavefronts of 32 x 32,
+// Groups that are not multiples of 32 columns (any shape and alignment): 64 x 64 outputs per workgroup, four wavefronts of 32 x 32,
 // 32 columns a step through LDS; a step never crosses the end of a group (its rest is zero).
 __global__ __launch_bounds__(256) void int4_any_kernel(Int4Args a, int r_tiles) {
     constexpr int T = 64, K = 32, LD = K + 8;

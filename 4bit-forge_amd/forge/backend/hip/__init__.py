@@ -100,6 +100,7 @@ def _declare(lib: ctypes.CDLL) -> ctypes.CDLL:
         "forge_rows_diagonal": ([vp, i32, vp, vp, vp, vp, i64, i64, vp], i32),
         "forge_rms_norm": ([vp, i32, i64, vp, i64, vp, i32, i64, i64, f32, vp, vp, vp], i32),
         "forge_rms_norm_fp8": ([vp, i32, i64, vp, i64, vp, i32, i64, i64, f32, vp, vp, vp, vp], i32),
+        "forge_pad_rows": ([vp, i64, i64, vp, i64, i64, i64, i64, i64, vp, vp], i32),
         "forge_gated_rows": ([vp, i64, vp, vp, vp, i64, i64, i64, i64, i64, i64, i32, vp, vp, vp, vp], i32),
         "forge_gated_rows_backward": ([vp, vp, vp, vp, i64, vp, vp, vp, i64, i64, i64, i64, i64, i64, i32,
                                        vp, vp, vp, vp, i64, vp], i32),
@@ -139,7 +140,7 @@ EXPORTED_SYMBOLS = (
     "forge_gptq_sweep_rows_blocked", "forge_gptq_sweep_rows_workspace_bytes",
     "forge_rows_operands", "forge_rows_diagonal",
     "forge_rms_norm", "forge_rms_norm_fp8", "forge_gated_rows", "forge_gated_rows_backward",
-    "forge_gated_rows_backward_workspace_bytes", "forge_linear_int4",
+    "forge_gated_rows_backward_workspace_bytes", "forge_linear_int4", "forge_pad_rows",
 )
 
 # FORGE_ACT_* of include/forge_hip.h
@@ -187,6 +188,12 @@ def _unit_rows(t):
                 return t.contiguous()
         return t
     return t.contiguous()
+
+
+def _pieces(t) -> bool:
+    """Rows that start on 16-byte boundaries and are whole 16-byte pieces long (16-bit elements)."""
+    return (t.shape[-1] % 8 == 0 and t.data_ptr() % 16 == 0 and t.stride(-1) == 1
+            and all(s % 8 == 0 for s in t.stride()[:-1]) and t.stride(-2) < 1 << 21)
 
 
 def _need_one_device(first, *tensors):
@@ -964,52 +971,90 @@ class _HipKernels:
                      scale_inv.data_ptr(), op)
         return codes, scale_inv, out
 
+    def pad_rows(self, t, rows=None, offsets=None):
+        """A copy of t [R,C] or [B,R,C] (16-bit, unit column stride) with zeros behind it up to `rows`
+        rows and a multiple of 8 columns; offsets [B+1]: matrices of experts without rows stay
+        unwritten."""
+        dev = _need_one_device(t, offsets)
+        t3 = t.unsqueeze(0) if t.dim() == 2 else t
+        assert t3.element_size() == 2 and t3.stride(2) == 1
+        assert offsets is None or (offsets.dtype == torch.int32 and offsets.is_contiguous()
+                                   and offsets.numel() == t3.shape[0] + 1)
+        B, R, C = t3.shape
+        Rp, Cp = R if rows is None else int(rows), -(-C // 8) * 8
+        out = torch.empty((B, Rp, Cp), dtype=t.dtype, device=dev)
+        self._launch(dev, self._lib.forge_pad_rows, t3.data_ptr(), t3.stride(0), max(t3.stride(1), C),
+                     out.data_ptr(), B, R, C, Rp, Cp, 0 if offsets is None else offsets.data_ptr())
+        return out[0] if t.dim() == 2 else out
+
+    def _gated_operands(self, rows, offsets, w_gate, w_up):
+        """The three operands as the kernels take them: themselves, or all padded to multiples of 8 (zeros,
+        which change no sum; features behind I come out as 0)."""
+        I, H = w_gate.shape[1:]
+        if I % 8 == 0 and _pieces(w_gate) and _pieces(w_up) and w_gate.stride() == w_up.stride():
+            return (rows if _pieces(rows) else self.pad_rows(rows)), w_gate, w_up
+        Ip = -(-I // 8) * 8
+        return ((rows if _pieces(rows) else self.pad_rows(rows)), self.pad_rows(w_gate, Ip, offsets),
+                self.pad_rows(w_up, Ip, offsets))
+
     def gated_rows(self, rows, offsets, w_gate, w_up, activation="silu", keep=False):
         """rows [N,H] bf16 grouped by expert, offsets [E+1] int32 on the device, w_gate / w_up
-        [E,I,H] bf16 with equal strides -> h [N,I] bf16; keep: also g and u [N,I] f32, for
-        gated_rows_backward.  Allocates its results and nothing else; nothing waits for the GPU."""
+        [E,I,H] bf16 -> h [N,I] bf16; keep: also g and u [N,I'] f32 for gated_rows_backward (I' = I
+        rounded up to a multiple of 8).  Nothing waits for the GPU.  Operands whose rows are not
+        16-byte pieces on 16-byte boundaries (H or I not a multiple of 8, odd pitches) are copied
+        first; h is then a view of a wider result where I is not a multiple of 8."""
         dev = _need_one_device(rows, offsets, w_gate, w_up)
         E, I, H = w_gate.shape
         N = rows.shape[0]
-        ws, ldw, one = w_gate.stride()
         assert rows.dtype == w_gate.dtype == w_up.dtype == torch.bfloat16 and rows.shape[1] == H
         assert offsets.dtype == torch.int32 and offsets.is_contiguous() and offsets.numel() == E + 1
-        assert rows.stride(1) == one == 1 and w_gate.stride() == w_up.stride()
-        assert w_up.shape == w_gate.shape
-        h = torch.empty((N, I), dtype=torch.bfloat16, device=dev)
+        assert rows.stride(1) == w_gate.stride(2) == w_up.stride(2) == 1 and w_up.shape == w_gate.shape
+        rows, w_gate, w_up = self._gated_operands(rows, offsets, w_gate, w_up)
+        ws, ldw, _ = w_gate.stride()
+        Ip, Hp = w_gate.shape[1:]
+        h = torch.empty((N, Ip), dtype=torch.bfloat16, device=dev)
         g = u = None
         if keep:
-            g, u = torch.empty((2, N, I), dtype=torch.float32, device=dev)
-        self._launch(dev, self._lib.forge_gated_rows, rows.data_ptr(), max(rows.stride(0), H),
-                     offsets.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), max(ldw, H), ws, N, E, H, I,
+            g, u = torch.empty((2, N, Ip), dtype=torch.float32, device=dev)
+        self._launch(dev, self._lib.forge_gated_rows, rows.data_ptr(), max(rows.stride(0), Hp),
+                     offsets.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), max(ldw, Hp), ws, N, E, Hp, Ip,
                      _act_code(activation), h.data_ptr(), g.data_ptr() if keep else 0,
                      u.data_ptr() if keep else 0)
+        if Ip != I:
+            h = h[:, :I]
         return (h, g, u) if keep else h
 
     def gated_rows_backward(self, dh, g, u, rows, offsets, w_gate, w_up, activation="silu",
                             need=(True, True, True)):
-        """Gradients of gated_rows for dh [N,I] bf16 contiguous: (d rows [N,H], d w_gate, d w_up
-        [E,I,H]) in bf16, None where `need` says so."""
+        """Gradients of gated_rows for dh [N,I] bf16: (d rows [N,H], d w_gate, d w_up [E,I,H]) in bf16,
+        None where `need` says so; views of wider results where H or I is not a multiple of 8."""
         dev = _need_one_device(dh, g, u, rows, offsets, w_gate, w_up)
         E, I, H = w_gate.shape
-        N = rows.shape[0]
-        ws, ldw, one = w_gate.stride()
+        N, Ip = rows.shape[0], -(-I // 8) * 8
         assert dh.dtype == rows.dtype == w_gate.dtype == w_up.dtype == torch.bfloat16
-        assert tuple(dh.shape) == tuple(g.shape) == tuple(u.shape) == (N, I) and dh.is_contiguous()
+        assert tuple(dh.shape) == (N, I) and tuple(g.shape) == tuple(u.shape) == (N, Ip)
         assert g.dtype == u.dtype == torch.float32 and g.is_contiguous() and u.is_contiguous()
         assert offsets.dtype == torch.int32 and offsets.is_contiguous() and offsets.numel() == E + 1
-        assert rows.stride(1) == one == 1 and w_gate.stride() == w_up.stride()
+        assert rows.stride(1) == w_gate.stride(2) == w_up.stride(2) == 1
         assert w_up.shape == w_gate.shape and tuple(rows.shape) == (N, H)
-        dx = torch.empty((N, H), dtype=torch.bfloat16, device=dev) if need[0] else None
-        dwg = torch.empty((E, I, H), dtype=torch.bfloat16, device=dev) if need[1] else None
-        dwu = torch.empty((E, I, H), dtype=torch.bfloat16, device=dev) if need[2] else None
-        nbytes = int(self._lib.forge_gated_rows_backward_workspace_bytes(N, I))
+        rows, w_gate, w_up = self._gated_operands(rows, offsets, w_gate, w_up)
+        if not dh.is_contiguous() or Ip != I or dh.data_ptr() % 16:
+            dh = self.pad_rows(_unit_rows(dh))
+        ws, ldw, _ = w_gate.stride()
+        Hp = w_gate.shape[2]
+        dx = torch.empty((N, Hp), dtype=torch.bfloat16, device=dev) if need[0] else None
+        dwg = torch.empty((E, Ip, Hp), dtype=torch.bfloat16, device=dev) if need[1] else None
+        dwu = torch.empty((E, Ip, Hp), dtype=torch.bfloat16, device=dev) if need[2] else None
+        nbytes = int(self._lib.forge_gated_rows_backward_workspace_bytes(N, Ip))
         work = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
         ptr = lambda t: 0 if t is None else t.data_ptr()   # noqa: E731
         self._launch(dev, self._lib.forge_gated_rows_backward, dh.data_ptr(), g.data_ptr(), u.data_ptr(),
-                     rows.data_ptr(), max(rows.stride(0), H), offsets.data_ptr(), w_gate.data_ptr(),
-                     w_up.data_ptr(), max(ldw, H), ws, N, E, H, I, _act_code(activation), ptr(dx), ptr(dwg),
+                     rows.data_ptr(), max(rows.stride(0), Hp), offsets.data_ptr(), w_gate.data_ptr(),
+                     w_up.data_ptr(), max(ldw, Hp), ws, N, E, Hp, Ip, _act_code(activation), ptr(dx), ptr(dwg),
                      ptr(dwu), work.data_ptr(), nbytes)
+        if Hp != H or Ip != I:
+            dx = None if dx is None else dx[:, :H]
+            dwg, dwu = (None if d is None else d[:, :I, :H] for d in (dwg, dwu))
         return dx, dwg, dwu
 
     def linear_int4(self, x, packed, scale, group_size, bias=None, activation=None, residual=None):
@@ -1018,7 +1063,7 @@ class _HipKernels:
         dev = _need_one_device(x, packed, scale, bias, residual)
         M, C = x.shape
         R, words = packed.shape
-        ldx, ldr, bp, rp = x.stride(0), 0, 0, 0
+        ldr, bp, rp = 0, 0, 0
         assert x.dtype == torch.bfloat16 and x.stride(1) == 1
         assert packed.dtype == torch.int32 and packed.is_contiguous() and words == (C + 7) // 8
         assert scale.dtype == torch.float32 and scale.is_contiguous()
@@ -1030,8 +1075,11 @@ class _HipKernels:
             assert residual.dtype == torch.bfloat16 and residual.stride(1) == 1
             assert residual.shape[0] == M and residual.shape[1] == R
             ldr, rp = max(residual.stride(0), R), residual.data_ptr()
+        if group_size % 8 == 0 and not _pieces(x):
+            x = self.pad_rows(x)                     # zeros: they meet the last word's spare nibbles
+            C = x.shape[1]
         y = torch.empty((M, R), dtype=torch.bfloat16, device=dev)
-        self._launch(dev, self._lib.forge_linear_int4, x.data_ptr(), max(ldx, C), packed.data_ptr(),
+        self._launch(dev, self._lib.forge_linear_int4, x.data_ptr(), max(x.stride(0), C), packed.data_ptr(),
                      scale.data_ptr(), int(group_size), bp, rp, ldr, M, C, R, _act_code(activation),
                      y.data_ptr())
         return y

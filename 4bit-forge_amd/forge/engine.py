@@ -135,7 +135,7 @@ class _GatedRows(torch.autograd.Function):
     def backward(ctx, dh):
         rows, offsets, w_gate, w_up, g, u = ctx.saved_tensors
         need = (ctx.needs_input_grad[0], ctx.needs_input_grad[2], ctx.needs_input_grad[3])
-        dx, dwg, dwu = kernels.gated_rows_backward(dh.contiguous(), g, u, rows, offsets, w_gate, w_up,
+        dx, dwg, dwu = kernels.gated_rows_backward(dh, g, u, rows, offsets, w_gate, w_up,
                                                    ctx.activation, need)
         return dx, None, dwg, dwu, None
 
@@ -187,8 +187,7 @@ def expert_gated_rows(rows: torch.Tensor, offsets: Union[torch.Tensor, Sequence[
                              f"[0, {N}]")
         off = torch.tensor(off, dtype=torch.int32).to(rows.device)
     rows = _unit_rows(rows)
-    if w_gate.stride() != w_up.stride() or _unit_rows(w_gate) is not w_gate:
-        w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
+    w_gate, w_up = _unit_rows(w_gate), _unit_rows(w_up)
     if torch.is_grad_enabled() and (rows.requires_grad or w_gate.requires_grad or w_up.requires_grad):
         return _GatedRows.apply(rows, off, w_gate, w_up, activation)
     return kernels.gated_rows(rows, off, w_gate, w_up, activation)

@@ -551,6 +551,13 @@ int forge_rms_norm_fp8(const void* x, int dtype, int64_t ldx, const void* residu
                        const void* weight, int w_dtype, int64_t T, int64_t C, float eps,
                        uint8_t* codes, float* scale_inv, void* residual_out, forge_stream_t stream);
 
+/* Copies of 16-bit matrices at the alignment the products below want: out [batch, Rp, Cp] contiguous
+ * and 16-byte aligned, out[b][r][c] = in[b * stride + r * ld + c], zero for r >= R or c >= C (Cp a multiple
+ * of 8).  in is 2-byte aligned.  offsets (may be NULL; device, int32 [batch + 1]): matrix b is left
+ * unwritten where offsets[b] >= offsets[b + 1], an expert without rows. */
+int forge_pad_rows(const void* in, int64_t stride, int64_t ld, void* out, int64_t batch, int64_t R,
+                   int64_t C, int64_t Rp, int64_t Cp, const int32_t* offsets, forge_stream_t stream);
+
 /* Gated feed-forward rows of all experts in one launch: the gate and up projections, the
  * activation and the product, i.e. the rows that reach the down projection (what the hooks of
  * forge/utils/engine.py:210-256 see after the expert's own modules have run).
@@ -558,9 +565,11 @@ int forge_rms_norm_fp8(const void* x, int dtype, int64_t ldx, const void* residu
  * rows [N, H] bf16 with row pitch ldx, grouped by expert; offsets [E + 1] int32 on the DEVICE,
  * ascending within [0, N] (values outside are clamped, so that no call reads or writes out of
  * bounds); Wg, Wu [E, I, H] bf16 with row pitch ldw and expert stride w_stride (both the same for the two);
- * h [N, I] bf16 contiguous.  Sums in f32, h rounded once.  Rows that belong to no expert (before
+ * h [N, I] bf16 contiguous.  H, I, the pitches and the stride are multiples of 8 elements and every
+ * pointer is 16-byte aligned.  Sums in f32, h rounded once.  Rows that belong to no expert (before
  * offsets[0], from offsets[E] on) get h = 0.  gate_out, up_out (both or neither): g and u
- * [N, I] f32, contiguous, for forge_gated_rows_backward (0 in rows of no expert). */
+ * [N, I] f32, contiguous, for forge_gated_rows_backward (0 in rows of no expert).  The weights of
+ * experts without rows are not read. */
 int forge_gated_rows(const void* rows, int64_t ldx, const int32_t* offsets, const void* Wg,
                      const void* Wu, int64_t ldw, int64_t w_stride, int64_t N, int64_t E, int64_t H,
                      int64_t I, int act, void* h, float* gate_out, float* up_out,
@@ -569,9 +578,9 @@ int forge_gated_rows(const void* rows, int64_t ldx, const int32_t* offsets, cons
  *   dg = dh * u * act'(g), du = dh * act(g)           (f32, rounded to bf16 once, into ws)
  *   drows = dg Wg + du Wu [N, H],  dWg[e] = dg_e^T x_e,  dWu[e] = du_e^T x_e [E, I, H]
  * all bf16 contiguous, sums in f32; any of the three may be NULL.  Rows of no expert: drows = 0 (what
- * dh holds there is not read into any gradient); experts without rows: dW = 0.  ws: device
- * workspace of forge_gated_rows_backward_workspace_bytes(N, I), 16-byte aligned.  Results do not
- * depend on the order in which workgroups run. */
+ * dh holds there is not read into any gradient); experts without rows: dW = 0.  Alignment as above.
+ * ws: device workspace of forge_gated_rows_backward_workspace_bytes(N, I), 16-byte aligned.  Results
+ * do not depend on the order in which workgroups run. */
 int forge_gated_rows_backward(const void* dh, const float* g, const float* u, const void* rows,
                               int64_t ldx, const int32_t* offsets, const void* Wg, const void* Wu,
                               int64_t ldw, int64_t w_stride, int64_t N, int64_t E, int64_t H,

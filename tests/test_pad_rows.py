@@ -1,0 +1,99 @@
+"""Padded copies of 16-bit matrices, and the shapes of the gated rows that need them."""
+import ctypes
+
+import pytest
+import torch
+
+from block_ref import gated64, within
+from forge import engine
+
+DEV = "cuda"
+
+
+def test_refusals_at_the_c_entries():
+    from forge.backend.hip import load_library
+    lib, p = load_library(), ctypes.c_void_p(4096)
+    pad = lambda src=p, ld=5, out=p, b=1, R=3, C=5, Rp=3, Cp=8: lib.forge_pad_rows(   # noqa: E731
+        src, 0, ld, out, b, R, C, Rp, Cp, None, None)
+    for bad, text in ((dict(Cp=7), "Cp=7"), (dict(Cp=0), "Cp=0"), (dict(Rp=2), "Rp=2"), (dict(R=-1), "R=-1"),
+                      (dict(C=0), "C=0"), (dict(b=-1), "batch=-1"), (dict(b=65536), "too large"),
+                      (dict(Rp=1 << 30), "too large"), (dict(ld=4), "pitch"), (dict(src=None), "null"),
+                      (dict(out=None), "null"), (dict(out=ctypes.c_void_p(4104)), "aligned"),
+                      (dict(src=ctypes.c_void_p(4097)), "aligned")):
+        assert pad(**bad) != 0
+        assert text in lib.forge_last_error().decode(), bad
+    assert pad(b=0, src=None, out=None) == 0 and pad(R=0, Rp=0, src=None, out=None) == 0
+
+    def gated(x=p, ldx=16, wg=p, ldw=16, ws=128, H=16, I=8):
+        return lib.forge_gated_rows(x, ldx, p, wg, p, ldw, ws, 6, 2, H, I, 0, p, None, None, None)
+    for bad in (dict(H=15), dict(I=7), dict(ldx=17), dict(ldw=20, ws=160), dict(ws=129), dict(x=ctypes.c_void_p(4098)),
+                dict(wg=ctypes.c_void_p(4104))):
+        assert gated(**bad) != 0
+        assert "multiples of 8" in lib.forge_last_error().decode(), bad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,R,C,lead,pitch,Rp", [
+    (1, 1, 1, 0, 1, 1), (1, 3, 5, 1, 7, 3), (2, 7, 8, 0, 8, 8), (3, 5, 9, 1, 9, 8), (2, 33, 513, 3, 517, 40),
+    (1, 9, 64, 1, 67, 9), (1, 300, 1030, 2, 1031, 304), (4, 16, 24, 8, 48, 16), (1, 4, 16, 5, 17, 4)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_pad_rows(hip, B, R, C, lead, pitch, Rp, dtype):
+    flat = torch.full((lead + B * R * pitch + 3,), float("nan"), dtype=dtype, device=DEV)
+    t = flat[lead:lead + B * R * pitch].view(B, R, pitch)[:, :, :C]
+    t.copy_(torch.randn(B, R, C, device=DEV))
+    want = torch.zeros(B, Rp, -(-C // 8) * 8, dtype=dtype, device=DEV)
+    want[:, :R, :C] = t
+    assert torch.equal(hip.pad_rows(t, Rp), want)
+    if Rp == R:
+        assert torch.equal(hip.pad_rows(t[-1]), want[-1])
+
+
+@pytest.mark.gpu
+def test_matrices_without_rows_are_left(hip):
+    t = torch.randn(4, 5, 9, device=DEV).bfloat16()
+    offs = torch.tensor([0, 3, 3, 7, 7], dtype=torch.int32, device=DEV)
+    out = torch.full((4, 8, 16), 7.0, device=DEV).bfloat16()
+    rc = hip._lib.forge_pad_rows(t.data_ptr(), t.stride(0), t.stride(1), out.data_ptr(), 4, 5, 9, 8, 16,
+                                 offs.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    for e in (0, 2):
+        assert torch.equal(out[e, :5, :9], t[e]) and out[e, 5:].eq(0).all() and out[e, :, 9:].eq(0).all()
+    assert out[1].eq(7).all() and out[3].eq(7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,I", [(33, 64), (64, 33), (33, 35)])
+@pytest.mark.parametrize("counts", [(1, 0, 3), (300, 0, 41)])
+def test_gated_rows_of_odd_sizes(hip, counts, H, I):
+    """NaN in the weights of an expert without rows reaches nothing, and a captured call replays"""
+    g = torch.Generator(device=DEV).manual_seed(H + I)
+    mk = lambda s, *sh: (s * torch.randn(*sh, generator=g, device=DEV)).bfloat16()   # noqa: E731
+    N, offs = sum(counts), [0, counts[0], counts[0], sum(counts)]
+    rows, wg, wu, dh = mk(1.0, N, H), mk(H ** -0.5, 3, I, H), mk(H ** -0.5, 3, I, H), mk(1.0, N, I)
+    wg[1], wu[1] = float("nan"), float("nan")
+    leaves = [t.clone().requires_grad_(True) for t in (rows, wg, wu)]
+    h = engine.expert_gated_rows(leaves[0], offs, leaves[1], leaves[2])
+    grads = torch.autograd.grad(h, leaves, dh)
+    z = [torch.nan_to_num(t) for t in (wg, wu)]
+    (want, bound), wants = gated64(rows, offs, z[0], z[1], "silu", dh)
+    within(h, want, bound)
+    for got, like, (w, b) in zip(grads, leaves, wants):
+        assert got.shape == like.shape
+        within(got, w, b)
+    o = torch.tensor(offs, dtype=torch.int32, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        hip.gated_rows(rows, o, wg, wu)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept, gate, up = hip.gated_rows(rows, o, wg, wu, "silu", keep=True)
+        back = hip.gated_rows_backward(dh, gate, up, rows, o, wg, wu)
+    for scale in (1.0, -0.5, 2.0):
+        rows.copy_(leaves[0].detach() * scale)
+        graph.replay()
+        torch.cuda.synchronize()
+        e, eg, eu = hip.gated_rows(rows, o, wg, wu, "silu", keep=True)
+        assert torch.equal(kept, e)
+        assert all(torch.equal(a, b) for a, b in zip(back, hip.gated_rows_backward(dh, eg, eu, rows, o, wg, wu)))
