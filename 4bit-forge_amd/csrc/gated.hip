@@ -39,6 +39,7 @@ struct GatedArgs {
 };
 
 enum { FORWARD = 0, DROWS = 1, DWEIGHTS = 2 };
+constexpr int kLightRows = 128;   // an expert with that many rows or fewer takes half a full tile's matrix work at most
 
 // ---------------------------------------------------------------- many rows
 // 256 x 256 outputs per workgroup (mfma_tile.h).  P runs along the registers of the accumulator, i.e. along
@@ -56,7 +57,10 @@ template <int MODE>
 __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tiles, int q_tiles) {
     using namespace forge;
     __shared__ __attribute__((aligned(1024))) char P0[kStageBytes], Q0[kStageBytes], P1[kStageBytes], Q1[kStageBytes];
-    __shared__ int slot[4];
+    // (DWEIGHTS has no light tiles)
+    constexpr int kLight = MODE == DWEIGHTS ? 16 : kLightStageBytes;
+    __shared__ __attribute__((aligned(1024))) char X0[kLight], X1[kLight], X2[kLight];
+    __shared__ FindSlot slot;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // wavefronts i and i + 4 share a SIMD; they get different quarters of Q, so that a tile with few rows
     // keeps one wavefront busy on every SIMD instead of two on some
@@ -77,17 +81,11 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
         r.rows = clamp_offset(a.offsets, r.expert + 1, r.row0, a.N) - r.row0;
         inner = r.rows;
     } else {
-        // runs of 4 tiles of Q by all tiles of P: the 32 workgroups that an XCD runs at a time are
-        // then 4 x 8 tiles, 12 panels through its L2 where 2 x 16 would be 18
-        if (!find_tile(a.offsets, a.E, a.N, kTile, [&](int q_count) {
-                const int t = xcd_tile(blockIdx.x, q_count * p_tiles);
-                if (t >= q_count * p_tiles) return -1;
-                const int run = t / (4 * p_tiles), in_run = t - run * 4 * p_tiles;
-                const int wide = min(q_count - run * 4, 4);
-                slot[3] = in_run / wide;
-                return run * 4 + in_run % wide;
+        if (!find_tile(a.offsets, a.E, a.N, kTile, kLightRows, p_tiles, [&](int full, int light) {
+                int t;
+                return xcd_tile(blockIdx.x, full, light, t) ? t : full + t;
             }, r, slot)) return;
-        pt = __builtin_amdgcn_readfirstlane(slot[3]);
+        pt = r.p;
         inner = r.expert < 0 ? 0 : MODE == FORWARD ? a.H : a.I;
     }
     const int p0 = pt * (MODE == FORWARD ? kTile / 2 : kTile);
@@ -95,6 +93,7 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
     // nothing to sum (rows of no expert, an expert without rows): one stage of zeros
     const int stages = max(MODE == DROWS ? 2 * per_phase : per_phase, 1);
     const int64_t we = (int64_t)(r.expert < 0 ? 0 : r.expert) * a.ws;
+    const bool light = MODE != DWEIGHTS && r.rows <= 64;
 
     // loaders
     InnerLoader<4> lp_in, lq_in;
@@ -114,28 +113,35 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
         lp_out.init(wave, lane, a.ldx, a.H - p0);
         lq_out.init(wave, lane, a.I, a.I - q0);
     }
-    auto load = [&](int s, char* P, char* Q) {
+    auto load_p = [&](int s, char* P) {
         if constexpr (MODE == FORWARD) {
             lp_in.stage(dp, P, wave, a.ldw, s * kStage, inner);
-            lq_in.stage(dq, Q, wave, a.ldx, s * kStage, inner);
         } else if constexpr (MODE == DROWS) {
             const bool up = s >= per_phase;
             const int k0 = (up ? s - per_phase : s) * kStage;
             lp_out.stage((up ? a.wu : a.wg) + we + (int64_t)k0 * a.ldw + p0, a.ldw, inner - k0, a.H - p0, P, wave);
-            const __amdgpu_buffer_rsrc_t d = descriptor((up ? a.du : a.dg) + (int64_t)r.row0 * a.I, (uint32_t)(r.rows * a.I * 2));
-            lq_in.stage(d, Q, wave, a.I, k0, inner);
         } else {
             const int64_t k0 = (int64_t)r.row0 + s * kStage;
             lp_out.stage(a.x + k0 * a.ldx + p0, a.ldx, r.rows - s * kStage, a.H - p0, P, wave);
-            lq_out.stage((which ? a.du : a.dg) + k0 * a.I + q0, a.I, r.rows - s * kStage, a.I - q0, Q, wave);
         }
     };
-    InnerFragment fp_in, fq_in;
-    OuterFragment<4> fp_out;
-    OuterFragment<2> fq_out;
-    if constexpr (MODE == FORWARD) fp_in.init(lane, wp * 4); else fp_out.init(lane, wp * 4);
-    if constexpr (MODE == DWEIGHTS) fq_out.init(lane, wq * 2); else fq_in.init(lane, wq * 2);
-
+    auto load_q = [&](const auto& loader, int s, char* Q) {
+        if constexpr (MODE == FORWARD) {
+            loader.stage(dq, Q, wave, a.ldx, s * kStage, inner);
+        } else if constexpr (MODE == DROWS) {
+            const bool up = s >= per_phase;
+            const int k0 = (up ? s - per_phase : s) * kStage;
+            const __amdgpu_buffer_rsrc_t d = descriptor((up ? a.du : a.dg) + (int64_t)r.row0 * a.I, (uint32_t)(r.rows * a.I * 2));
+            loader.stage(d, Q, wave, a.I, k0, inner);
+        } else {
+            const int64_t k0 = (int64_t)r.row0 + s * kStage;
+            loader.stage((which ? a.du : a.dg) + k0 * a.I + q0, a.I, r.rows - s * kStage, a.I - q0, Q, wave);
+        }
+    };
+    auto load = [&](int s, char* P, char* Q) {
+        load_p(s, P);
+        if constexpr (MODE == DWEIGHTS) load_q(lq_out, s, Q); else load_q(lq_in, s, Q);
+    };
     // Registers 4 j .. 4 j + 3 of a tile: rows 8 j + 4 (lane / 32) .. + 3 of P, column lane & 31 of Q, i.e.
     // 8 bytes of 32 rows of the output at a time.  The tile goes through LDS, [row of Q][column of P] with
     // 16-byte piece c of row q at c ^ (q % 32), and leaves in runs of a whole row.
@@ -147,59 +153,105 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
     };
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    if (wq * 64 < (MODE == DWEIGHTS ? a.I - q0 : r.rows)) {
-        f32x16_t acc[4][2];
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) acc[t][n][v] = 0.0f;
-        if constexpr (MODE == FORWARD) multiply_stages(stages, P0, Q0, P1, Q1, load, fp_in, fq_in, acc);
-        else if constexpr (MODE == DROWS) multiply_stages(stages, P0, Q0, P1, Q1, load, fp_out, fq_in, acc);
-        else multiply_stages(stages, P0, Q0, P1, Q1, load, fp_out, fq_out, acc);
-        __syncthreads();
+    // 32 columns (block) x 32 rows (from row0 on) of the output; FORWARD: g and u
+    auto put = [&](int row0, int block, const f32x16_t& x, const f32x16_t& y) {
         // an opaque copy: addresses made from it are not formed before the inner loop, where they would
         // cost registers
         int lane_e = lane;
         asm volatile("" : "+v"(lane_e));
-        lds_char* to = buffer(wq * 64 / kRows);
+        const int q = row0 + (lane_e & 31);
+        lds_char* row = buffer(row0 / kRows) + (q % kRows) * (kCols * 2) + (lane_e >> 5) * 8;
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const int q = wq * 64 + n * 32 + (lane_e & 31);
-            lds_char* row = to + (q % kRows) * (kCols * 2) + (lane_e >> 5) * 8;
+        for (int j = 0; j < 4; ++j) {
+            float h[4];
             if constexpr (MODE == FORWARD) {
+                f32x4_t g, u;
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        f32x4_t g, u;
-                        float h[4];
-#pragma unroll
-                        for (int v = 0; v < 4; ++v) {
-                            g[v] = acc[t][n][4 * j + v];
-                            u[v] = acc[t + 2][n][4 * j + v];
-                            h[v] = act_f32(a.act, g[v]) * u[v];
-                        }
-                        *(__attribute__((address_space(3))) u32x2*)(row + (((wp * 8 + t * 4 + j) ^ (q % kPieces)) * 16)) =
-                            u32x2{pack_bf16(h[0], h[1]), pack_bf16(h[2], h[3])};
-                        const int i = p0 + wp * 64 + t * 32 + 8 * j + 4 * (lane_e >> 5);
-                        if (a.g && q < r.rows && i < a.I) {
-                            const int64_t at = (int64_t)(r.row0 + q) * a.I + i;
-                            *reinterpret_cast<f32x4_t*>(a.g + at) = g;
-                            *reinterpret_cast<f32x4_t*>(a.u + at) = u;
-                        }
-                    }
+                for (int v = 0; v < 4; ++v) {
+                    g[v] = x[4 * j + v];
+                    u[v] = y[4 * j + v];
+                    h[v] = act_f32(a.act, g[v]) * u[v];
+                }
+                const int i = p0 + block * 32 + 8 * j + 4 * (lane_e >> 5);
+                if (a.g && q < r.rows && i < a.I) {
+                    const int64_t at = (int64_t)(r.row0 + q) * a.I + i;
+                    *reinterpret_cast<f32x4_t*>(a.g + at) = g;
+                    *reinterpret_cast<f32x4_t*>(a.u + at) = u;
+                }
             } else {
 #pragma unroll
-                for (int t = 0; t < 4; ++t)
+                for (int v = 0; v < 4; ++v) h[v] = x[4 * j + v];
+            }
+            *(__attribute__((address_space(3))) u32x2*)(row + (((block * 4 + j) ^ (q % kPieces)) * 16)) =
+                u32x2{pack_bf16(h[0], h[1]), pack_bf16(h[2], h[3])};
+        }
+    };
+    auto clear = [](auto& acc, int n_p, int n_q) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        *(__attribute__((address_space(3))) u32x2*)(row + (((wp * 16 + t * 4 + j) ^ (q % kPieces)) * 16)) =
-                            u32x2{pack_bf16(acc[t][n][4 * j], acc[t][n][4 * j + 1]),
-                                  pack_bf16(acc[t][n][4 * j + 2], acc[t][n][4 * j + 3])};
+        for (int t = 0; t < n_p; ++t)
+#pragma unroll
+            for (int n = 0; n < n_q; ++n)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) acc[t][n][v] = 0.0f;
+    };
+    InnerFragment fq_in;
+    if (light) {
+        if constexpr (MODE != DWEIGHTS) {
+            // wavefront w: rows 32 (w / 4) .. + 31, columns 32 (w % 4) .. (FORWARD) or 64 (w % 4) .. + 63
+            const int block = wave & 3, row0 = (wave >> 2) * 32;
+            InnerLoader<1> lx;
+            lx.init(lane, MODE == FORWARD ? a.ldx : a.I, wave * 8);
+            lx.piece ^= (wave & 1) * 32;
+            auto load_light = [&](int s, char* P, char* X) {
+                load_p(s, P);
+                load_q(lx, s, X);
+            };
+            fq_in.init(lane, wave >> 2);
+            f32x16_t acc[2][1];
+            clear(acc, 2, 1);
+            if constexpr (MODE == FORWARD) {
+                InnerFragment fp;
+                fp.init(lane, (block >> 1) * 4 + (block & 1));
+                multiply_light_stages<2>(stages, P0, Q0, P1, X0, X1, X2, load_light, fp, fq_in, acc);
+                __syncthreads();
+                put(row0, block, acc[0][0], acc[1][0]);
+            } else {
+                OuterFragment<2> fp;
+                fp.init(lane, block * 2);
+                multiply_light_stages<1>(stages, P0, Q0, P1, X0, X1, X2, load_light, fp, fq_in, acc);
+                __syncthreads();
+                put(row0, block * 2, acc[0][0], acc[0][0]);
+                put(row0, block * 2 + 1, acc[1][0], acc[1][0]);
             }
         }
+    } else if (wq * 64 < (MODE == DWEIGHTS ? a.I - q0 : r.rows)) {
+        f32x16_t acc[4][2];
+        clear(acc, 4, 2);
+        if constexpr (MODE == FORWARD) {
+            InnerFragment fp;
+            fp.init(lane, wp * 4);
+            fq_in.init(lane, wq * 2);
+            multiply_stages(stages, P0, Q0, P1, Q1, load, fp, fq_in, acc);
+        } else {
+            OuterFragment<4> fp;
+            OuterFragment<2> fq_out;
+            fp.init(lane, wp * 4);
+            if constexpr (MODE == DROWS) {
+                fq_in.init(lane, wq * 2);
+                multiply_stages(stages, P0, Q0, P1, Q1, load, fp, fq_in, acc);
+            } else {
+                fq_out.init(lane, wq * 2);
+                multiply_stages(stages, P0, Q0, P1, Q1, load, fp, fq_out, acc);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int t = 0; t < (MODE == FORWARD ? 2 : 4); ++t) {
+                if constexpr (MODE == FORWARD) put(wq * 64 + n * 32, wp * 2 + t, acc[t][n], acc[t + 2][n]);
+                else put(wq * 64 + n * 32, wp * 4 + t, acc[t][n], acc[t][n]);
+            }
     } else {
         load_stages(stages, P0, Q0, P1, Q1, load);
         __syncthreads();
@@ -218,13 +270,14 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
         out = (which ? a.dwu : a.dwg) + ((int64_t)r.expert * a.I + q0) * a.H + p0;
         pitch = a.H; rows = a.I - q0; cols = a.H - p0;
     }
-    // wavefront w writes rows 32 w .. 32 w + 31
-    lds_char* from = buffer(wave * 32 / kRows);
+    // every wavefront writes 32 rows, or 8 of a light tile's
+    const int own = light ? 8 : 32;
+    lds_char* from = buffer(wave * own / kRows);
     const int piece = lane % kPieces;
     if (piece * 8 < cols) {
 #pragma unroll 4
-        for (int i = 0; i < 32 * kPieces / 64; ++i) {
-            const int q = wave * 32 + i * (64 / kPieces) + lane / kPieces;
+        for (int i = 0; i < own * kPieces / 64; ++i) {
+            const int q = wave * own + i * (64 / kPieces) + lane / kPieces;
             if (q >= rows) break;
             const u32x4 v = *(__attribute__((address_space(3))) u32x4*)(from + (q % kRows) * (kCols * 2) +
                                                                         ((piece ^ (q % kPieces)) * 16));
@@ -249,14 +302,13 @@ __global__ __launch_bounds__(512) void gated_few_kernel(GatedArgs a, int p_tiles
     using namespace forge;
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     __shared__ __attribute__((aligned(1024))) char S0[8 * kRunBytes], S1[8 * kRunBytes];
-    __shared__ int slot[4];
+    __shared__ FindSlot slot;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, kb = lane >> 4;
     const int share = wave % split;                              // which of its features' runs
-    const int f0 = (blockIdx.x % p_tiles) * (128 / split), qt = blockIdx.x / p_tiles;
-    const int i0 = f0 + wave / split * 16;
     RaggedTile r;
-    if (!find_tile(a.offsets, a.E, a.N, 16 * MT, [=](int) { return qt; }, r, slot)) return;
+    if (!find_tile(a.offsets, a.E, a.N, 16 * MT, 0, p_tiles, [](int, int) { return (int)blockIdx.x; }, r, slot)) return;
+    const int f0 = r.p * (128 / split), i0 = f0 + wave / split * 16;
     const int inner = r.expert < 0 ? 0 : a.H;
     const int wrows = min(a.I - i0, 16);                          // none for a wavefront behind the last feature
     const int64_t we = (int64_t)(r.expert < 0 ? 0 : r.expert) * a.ws + (wrows > 0 ? (int64_t)i0 * a.ldw : 0);
@@ -369,11 +421,11 @@ __global__ __launch_bounds__(512) void gated_drows_few_kernel(GatedArgs a, int p
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     constexpr int kRun = 32 * 256;
     __shared__ __attribute__((aligned(1024))) char S0[8 * kRun], S1[8 * kRun];
-    __shared__ int slot[4];
+    __shared__ FindSlot slot;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int p0 = (blockIdx.x % p_tiles) * 128, qt = blockIdx.x / p_tiles;
     RaggedTile r;
-    if (!find_tile(a.offsets, a.E, a.N, 32, [=](int) { return qt; }, r, slot)) return;
+    if (!find_tile(a.offsets, a.E, a.N, 32, 0, p_tiles, [](int, int) { return (int)blockIdx.x; }, r, slot)) return;
+    const int p0 = r.p * 128;
     const int per_phase = r.expert < 0 ? 0 : (a.I + 31) / 32, runs = 2 * per_phase;
     const int64_t we = (int64_t)(r.expert < 0 ? 0 : r.expert) * a.ws + p0;
     const int cols = min(a.H - p0, 128);
@@ -512,11 +564,20 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(const uint4* __restrict
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 constexpr int64_t kFillWorkgroups = 256;
-// The kernels for few rows rather than the tiles (7168 x 2048, weights from HBM, us, few against tiles:
-// forward 8 experts of 8 rows 96 / 166, of 32 116 / 175, of 64 152 / 181, one expert of 256 79 / 126, of 512
-// 153 / 127; d rows 8 experts of 32 rows 102 / 110, of 64 146 / 114, one of 256 49 / 80, of 512 93 / 82;
-// 128 experts at 2048 x 768 forward of 4 rows 183 / 222, of 64 269 / 219).
-bool few_rows(int64_t N, int64_t E) { return N <= 256 || N <= 32 * E; }
+// The kernels for few rows rather than the tiles: where there are few rows in all, and where the tiles would not
+// fill the GPU.  Weights from HBM, us, few against tiles:
+//   forward, 7168 x 2048: one expert of 64 rows 33 / 96, of 256 88 / 180; 8 experts of 8 rows 136 / 149, of 32 144 /
+//     150, of 64 173 / 153; 32 experts of 4 rows 372 / 372, of 32 420 / 374
+//   forward, 2048 x 768: 8 experts of 32 rows 28 / 31, of 64 40 / 33; 32 of 8 rows 58 / 64, of 32 73 / 67; 128 of 2
+//     rows 209 / 216, of 4 206 / 200, of 64 291 / 208
+//   d rows, 7168 x 2048: one expert of 64 rows 30 / 39, of 256 78 / 82; 8 experts of 8 rows 87 / 80
+//   d rows, 2048 x 768: one expert of 256 rows 16 / 35; 8 of 8 rows 15 / 19, of 64 23 / 20; 32 of 8 rows 38 / 35
+bool few_rows(int64_t N, int64_t E, int64_t I) {
+    return N <= 256 || (N <= 32 * E && E * forge::ceil_div(I, 128) < kFillWorkgroups);
+}
+bool few_rows_back(int64_t N, int64_t E, int64_t H) {
+    return N <= 256 && (N < E ? N : E) * forge::ceil_div(H, 256) <= kFillWorkgroups / 2;
+}
 // and how many rows of x per workgroup (8 experts of 16 rows: 98 with 16, 101 with 32, 116 with 64;
 // of 64 rows: 238, 178, 152)
 int few_tile(int64_t N, int64_t E) { return N <= 32 || N <= 16 * E ? 16 : N <= 64 || N <= 48 * E ? 32 : 64; }
@@ -615,13 +676,13 @@ extern "C" int forge_gated_rows(const void* rows, int64_t ldx, const int32_t* of
     a.h = (uint16_t*)h; a.g = gate_out; a.u = up_out;
     hipStream_t st = (hipStream_t)stream;
     forge::KernelTiming timing("gated_rows", st, 4.0 * N * H * I, forge::WORK_FLOPS);
-    const bool few = few_rows(N, E);
+    const bool few = few_rows(N, E, I);
     const int64_t live = N < E ? N : E;                           // experts with rows, at most
     int split = 1;
     while (few && split < 8 && forge::ceil_div(I, 128 / split) * live < kFillWorkgroups) split *= 2;
     const int64_t p_tiles = forge::ceil_div(I, few ? 128 / split : 128);
     const int q_tile = few ? few_tile(N, E) : 256;
-    const int64_t blocks = forge::ceil_div(p_tiles * forge::ragged_tiles(N, E, q_tile), 8) * 8;
+    const int64_t blocks = forge::ceil_div(p_tiles * forge::ragged_tiles(N, E, q_tile), 8) * 8 + 8;
     FORGE_REQUIRE(blocks <= INT32_MAX, "%s: %lld workgroups", name, (long long)blocks);
     const dim3 grid((unsigned)blocks);
     if (!few) gated_tile_kernel<FORWARD><<<grid, 512, 0, st>>>(a, (int)p_tiles, 1);
@@ -658,9 +719,9 @@ extern "C" int forge_gated_rows_backward(const void* dh, const float* g, const f
     a.N = (int)N; a.E = (int)E; a.H = (int)H; a.I = (int)I; a.act = act;
     a.dg = dg; a.du = du;
     a.dx = (uint16_t*)drows; a.dwg = (uint16_t*)dWg; a.dwu = (uint16_t*)dWu;
-    const bool few = few_rows(N, E);
+    const bool few = few_rows_back(N, E, H);
     const int64_t h_tiles = forge::ceil_div(H, 256), i_tiles = forge::ceil_div(I, 256), p_tiles = few ? forge::ceil_div(H, 128) : h_tiles;
-    const int64_t row_blocks = forge::ceil_div(p_tiles * forge::ragged_tiles(N, E, few ? 32 : 256), 8) * 8;
+    const int64_t row_blocks = forge::ceil_div(p_tiles * forge::ragged_tiles(N, E, few ? 32 : 256), 8) * 8 + 8;
     const int64_t weight_blocks = forge::ceil_div(h_tiles * i_tiles, 8) * 8 * E;
     FORGE_REQUIRE(row_blocks <= INT32_MAX && 2 * weight_blocks <= INT32_MAX && N * I / 8 / 256 < INT32_MAX, "%s: too many workgroups", name);
     if (N > 0) {

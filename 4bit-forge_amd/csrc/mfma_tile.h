@@ -133,25 +133,25 @@ struct OuterFragment {
     }
 };
 
-// The fragments of one step: NP of P, 2 of Q
-template <int NP>
+// The fragments of one step: NP of P (every SKIP-th), NQ of Q
+template <int NP, int NQ = 2, int SKIP = 1>
 struct Fragments {
-    bf16x8_t p[NP], q[2];
+    bf16x8_t p[NP], q[NQ];
     template <typename FP, typename FQ>
     __device__ __forceinline__ void read(const char* P, const char* Q, const FP& fp, const FQ& fq, int s) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) q[t] = fq.read(Q, t, s);
+        for (int t = 0; t < NQ; ++t) q[t] = fq.read(Q, t, s);
 #pragma unroll
-        for (int t = 0; t < NP; ++t) p[t] = fp.read(P, t, s);
+        for (int t = 0; t < NP; ++t) p[t] = fp.read(P, t * SKIP, s);
     }
     // FIRST: the sums start from zero, which the matrix instruction takes as a constant
     template <bool FIRST = false>
-    __device__ __forceinline__ void multiply(f32x16_t (&acc)[NP][2]) const {
+    __device__ __forceinline__ void multiply(f32x16_t (&acc)[NP][NQ]) const {
         const f32x16_t zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
         for (int t = 0; t < NP; ++t)
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < NQ; ++n)
                 acc[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[t], q[n], FIRST ? zero : acc[t][n], 0, 0, 0);
     }
 };
@@ -240,12 +240,60 @@ __device__ __forceinline__ void load_stages(int stages, char* P0, char* Q0, char
     wait_loads<0>();
 }
 
+// Tiles with up to 64 rows of Q: bound by P's bytes, so three stages are on their way instead of two.
+// Q's stages are 8 KB (X0 .. X2), P's lie in three of the four buffers.  Wavefront w has 32 rows of Q (w / 4) and
+// two tiles of P; load(s, P, X) issues 5 loads.
+constexpr int kLightStageBytes = 64 * kStage * 2;
+template <int SKIP, typename LOAD, typename FP, typename FQ>
+__device__ __forceinline__ void one_light_stage(int s, char* P, char* X, LOAD& load, const FP& fp, const FQ& fq, f32x16_t (&acc)[2][1]) {
+    Fragments<2, 1, SKIP> f[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[k].read(P, X, fp, fq, k);
+    wait_loads_barrier<5>();                 // this stage has been read, and the next one has arrived
+    load(s + 3, P, X);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[k].multiply(acc);
+}
+template <int SKIP, typename LOAD, typename FP, typename FQ>
+__device__ __forceinline__ void multiply_light_stages(int stages, char* P0, char* P1, char* P2, char* X0, char* X1, char* X2, LOAD& load,
+                                                      const FP& fp, const FQ& fq, f32x16_t (&acc)[2][1]) {
+    load(0, P0, X0);
+    load(1, P1, X1);
+    load(2, P2, X2);
+    wait_loads_barrier<10>();
+    // stages behind the last are zeros
+    for (int s = 0; s < stages; s += 3) {
+        one_light_stage<SKIP>(s, P0, X0, load, fp, fq, acc);
+        one_light_stage<SKIP>(s + 1, P1, X1, load, fp, fq, acc);
+        one_light_stage<SKIP>(s + 2, P2, X2, load, fp, fq, acc);
+    }
+    wait_loads<0>();
+}
+
 // Workgroup b of a launch runs on XCD b % 8 (each has its own L2).  Of `tiles` tiles every XCD takes
 // a run of consecutive ones, so that tiles that share an operand share an L2; the tile of b's, or
 // `tiles` or more if there is none.
 __device__ __forceinline__ int xcd_tile(int b, int tiles) {
     const int per = (tiles + 7) / 8, i = b / 8;
     return i < per ? (b % 8) * per + i : tiles;
+}
+
+// The same for two lists, `full` tiles that take long and `light` ones that take little matrix work but as many
+// bytes: every XCD takes an eighth of either list.  The light ones lie evenly between the others, so
+// that the memory is in use all the time, but for the last 32, which even out the end.  True and t: a full tile;
+// false: a light one (t = light or more: none).  Launch 8 workgroups more than there are tiles, rounded up to 8.
+__device__ __forceinline__ bool xcd_tile(int b, int full, int light, int& t) {
+    const int x = b % 8, i = b / 8;
+    const int f0 = min(x * ((full + 7) / 8), full), fn = min((x + 1) * ((full + 7) / 8), full) - f0;
+    const int l0 = min(x * ((light + 7) / 8), light), ln = min((x + 1) * ((light + 7) / 8), light) - l0;
+    const int n = fn + max(ln - 32, 0);
+    if (i >= n) {
+        t = i - fn < ln ? l0 + i - fn : light;
+        return false;
+    }
+    const int before = (int)(((int64_t)i * fn + n - 1) / n), upto = (int)(((int64_t)(i + 1) * fn + n - 1) / n);
+    t = upto > before ? f0 + before : l0 + i - before;
+    return upto > before;
 }
 
 }  // namespace forge
