@@ -56,11 +56,7 @@ constexpr int kLightRows = 128;   // an expert with that many rows or fewer take
 template <int MODE>
 __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tiles, int q_tiles) {
     using namespace forge;
-    __shared__ __attribute__((aligned(1024))) char P0[kStageBytes], Q0[kStageBytes], P1[kStageBytes], Q1[kStageBytes];
-    // (DWEIGHTS has no light tiles)
-    constexpr int kLight = MODE == DWEIGHTS ? 16 : kLightStageBytes;
-    __shared__ __attribute__((aligned(1024))) char X0[kLight], X1[kLight], X2[kLight];
-    __shared__ FindSlot slot;
+    __shared__ __attribute__((aligned(1024))) char P0[kStageBytes], P1[kStageBytes], P2[kStageBytes], Q0[kStageBytes], Q1[kStageBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // wavefronts i and i + 4 share a SIMD; they get different quarters of Q, so that a tile with few rows
     // keeps one wavefront busy on every SIMD instead of two on some
@@ -84,7 +80,8 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
         if (!find_tile(a.offsets, a.E, a.N, kTile, kLightRows, p_tiles, [&](int full, int light) {
                 int t;
                 return xcd_tile(blockIdx.x, full, light, t) ? t : full + t;
-            }, r, slot)) return;
+            }, r, *reinterpret_cast<FindSlot*>(P2))) return;
+        __syncthreads();                                          // P2 is read
         pt = r.p;
         inner = r.expert < 0 ? 0 : MODE == FORWARD ? a.H : a.I;
     }
@@ -125,7 +122,7 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
             lp_out.stage(a.x + k0 * a.ldx + p0, a.ldx, r.rows - s * kStage, a.H - p0, P, wave);
         }
     };
-    auto load_q = [&](const auto& loader, int s, char* Q) {
+    auto load_q_by = [&](const auto& loader, int s, char* Q) {
         if constexpr (MODE == FORWARD) {
             loader.stage(dq, Q, wave, a.ldx, s * kStage, inner);
         } else if constexpr (MODE == DROWS) {
@@ -138,9 +135,8 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
             loader.stage((which ? a.du : a.dg) + k0 * a.I + q0, a.I, r.rows - s * kStage, a.I - q0, Q, wave);
         }
     };
-    auto load = [&](int s, char* P, char* Q) {
-        load_p(s, P);
-        if constexpr (MODE == DWEIGHTS) load_q(lq_out, s, Q); else load_q(lq_in, s, Q);
+    auto load_q = [&](int s, char* Q) {
+        if constexpr (MODE == DWEIGHTS) load_q_by(lq_out, s, Q); else load_q_by(lq_in, s, Q);
     };
     // Registers 4 j .. 4 j + 3 of a tile: rows 8 j + 4 (lane / 32) .. + 3 of P, column lane & 31 of Q, i.e.
     // 8 bytes of 32 rows of the output at a time.  The tile goes through LDS, [row of Q][column of P] with
@@ -148,7 +144,7 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
     // (32 KB of the tile per buffer: 64 rows of 512 bytes, or 128 of FORWARD's 256 bytes.)
     constexpr int kCols = MODE == FORWARD ? kTile / 2 : kTile, kPieces = kCols / 8, kRows = kStageBytes / (kCols * 2);
     auto buffer = [&](int i) {
-        lds_char *b0 = (lds_char*)P0, *b1 = (lds_char*)Q0, *b2 = (lds_char*)P1, *b3 = (lds_char*)Q1;
+        lds_char *b0 = (lds_char*)P0, *b1 = (lds_char*)P1, *b2 = (lds_char*)P2, *b3 = (lds_char*)Q0;
         return i == 0 ? b0 : i == 1 ? b1 : i == 2 ? b2 : b3;
     };
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -202,23 +198,20 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
             InnerLoader<1> lx;
             lx.init(lane, MODE == FORWARD ? a.ldx : a.I, wave * 8);
             lx.piece ^= (wave & 1) * 32;
-            auto load_light = [&](int s, char* P, char* X) {
-                load_p(s, P);
-                load_q(lx, s, X);
-            };
+            auto load_light = [&](int s, char* Q) { load_q_by(lx, s, Q); };
             fq_in.init(lane, wave >> 2);
             f32x16_t acc[2][1];
             clear(acc, 2, 1);
             if constexpr (MODE == FORWARD) {
                 InnerFragment fp;
                 fp.init(lane, (block >> 1) * 4 + (block & 1));
-                multiply_light_stages<2>(stages, P0, Q0, P1, X0, X1, X2, load_light, fp, fq_in, acc);
+                multiply_light_stages<2>(stages, P0, P1, P2, Q0, Q1, load_p, load_light, fp, fq_in, acc);
                 __syncthreads();
                 put(row0, block, acc[0][0], acc[1][0]);
             } else {
                 OuterFragment<2> fp;
                 fp.init(lane, block * 2);
-                multiply_light_stages<1>(stages, P0, Q0, P1, X0, X1, X2, load_light, fp, fq_in, acc);
+                multiply_light_stages<1>(stages, P0, P1, P2, Q0, Q1, load_p, load_light, fp, fq_in, acc);
                 __syncthreads();
                 put(row0, block * 2, acc[0][0], acc[0][0]);
                 put(row0, block * 2 + 1, acc[1][0], acc[1][0]);
@@ -231,17 +224,17 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
             InnerFragment fp;
             fp.init(lane, wp * 4);
             fq_in.init(lane, wq * 2);
-            multiply_stages(stages, P0, Q0, P1, Q1, load, fp, fq_in, acc);
+            multiply_stages(stages, P0, P1, P2, Q0, Q1, load_p, load_q, fp, fq_in, acc);
         } else {
             OuterFragment<4> fp;
             OuterFragment<2> fq_out;
             fp.init(lane, wp * 4);
             if constexpr (MODE == DROWS) {
                 fq_in.init(lane, wq * 2);
-                multiply_stages(stages, P0, Q0, P1, Q1, load, fp, fq_in, acc);
+                multiply_stages(stages, P0, P1, P2, Q0, Q1, load_p, load_q, fp, fq_in, acc);
             } else {
                 fq_out.init(lane, wq * 2);
-                multiply_stages(stages, P0, Q0, P1, Q1, load, fp, fq_out, acc);
+                multiply_stages(stages, P0, P1, P2, Q0, Q1, load_p, load_q, fp, fq_out, acc);
             }
         }
         __syncthreads();
@@ -253,7 +246,7 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
                 else put(wq * 64 + n * 32, wp * 4 + t, acc[t][n], acc[t][n]);
             }
     } else {
-        load_stages(stages, P0, Q0, P1, Q1, load);
+        load_stages(stages, P0, P1, P2, Q0, Q1, load_p, load_q);
         __syncthreads();
     }
     __syncthreads();

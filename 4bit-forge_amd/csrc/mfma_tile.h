@@ -7,9 +7,11 @@
 // bytes a clock, so the matrix pipe and not the LDS is the limit; 64 x 64 per wavefront (16
 // wavefronts) would need 256 KB and sit exactly on it.
 //
-// A stage is 64 deep and there are two buffers.  Stages go from memory to LDS without touching
-// registers (buffer_load ... lds, 16 bytes a lane), issued as soon as their buffer has been read,
-// seven eighths of two stages before their use.  A lane whose element lies outside the matrix gets an
+// A stage is 64 deep; the 160 KB of LDS are three buffers of P and two of Q.  Stages go from memory to LDS
+// without touching registers (buffer_load ... lds, 16 bytes a lane), issued as soon as their buffer has been
+// read: Q's a stage before their use, P's two (with two buffers of P, 128 KB, a stage that comes from HBM
+// arrives too late: 16 experts at 7168 x 2048 and 16384 rows took 950 us and now 855, one expert at 7168 x 1024
+// and 32768 rows 768 and now 722, 1334 TFLOP/s).  A lane whose element lies outside the matrix gets an
 // offset beyond the descriptor's range, for which the hardware writes zeros; stages behind the last
 // are fetched like that too.
 //
@@ -169,21 +171,23 @@ __device__ __forceinline__ void order_step() {
     }
 }
 
-// The inner loop.  load(s, P, Q) issues stage s's loads (8 per wavefront).  A stage is four steps;
-// while a step's 8 matrix instructions run, the next step's fragments are read.  The one barrier of
-// a stage sits before its last step, whose fragments are in registers by then: nothing waits behind
-// it.  It publishes that the next stage has arrived and that this stage's buffer has been read, which
-// the loads of the stage after next then fill.
+// The inner loop.  load_p(s, P) and load_q(s, Q) issue stage s's loads (4 each per wavefront).  A stage is
+// four steps; while a step's 8 matrix instructions run, the next step's fragments are read.  The one
+// barrier of a stage sits before its last step, whose fragments are in registers by then: nothing waits
+// behind it.  It publishes that the next stage has arrived and that this stage's buffers have been read, which
+// the loads of Q's stage after next, and a step later of P's third next, then fill.  Loads return in the
+// order of their issue, so the wait is for all but the youngest four.
 // The buffers are separate arrays and the loop is unrolled over them because the compiler otherwise
 // has to assume that a load on its way to LDS may hit what is being read, and waits for it.
-template <typename LOAD, typename FP, typename FQ>
-__device__ __forceinline__ void one_stage(int s, char* P, char* Q, const char* Pn, const char* Qn, LOAD& load,
+template <typename LOADP, typename LOADQ, typename FP, typename FQ>
+__device__ __forceinline__ void one_stage(int s, const char* P, char* Q, const char* Pn, const char* Qn, char* Pl, LOADP& load_p, LOADQ& load_q,
                                           const FP& fp, const FQ& fq, Fragments<4>& f, f32x16_t (&acc)[4][2]) {
     constexpr int kReads = 4 * FP::kReads + 2 * FQ::kReads;
     Fragments<4> g;
+    load_p(s + 2, Pl);
     g.read(P, Q, fp, fq, 1);
     f.multiply(acc);
-    order_step<kReads, 0>();
+    order_step<kReads, 4>();
     __builtin_amdgcn_sched_barrier(0);
     f.read(P, Q, fp, fq, 2);
     g.multiply(acc);
@@ -192,80 +196,111 @@ __device__ __forceinline__ void one_stage(int s, char* P, char* Q, const char* P
     g.read(P, Q, fp, fq, 3);
     f.multiply(acc);
     order_step<kReads, 0>();
-    wait_loads_barrier<0>();
-    load(s + 2, P, Q);
+    wait_loads_barrier<4>();
+    load_q(s + 2, Q);
     f.read(Pn, Qn, fp, fq, 0);
     g.multiply(acc);
-    order_step<kReads, 8>();
+    order_step<kReads, 4>();
     __builtin_amdgcn_sched_barrier(0);
 }
 
 // stages >= 1
-template <typename LOAD, typename FP, typename FQ>
-__device__ __forceinline__ void multiply_stages(int stages, char* P0, char* Q0, char* P1, char* Q1, LOAD& load,
+template <typename LOADP, typename LOADQ, typename FP, typename FQ>
+__device__ __forceinline__ void multiply_stages(int stages, char* P0, char* P1, char* P2, char* Q0, char* Q1, LOADP& load_p, LOADQ& load_q,
                                                 const FP& fp, const FQ& fq, f32x16_t (&acc)[4][2]) {
-    load(0, P0, Q0);
-    load(1, P1, Q1);
+    load_p(0, P0);
+    load_q(0, Q0);
+    __builtin_amdgcn_sched_barrier(0);
+    load_p(1, P1);
+    load_q(1, Q1);
     wait_loads_barrier<8>();
     Fragments<4> f;
     f.read(P0, Q0, fp, fq, 0);
     int s = 0;
-    for (; s + 2 <= stages; s += 2) {
-        one_stage(s, P0, Q0, P1, Q1, load, fp, fq, f, acc);
-        one_stage(s + 1, P1, Q1, P0, Q0, load, fp, fq, f, acc);
+    for (; s + 6 <= stages; s += 6) {
+        one_stage(s, P0, Q0, P1, Q1, P2, load_p, load_q, fp, fq, f, acc);
+        one_stage(s + 1, P1, Q1, P2, Q0, P0, load_p, load_q, fp, fq, f, acc);
+        one_stage(s + 2, P2, Q0, P0, Q1, P1, load_p, load_q, fp, fq, f, acc);
+        one_stage(s + 3, P0, Q1, P1, Q0, P2, load_p, load_q, fp, fq, f, acc);
+        one_stage(s + 4, P1, Q0, P2, Q1, P0, load_p, load_q, fp, fq, f, acc);
+        one_stage(s + 5, P2, Q1, P0, Q0, P1, load_p, load_q, fp, fq, f, acc);
     }
-    if (s < stages) one_stage(s, P0, Q0, P1, Q1, load, fp, fq, f, acc);
+    if (s < stages) one_stage(s, P0, Q0, P1, Q1, P2, load_p, load_q, fp, fq, f, acc);
+    if (s + 1 < stages) one_stage(s + 1, P1, Q1, P2, Q0, P0, load_p, load_q, fp, fq, f, acc);
+    if (s + 2 < stages) one_stage(s + 2, P2, Q0, P0, Q1, P1, load_p, load_q, fp, fq, f, acc);
+    if (s + 3 < stages) one_stage(s + 3, P0, Q1, P1, Q0, P2, load_p, load_q, fp, fq, f, acc);
+    if (s + 4 < stages) one_stage(s + 4, P1, Q0, P2, Q1, P0, load_p, load_q, fp, fq, f, acc);
     // loads of stages behind the last (zeros) are still on their way to LDS: a workgroup that ends
     // gives its LDS away
     wait_loads<0>();
 }
 
 // What a wavefront without outputs of its own does meanwhile: its share of the loads, and the barriers
-template <typename LOAD>
-__device__ __forceinline__ void load_stages(int stages, char* P0, char* Q0, char* P1, char* Q1, LOAD& load) {
-    load(0, P0, Q0);
-    load(1, P1, Q1);
+template <typename LOADP, typename LOADQ>
+__device__ __forceinline__ void load_stages(int stages, char* P0, char* P1, char* P2, char* Q0, char* Q1, LOADP& load_p, LOADQ& load_q) {
+    load_p(0, P0);
+    load_q(0, Q0);
+    __builtin_amdgcn_sched_barrier(0);
+    load_p(1, P1);
+    load_q(1, Q1);
     wait_loads_barrier<8>();
+    auto stage = [&](int s, char* Q, char* Pl) {
+        load_p(s + 2, Pl);
+        wait_loads_barrier<4>();
+        load_q(s + 2, Q);
+        __builtin_amdgcn_sched_barrier(0);
+    };
     int s = 0;
-    for (; s + 2 <= stages; s += 2) {
-        wait_loads_barrier<0>();
-        load(s + 2, P0, Q0);
-        wait_loads_barrier<0>();
-        load(s + 3, P1, Q1);
+    for (; s + 6 <= stages; s += 6) {
+        stage(s, Q0, P2);
+        stage(s + 1, Q1, P0);
+        stage(s + 2, Q0, P1);
+        stage(s + 3, Q1, P2);
+        stage(s + 4, Q0, P0);
+        stage(s + 5, Q1, P1);
     }
-    if (s < stages) {
-        wait_loads_barrier<0>();
-        load(s + 2, P0, Q0);
-    }
+    if (s < stages) stage(s, Q0, P2);
+    if (s + 1 < stages) stage(s + 1, Q1, P0);
+    if (s + 2 < stages) stage(s + 2, Q0, P1);
+    if (s + 3 < stages) stage(s + 3, Q1, P2);
+    if (s + 4 < stages) stage(s + 4, Q0, P0);
     wait_loads<0>();
 }
 
-// Tiles with up to 64 rows of Q: bound by P's bytes, so three stages are on their way instead of two.
-// Q's stages are 8 KB (X0 .. X2), P's lie in three of the four buffers.  Wavefront w has 32 rows of Q (w / 4) and
-// two tiles of P; load(s, P, X) issues 5 loads.
-constexpr int kLightStageBytes = 64 * kStage * 2;
-template <int SKIP, typename LOAD, typename FP, typename FQ>
-__device__ __forceinline__ void one_light_stage(int s, char* P, char* X, LOAD& load, const FP& fp, const FQ& fq, f32x16_t (&acc)[2][1]) {
+// Tiles with up to 64 rows of Q: bound by P's bytes, so its loads go out a stage earlier, three ahead.
+// Q's stages are 8 KB; wavefront w has 32 rows of Q (w / 4) and two tiles of P; load_q issues one load.
+template <int SKIP, typename LOADP, typename LOADQ, typename FP, typename FQ>
+__device__ __forceinline__ void one_light_stage(int s, char* P, char* Q, LOADP& load_p, LOADQ& load_q, const FP& fp, const FQ& fq, f32x16_t (&acc)[2][1]) {
     Fragments<2, 1, SKIP> f[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) f[k].read(P, X, fp, fq, k);
-    wait_loads_barrier<5>();                 // this stage has been read, and the next one has arrived
-    load(s + 3, P, X);
+    for (int k = 0; k < 4; ++k) f[k].read(P, Q, fp, fq, k);
+    wait_loads_barrier<4>();                 // this stage has been read; the next one is here (its third next's P is not)
+    load_q(s + 2, Q);
+    __builtin_amdgcn_sched_barrier(0);
+    load_p(s + 3, P);
 #pragma unroll
     for (int k = 0; k < 4; ++k) f[k].multiply(acc);
 }
-template <int SKIP, typename LOAD, typename FP, typename FQ>
-__device__ __forceinline__ void multiply_light_stages(int stages, char* P0, char* P1, char* P2, char* X0, char* X1, char* X2, LOAD& load,
+template <int SKIP, typename LOADP, typename LOADQ, typename FP, typename FQ>
+__device__ __forceinline__ void multiply_light_stages(int stages, char* P0, char* P1, char* P2, char* Q0, char* Q1, LOADP& load_p, LOADQ& load_q,
                                                       const FP& fp, const FQ& fq, f32x16_t (&acc)[2][1]) {
-    load(0, P0, X0);
-    load(1, P1, X1);
-    load(2, P2, X2);
-    wait_loads_barrier<10>();
+    load_p(0, P0);
+    load_q(0, Q0);
+    __builtin_amdgcn_sched_barrier(0);
+    load_p(1, P1);
+    load_q(1, Q1);
+    __builtin_amdgcn_sched_barrier(0);
+    load_p(2, P2);
+    wait_loads_barrier<9>();
     // stages behind the last are zeros
-    for (int s = 0; s < stages; s += 3) {
-        one_light_stage<SKIP>(s, P0, X0, load, fp, fq, acc);
-        one_light_stage<SKIP>(s + 1, P1, X1, load, fp, fq, acc);
-        one_light_stage<SKIP>(s + 2, P2, X2, load, fp, fq, acc);
+    for (int s = 0; s < stages; s += 6) {
+        one_light_stage<SKIP>(s, P0, Q0, load_p, load_q, fp, fq, acc);
+        one_light_stage<SKIP>(s + 1, P1, Q1, load_p, load_q, fp, fq, acc);
+        one_light_stage<SKIP>(s + 2, P2, Q0, load_p, load_q, fp, fq, acc);
+        if (s + 3 >= stages) break;
+        one_light_stage<SKIP>(s + 3, P0, Q1, load_p, load_q, fp, fq, acc);
+        one_light_stage<SKIP>(s + 4, P1, Q0, load_p, load_q, fp, fq, acc);
+        one_light_stage<SKIP>(s + 5, P2, Q1, load_p, load_q, fp, fq, acc);
     }
     wait_loads<0>();
 }
