@@ -94,7 +94,7 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
 
     // loaders
     InnerLoader<4> lp_in, lq_in;
-    OuterLoader lp_out, lq_out;
+    OuterLoader<> lp_out, lq_out;
     __amdgpu_buffer_rsrc_t dp, dq;
     if constexpr (MODE == FORWARD) {
         const bool up = (wave & 3) >= 2;                       // this wavefront loads rows of Wu
@@ -277,6 +277,157 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
             *reinterpret_cast<u32x4*>(out + q * pitch + piece * 8) = v;
         }
     }
+}
+
+// ---------------------------------------------------------------- DWEIGHTS
+// P = columns of X, Q = rows of dW (columns of dg or du), inner dimension the expert's rows.  An expert has a
+// few stages only, and 128 KB of output per tile: a workgroup per tile spends as long on its beginning and
+// its end as on the product.  So there is one workgroup per CU, which takes tile after tile: during a tile's last
+// stages the next tile's first ones are on their way, and the output leaves while the next tile begins,
+// through 2 KB of LDS of every wavefront's own.  A tile has a multiple of four stages (zeros where there are
+// no rows).  Experts differ in rows, so the tiles are given out by a counter per XCD (which workgroup computes
+// a tile changes nothing in it); the counter is asked three tiles ahead.  128 experts of 64 rows at 2048 x 768 are
+// written at 4.7 TB/s, the rate of a copy (172 us, 218 with a workgroup per tile); where there is more to multiply the
+// stores of all CUs come at the same time, and a tile's fourth stage waits for them.
+__global__ __launch_bounds__(512) void gated_dweights_kernel(GatedArgs a, int p_tiles, int q_tiles, int* counters) {
+    using namespace forge;
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    constexpr int kShortBytes = kTile * kShort * 2;
+    __shared__ __attribute__((aligned(1024))) char P0[kShortBytes], P1[kShortBytes], P2[kShortBytes], P3[kShortBytes],
+        Q0[kShortBytes], Q1[kShortBytes], Q2[kShortBytes], Q3[kShortBytes], S[8 * 2048];
+    __shared__ int slot[2];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wp = wave >> 2, wq = wave & 3;
+    // Every XCD takes an eighth of every expert's tiles: those of up to 8 tiles of Q by some of P, which share
+    // their panels in its L2.  Q counts the gate's tiles, then the up projection's.
+    const int tiles = p_tiles * q_tiles, per = (tiles + 7) / 8, t0 = (blockIdx.x % 8) * per;
+    const int here = min(tiles - t0, per), items = here > 0 ? here * a.E : 0, workers = gridDim.x / 8;
+    const int first = blockIdx.x / 8;
+    if (first >= items) return;
+
+    typedef __attribute__((address_space(4))) int32_t scalar_int;
+    struct Tile {
+        int expert, which, p0, q0, row0, rows, stages;
+        OuterLoader<kShort> p, q;
+    };
+    auto tile_at = [&](int item) {
+        Tile t;
+        t.expert = item / here;
+        const int c = t0 + item - t.expert * here, group = c / (8 * p_tiles), in_group = c - group * 8 * p_tiles;
+        const int wide = min(q_tiles - group * 8, 8), up_from = (a.I + kTile - 1) / kTile;
+        const int q = group * 8 + in_group % wide;
+        t.which = q >= up_from;
+        t.p0 = in_group / wide * kTile;
+        t.q0 = (t.which ? q - up_from : q) * kTile;
+        // scalar loads: a vector load would have to wait for the stores before it
+        const scalar_int* o = (const scalar_int*)a.offsets + t.expert;
+        t.row0 = max(0, min(o[0], a.N));
+        t.rows = max(t.row0, min(o[1], a.N)) - t.row0;
+        t.stages = max((t.rows + 4 * kShort - 1) / (4 * kShort) * 4, 4);
+        t.p.init(wave, lane, a.ldx, a.H - t.p0);
+        t.q.init(wave, lane, a.I, a.I - t.q0);
+        return t;
+    };
+    Tile t = tile_at(first), next = t;
+    // stage s of tile t; behind its last, the first ones of the next
+    auto load = [&](int s, char* P, char* Q) {
+        // (selected with a mask: from conditional expressions the compiler makes branches between the products)
+        const int on = (t.stages - 1 - s) >> 31;
+        auto pick = [&](int mine, int others) { return mine ^ ((mine ^ others) & on); };
+        const int k = (s - (t.stages & on)) * kShort, left = pick(t.rows, next.rows) - k;
+        const int64_t row = pick(t.row0, next.row0) + k;
+        const int p0 = pick(t.p0, next.p0), q0 = pick(t.q0, next.q0);
+        OuterLoader<kShort> p, q;
+        p.even = pick(t.p.even, next.p.even);
+        p.odd = pick(t.p.odd, next.p.odd);
+        q.even = pick(t.q.even, next.q.even);
+        q.odd = pick(t.q.odd, next.q.odd);
+        const int64_t dudg = (const char*)a.du - (const char*)a.dg;
+        const uint16_t* grad = (const uint16_t*)((const char*)a.dg + (dudg & -(int64_t)pick(t.which, next.which)));
+        p.stage(a.x + row * a.ldx + p0, a.ldx, left, a.H - p0, P, wave);
+        q.stage(grad + row * a.I + q0, a.I, left, a.I - q0, Q, wave);
+    };
+    OuterFragment<4> fp;
+    OuterFragment<2> fq;
+    fp.init(lane, wp * 4);
+    fq.init(lane, wq * 2);
+    f32x16_t acc[4][2];
+    auto clear = [&] {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) acc[t][n][v] = 0.0f;
+    };
+    load(0, P0, Q0);
+    load(1, P1, Q1);
+    load(2, P2, Q2);
+    load(3, P3, Q3);
+    wait_loads_barrier<0>();                                      // all four: no stores are behind their loads yet
+    Fragments<4> f;
+    f.read(P0, Q0, fp, fq, 0);
+    clear();
+    constexpr int kStores = 16;
+    int coming = first + workers;                                 // the tile after this one
+    for (int turn = 0;; ++turn) {
+        // asked for now, looked at behind the tile: the third one from here (the sum would wait for the answer)
+        int count = 0, opaque = 0;
+        asm volatile("" : "+v"(opaque));                          // else the compiler adds up over lanes, and waits
+        if (counters && threadIdx.x == 0)
+            count = __hip_atomic_fetch_add(counters + blockIdx.x % 8 + opaque, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const bool more = coming < items;
+        next = tile_at(more ? coming : first);
+        if (!more) next.rows = 0;                                 // zeros, which nobody reads
+        // the stores of the tile before are younger than the loads of this one's first four stages
+        one_short_stage<8 + kStores>(P0, Q0, P1, Q1, [&] { load(4, P0, Q0); }, fp, fq, f, acc);
+        one_short_stage<8 + kStores>(P1, Q1, P2, Q2, [&] { load(5, P1, Q1); }, fp, fq, f, acc);
+        one_short_stage<8 + kStores>(P2, Q2, P3, Q3, [&] { load(6, P2, Q2); }, fp, fq, f, acc);
+        one_short_stage<8>(P3, Q3, P0, Q0, [&] { load(7, P3, Q3); }, fp, fq, f, acc);
+        for (int s = 4; s < t.stages; s += 4) {
+            one_short_stage<8>(P0, Q0, P1, Q1, [&] { load(s + 4, P0, Q0); }, fp, fq, f, acc);
+            one_short_stage<8>(P1, Q1, P2, Q2, [&] { load(s + 5, P1, Q1); }, fp, fq, f, acc);
+            one_short_stage<8>(P2, Q2, P3, Q3, [&] { load(s + 6, P2, Q2); }, fp, fq, f, acc);
+            one_short_stage<8>(P3, Q3, P0, Q0, [&] { load(s + 7, P3, Q3); }, fp, fq, f, acc);
+        }
+
+        // 32 rows of Q by 32 columns of P at a time: [row][64 bytes], 16-byte piece c of row q at c ^ (q / 4 % 4).
+        // Outside the matrix the stores are out of the descriptor's range: all are issued, as counted above.
+        uint16_t* out = (t.which ? a.dwu : a.dwg) + ((int64_t)t.expert * a.I + t.q0) * a.H + t.p0;
+        const int rows = min(a.I - t.q0, kTile), cols = a.H - t.p0;
+        const __amdgpu_buffer_rsrc_t d = descriptor(out, (uint32_t)(((rows - 1) * (int64_t)a.H + min(cols, kTile)) * 2));
+        lds_char* mine = (lds_char*)S + wave * 2048;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                int lane_e = lane;
+                asm volatile("" : "+v"(lane_e));                  // addresses are formed here, not before the loop
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f32x16_t& v = acc[b][n];
+                    *(__attribute__((address_space(3))) u32x2*)(mine + (lane_e & 31) * 64 + ((j ^ ((lane_e >> 2) & 3)) * 16) + (lane_e >> 5) * 8) =
+                        u32x2{pack_bf16(v[4 * j], v[4 * j + 1]), pack_bf16(v[4 * j + 2], v[4 * j + 3])};
+                }
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int q = r * 16 + (lane_e >> 2), c = lane_e & 3;
+                    const u32x4 v = *(__attribute__((address_space(3))) u32x4*)(mine + q * 64 + ((c ^ ((q >> 2) & 3)) * 16));
+                    const int col = wp * 128 + b * 32 + c * 8, row = wq * 64 + n * 32 + q;
+                    __builtin_amdgcn_raw_buffer_store_b128(v, d, col < cols && row < rows ? (int)((row * (int64_t)a.H + col) * 2) : (int)kOutside, 0, 0);
+                }
+            }
+        __builtin_amdgcn_sched_barrier(0);
+        if (!more) break;
+        clear();
+        t = next;
+        // what was asked for a tile ago was written before a barrier of this tile's
+        coming = turn ? __builtin_amdgcn_readfirstlane(slot[(turn - 1) & 1]) : first + 2 * workers;
+        if (threadIdx.x == 0) slot[turn & 1] = counters ? 3 * workers + count : first + (turn + 3) * workers;
+    }
+    // loads of zeros are still on their way to LDS: a workgroup that ends gives its LDS away
+    wait_loads<0>();
 }
 
 // ---------------------------------------------------------------- few rows: FORWARD alone
@@ -529,8 +680,9 @@ __global__ __launch_bounds__(512) void gated_drows_few_kernel(GatedArgs a, int p
 __global__ __launch_bounds__(256) void gated_grad_kernel(const uint4* __restrict__ dh,
                                                           const f32x4_t* __restrict__ g,
                                                           const f32x4_t* __restrict__ u, uint4* __restrict__ dg,
-                                                          uint4* __restrict__ du, int64_t n8, int act) {
+                                                          uint4* __restrict__ du, int64_t n8, int act, int* __restrict__ counters) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < 8) counters[i] = 0;                                   // for the launch behind this one
     if (i >= n8) return;
     const uint4 d4 = dh[i];
     const f32x4_t gv[2] = {g[2 * i], g[2 * i + 1]}, uv[2] = {u[2 * i], u[2 * i + 1]};
@@ -574,6 +726,12 @@ bool few_rows_back(int64_t N, int64_t E, int64_t H) {
 // and how many rows of x per workgroup (8 experts of 16 rows: 98 with 16, 101 with 32, 116 with 64;
 // of 64 rows: 238, 178, 152)
 int few_tile(int64_t N, int64_t E) { return N <= 32 || N <= 16 * E ? 16 : N <= 64 || N <= 48 * E ? 32 : 64; }
+
+// From so many rows per expert on a workgroup per tile does better than one per CU (gated_dweights_kernel), whose
+// stages are fetched less far ahead: 7168 x 2048, us, per CU against per tile: 16 experts of 64 rows 212 / 256, 16
+// with 8168 rows by popularity 545 / 630, of 1024 rows 905 / 975, 8 of 2048 rows 831 / 811, 4 of 4096 rows 790 / 742,
+// one of 8192 411 / 365
+constexpr int64_t kLongExperts = 2048;
 
 int64_t grad_bytes(int64_t N, int64_t I) { return forge::ceil_div(2 * N * I, 256) * 256; }
 
@@ -687,7 +845,7 @@ extern "C" int forge_gated_rows(const void* rows, int64_t ldx, const int32_t* of
 }
 
 extern "C" int64_t forge_gated_rows_backward_workspace_bytes(int64_t N, int64_t I) {
-    return N > 0 && I > 0 ? 2 * grad_bytes(N, I) : 0;
+    return N > 0 && I > 0 ? 2 * grad_bytes(N, I) + 256 : 0;
 }
 
 extern "C" int forge_gated_rows_backward(const void* dh, const float* g, const float* u, const void* rows,
@@ -715,12 +873,11 @@ extern "C" int forge_gated_rows_backward(const void* dh, const float* g, const f
     const bool few = few_rows_back(N, E, H);
     const int64_t h_tiles = forge::ceil_div(H, 256), i_tiles = forge::ceil_div(I, 256), p_tiles = few ? forge::ceil_div(H, 128) : h_tiles;
     const int64_t row_blocks = forge::ceil_div(p_tiles * forge::ragged_tiles(N, E, few ? 32 : 256), 8) * 8 + 8;
-    const int64_t weight_blocks = forge::ceil_div(h_tiles * i_tiles, 8) * 8 * E;
-    FORGE_REQUIRE(row_blocks <= INT32_MAX && 2 * weight_blocks <= INT32_MAX && N * I / 8 / 256 < INT32_MAX, "%s: too many workgroups", name);
+    FORGE_REQUIRE(row_blocks <= INT32_MAX && 16 * forge::ceil_div(h_tiles * i_tiles, 8) * E <= INT32_MAX && N * I / 8 / 256 < INT32_MAX, "%s: too many workgroups", name);
     if (N > 0) {
         forge::KernelTiming timing("gated_grad", st, 14.0 * N * I, forge::WORK_BYTES);
         gated_grad_kernel<<<dim3((unsigned)forge::ceil_div(N * I / 8, 256)), 256, 0, st>>>(
-            (const uint4*)dh, (const f32x4_t*)g, (const f32x4_t*)u, (uint4*)dg, (uint4*)du, N * I / 8, act);
+            (const uint4*)dh, (const f32x4_t*)g, (const f32x4_t*)u, (uint4*)dg, (uint4*)du, N * I / 8, act, (int*)((char*)ws + 2 * grad_bytes(N, I)));
         FORGE_LAUNCH_CHECK();
     }
     if (drows && N > 0) {
@@ -734,7 +891,15 @@ extern "C" int forge_gated_rows_backward(const void* dh, const float* g, const f
         // gate weights first, then up weights; one alone is passed as the first
         const int both = dWg && dWu ? 2 : 1;
         if (!dWg) { a.dg = du; a.dwg = a.dwu; }
-        gated_tile_kernel<DWEIGHTS><<<dim3((unsigned)(weight_blocks * both)), 512, 0, st>>>(a, (int)h_tiles, (int)i_tiles);
+        if (N >= kLongExperts * E) {
+            const int64_t blocks = forge::ceil_div(h_tiles * i_tiles, 8) * 8 * E * both;
+            gated_tile_kernel<DWEIGHTS><<<dim3((unsigned)blocks), 512, 0, st>>>(a, (int)h_tiles, (int)i_tiles);
+        } else {
+            const int64_t items = forge::ceil_div(h_tiles * i_tiles * both, 8) * E;    // of an XCD
+            const int64_t blocks = 8 * (items < kFillWorkgroups / 8 ? items : kFillWorkgroups / 8);
+            gated_dweights_kernel<<<dim3((unsigned)blocks), 512, 0, st>>>(
+                a, (int)h_tiles, (int)(i_tiles * both), N > 0 ? (int*)((char*)ws + 2 * grad_bytes(N, I)) : nullptr);
+        }
         FORGE_LAUNCH_CHECK();
     }
     return FORGE_OK;

@@ -80,22 +80,24 @@ struct InnerLoader {
 };
 // ---- K_OUTER: columns `col0 ..` of a matrix whose rows are the inner dimension.  The descriptor is
 // made per stage (base at the stage's first row), so row offsets never pass 32 bits.
+template <int DEPTH = kStage>
 struct OuterLoader {
+    static constexpr int kLoads = DEPTH / 16;      // of a wavefront, two rows each
     uint32_t even, odd;  // byte offsets of loads 0 and 1; 2 and 3 are 4 rows behind
     __device__ __forceinline__ void init(int wave, int lane, int64_t ld, int cols) {
-        const int k = wave * 8 + lane / 32, c = (lane & 31) ^ ((lane / 32) << 2);
+        const int k = wave * 2 * kLoads + lane / 32, c = (lane & 31) ^ ((lane / 32) << 2);
         even = c * 8 < cols ? (uint32_t)(k * ld * 2) + c * 16 : kOutside;
         odd = (c ^ 8) * 8 < cols ? (uint32_t)((k + 2) * ld * 2) + (c ^ 8) * 16 : kOutside;
     }
     // base: first row of the stage at the tile's first column; rows left in the matrix from there
     __device__ __forceinline__ void stage(const uint16_t* base, int64_t ld, int left, int cols, char* lds, int wave) const {
-        const int rows = min(left, kStage), width = min(cols, kTile);
+        const int rows = min(left, DEPTH), width = min(cols, kTile);
         const int size = max((rows - 1) * (int)ld + width, 0);           // 0 rows or fewer: nothing
         const __amdgpu_buffer_rsrc_t d = descriptor(base, (uint32_t)size * 2);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < kLoads; ++j)
             // (kOutside plus a few rows is still outside)
-            load_to_lds(d, lds + (wave * 4 + j) * 1024, ((j & 1) ? odd : even) + (uint32_t)((j >> 1) * 8 * ld));
+            load_to_lds(d, lds + (wave * kLoads + j) * 1024, ((j & 1) ? odd : even) + (uint32_t)((j >> 1) * 8 * ld));
     }
 };
 
@@ -233,6 +235,28 @@ __device__ __forceinline__ void multiply_stages(int stages, char* P0, char* P1, 
     // loads of stages behind the last (zeros) are still on their way to LDS: a workgroup that ends
     // gives its LDS away
     wait_loads<0>();
+}
+
+// The same where both operands are K_OUTER, for tiles that follow one another without a pause (the loads go on across
+// the border): stages of 32 with four buffers of either, fetched three stages ahead.  Half as deep would be half as
+// many bytes of a row where the inner dimension is contiguous; here a row's 512 bytes stay together.
+// load() issues the loads that this stage's buffers are to get (4 per wavefront); YOUNGER is how many loads and
+// stores were issued behind those of the next stage, which are all that is waited for.
+constexpr int kShort = 32;
+template <int YOUNGER, typename LOAD, typename FP, typename FQ>
+__device__ __forceinline__ void one_short_stage(const char* P, const char* Q, const char* Pn, const char* Qn, LOAD load, const FP& fp,
+                                                const FQ& fq, Fragments<4>& f, f32x16_t (&acc)[4][2]) {
+    constexpr int kReads = 4 * FP::kReads + 2 * FQ::kReads;
+    Fragments<4> g;
+    g.read(P, Q, fp, fq, 1);
+    f.multiply(acc);
+    order_step<kReads, 0>();
+    wait_loads_barrier<YOUNGER>();
+    load();
+    f.read(Pn, Qn, fp, fq, 0);
+    g.multiply(acc);
+    order_step<kReads, 4>();
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // What a wavefront without outputs of its own does meanwhile: its share of the loads, and the barriers

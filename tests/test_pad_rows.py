@@ -97,3 +97,55 @@ def test_gated_rows_of_odd_sizes(hip, counts, H, I):
         e, eg, eu = hip.gated_rows(rows, o, wg, wu, "silu", keep=True)
         assert torch.equal(kept, e)
         assert all(torch.equal(a, b) for a, b in zip(back, hip.gated_rows_backward(dh, eg, eu, rows, o, wg, wu)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts,H,I", [([2100], 136, 72), ([4096, 0, 2300], 264, 40)])
+def test_weight_gradients_of_experts_with_many_rows(hip, counts, H, I):
+    g = torch.Generator(device=DEV).manual_seed(H)
+    mk = lambda s, *sh: (s * torch.randn(*sh, generator=g, device=DEV)).bfloat16()   # noqa: E731
+    offs = [0] + torch.tensor(counts).cumsum(0).tolist()
+    N, E = offs[-1], len(counts)
+    leaves = [t.requires_grad_(True) for t in (mk(1.0, N, H), mk(H ** -0.5, E, I, H), mk(H ** -0.5, E, I, H))]
+    dh = mk(1.0, N, I)
+    h = engine.expert_gated_rows(leaves[0], offs, leaves[1], leaves[2])
+    grads = torch.autograd.grad(h, leaves, dh)
+    (want, bound), wants = gated64(*[t.detach() for t in leaves[:1]], offs, *[t.detach() for t in leaves[1:]], "silu", dh)
+    within(h.detach(), want, bound)
+    for got, (w, b) in zip(grads, wants):
+        within(got, w, b)
+
+
+@pytest.mark.gpu
+def test_weight_gradients_hand_their_tiles_out_once(hip):
+    """more tiles than workgroups, experts of very different lengths: every tile is written, in every one of
+    several passes and replays alike"""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    counts = [900, 0, 3, 60, 0, 200, 1, 40] * 6
+    offs = [0] + torch.tensor(counts).cumsum(0).tolist()
+    N, E, H, I = offs[-1], len(counts), 520, 264
+    mk = lambda s, *sh: (s * torch.randn(*sh, generator=g, device=DEV)).bfloat16()   # noqa: E731
+    rows, wg, wu, dh = mk(1.0, N, H), mk(0.05, E, I, H), mk(0.05, E, I, H), mk(1.0, N, I)
+    o = torch.tensor(offs, dtype=torch.int32, device=DEV)
+    _, gate, up = hip.gated_rows(rows, o, wg, wu, "silu", keep=True)
+    first = hip.gated_rows_backward(dh, gate, up, rows, o, wg, wu)
+    _, wants = gated64(rows, offs, wg, wu, "silu", dh)
+    for got, (w, b) in zip(first, wants):
+        within(got, w, b)
+    for need in ((False, True, False), (False, False, True)):
+        part = hip.gated_rows_backward(dh, gate, up, rows, o, wg, wu, need=need)
+        assert all(p is None or torch.equal(p, f) for p, f in zip(part, first))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = hip.gated_rows_backward(dh, gate, up, rows, o, wg, wu)
+    for _ in range(3):
+        for t in kept:
+            t.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        again = hip.gated_rows_backward(dh, gate, up, rows, o, wg, wu)
+        assert all(torch.equal(a, f) and torch.equal(b, f) for a, b, f in zip(kept, again, first))
+    # no rows at all: nothing counts the tiles, all are zero
+    zero = torch.zeros(E + 1, dtype=torch.int32, device=DEV)
+    empty = hip.gated_rows_backward(dh[:0], gate[:0], up[:0], rows[:0], zero, wg, wu)
+    assert all((t == 0).all() for t in empty[1:])
