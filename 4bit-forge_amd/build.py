@@ -46,6 +46,8 @@ NO_SCRATCH = (
     "lowrank_gram_wide_kernel", "lowrank_sweep_kernel", "mse_grid_kernel",
     "split_gemm_kernel", "chain_gemm_fast_kernel", "syrk_bf16_big_kernel", "syrk_bf16_kernel",
     "diag_block_kernel",
+    "gated_tile_kernel", "gated_dweights_kernel", "gated_few_kernel", "gated_drows_few_kernel", "rms_norm_kernel",
+    "int4_few_kernel", "int4_split_kernel", "int4_tile_kernel",
     # the LDS-staged variants of the in-block chain (sixth template argument, TAIL, false)
     re.compile(r"sweep_block_kernel<\d+, \d+, \w+, \w+, \w+, false"),
 )

@@ -316,16 +316,20 @@ __device__ __forceinline__ void multiply_light_stages(int stages, char* P0, char
     __builtin_amdgcn_sched_barrier(0);
     load_p(2, P2);
     wait_loads_barrier<9>();
-    // stages behind the last are zeros
-    for (int s = 0; s < stages; s += 6) {
+    int s = 0;
+    for (; s + 6 <= stages; s += 6) {
         one_light_stage<SKIP>(s, P0, Q0, load_p, load_q, fp, fq, acc);
         one_light_stage<SKIP>(s + 1, P1, Q1, load_p, load_q, fp, fq, acc);
         one_light_stage<SKIP>(s + 2, P2, Q0, load_p, load_q, fp, fq, acc);
-        if (s + 3 >= stages) break;
         one_light_stage<SKIP>(s + 3, P0, Q1, load_p, load_q, fp, fq, acc);
         one_light_stage<SKIP>(s + 4, P1, Q0, load_p, load_q, fp, fq, acc);
         one_light_stage<SKIP>(s + 5, P2, Q1, load_p, load_q, fp, fq, acc);
     }
+    if (s < stages) one_light_stage<SKIP>(s, P0, Q0, load_p, load_q, fp, fq, acc);
+    if (s + 1 < stages) one_light_stage<SKIP>(s + 1, P1, Q1, load_p, load_q, fp, fq, acc);
+    if (s + 2 < stages) one_light_stage<SKIP>(s + 2, P2, Q0, load_p, load_q, fp, fq, acc);
+    if (s + 3 < stages) one_light_stage<SKIP>(s + 3, P0, Q1, load_p, load_q, fp, fq, acc);
+    if (s + 4 < stages) one_light_stage<SKIP>(s + 4, P1, Q0, load_p, load_q, fp, fq, acc);
     wait_loads<0>();
 }
 

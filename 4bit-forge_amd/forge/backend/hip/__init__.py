@@ -987,7 +987,7 @@ class _HipKernels:
                      out.data_ptr(), B, R, C, Rp, Cp, 0 if offsets is None else offsets.data_ptr())
         return out[0] if t.dim() == 2 else out
 
-    def _gated_operands(self, rows, offsets, w_gate, w_up):
+    def gated_operands(self, rows, offsets, w_gate, w_up):
         """The three operands as the kernels take them: themselves, or all padded to multiples of 8 (zeros,
         which change no sum; features behind I come out as 0)."""
         I, H = w_gate.shape[1:]
@@ -1009,7 +1009,7 @@ class _HipKernels:
         assert rows.dtype == w_gate.dtype == w_up.dtype == torch.bfloat16 and rows.shape[1] == H
         assert offsets.dtype == torch.int32 and offsets.is_contiguous() and offsets.numel() == E + 1
         assert rows.stride(1) == w_gate.stride(2) == w_up.stride(2) == 1 and w_up.shape == w_gate.shape
-        rows, w_gate, w_up = self._gated_operands(rows, offsets, w_gate, w_up)
+        rows, w_gate, w_up = self.gated_operands(rows, offsets, w_gate, w_up)
         ws, ldw, _ = w_gate.stride()
         Ip, Hp = w_gate.shape[1:]
         h = torch.empty((N, Ip), dtype=torch.bfloat16, device=dev)
@@ -1037,7 +1037,7 @@ class _HipKernels:
         assert offsets.dtype == torch.int32 and offsets.is_contiguous() and offsets.numel() == E + 1
         assert rows.stride(1) == w_gate.stride(2) == w_up.stride(2) == 1
         assert w_up.shape == w_gate.shape and tuple(rows.shape) == (N, H)
-        rows, w_gate, w_up = self._gated_operands(rows, offsets, w_gate, w_up)
+        rows, w_gate, w_up = self.gated_operands(rows, offsets, w_gate, w_up)
         if not dh.is_contiguous() or Ip != I or dh.data_ptr() % 16:
             dh = self.pad_rows(_unit_rows(dh))
         ws, ldw, _ = w_gate.stride()

@@ -125,18 +125,27 @@ class _GatedRows(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, rows, offsets, w_gate, w_up, activation):
+        I, H = w_gate.shape[1:]
+        # odd sizes: the padded copies are kept, so that the backward pass need not make them again
+        rows, w_gate, w_up = kernels.gated_operands(rows, offsets, w_gate, w_up)
         h, g, u = kernels.gated_rows(rows, offsets, w_gate, w_up, activation, keep=True)
         ctx.save_for_backward(rows, offsets, w_gate, w_up, g, u)
-        ctx.activation = activation
-        return h
+        ctx.activation, ctx.sizes = activation, (H, I)
+        return h if h.shape[1] == I else h[:, :I]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
         rows, offsets, w_gate, w_up, g, u = ctx.saved_tensors
+        H, I = ctx.sizes
         need = (ctx.needs_input_grad[0], ctx.needs_input_grad[2], ctx.needs_input_grad[3])
+        if g.shape[1] != I:
+            dh = kernels.pad_rows(_unit_rows(dh))
         dx, dwg, dwu = kernels.gated_rows_backward(dh, g, u, rows, offsets, w_gate, w_up,
                                                    ctx.activation, need)
+        if rows.shape[1] != H or g.shape[1] != I:
+            dx = None if dx is None else dx[:, :H]
+            dwg, dwu = (None if d is None else d[:, :I, :H] for d in (dwg, dwu))
         return dx, None, dwg, dwu, None
 
 

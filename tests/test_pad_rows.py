@@ -149,3 +149,27 @@ def test_weight_gradients_hand_their_tiles_out_once(hip):
     zero = torch.zeros(E + 1, dtype=torch.int32, device=DEV)
     empty = hip.gated_rows_backward(dh[:0], gate[:0], up[:0], rows[:0], zero, wg, wu)
     assert all((t == 0).all() for t in empty[1:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("per", [1, 9], ids=["few", "many"])
+def test_more_experts_than_a_workgroup_has_threads(hip, per):
+    """offsets of 1300 experts, most of them without rows"""
+    g = torch.Generator(device=DEV).manual_seed(per)
+    E, H, I = 1300, 48, 40
+    counts = [0] * E
+    for e in range(3, E, 13):
+        counts[e] = per * (1 + e % 3)
+    counts[700] = 130
+    offs = [0] + torch.tensor(counts).cumsum(0).tolist()
+    mk = lambda s, *sh: (s * torch.randn(*sh, generator=g, device=DEV)).bfloat16()   # noqa: E731
+    rows, wg, wu, dh = mk(1.0, offs[-1] + 5, H), mk(0.15, E, I, H), mk(0.15, E, I, H), mk(1.0, offs[-1] + 5, I)
+    leaves = [t.clone().requires_grad_(True) for t in (rows, wg, wu)]
+    h = engine.expert_gated_rows(leaves[0], torch.tensor(offs, device=DEV), leaves[1], leaves[2])
+    grads = torch.autograd.grad(h, leaves, dh)
+    n = offs[-1]
+    assert (h[n:] == 0).all() and (grads[0][n:] == 0).all()
+    (want, bound), wants = gated64(rows[:n], offs, wg, wu, "silu", dh[:n])
+    within(h[:n], want, bound)
+    for got, (w, b) in zip((grads[0][:n], *grads[1:]), wants):
+        within(got, w, b)
