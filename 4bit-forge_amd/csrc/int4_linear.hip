@@ -156,16 +156,17 @@ __global__ __launch_bounds__(512) void int4_few_kernel(Int4Args a) {
 }
 
 // ---------------------------------------------------------------- many rows of x
-// 128 rows of x by 256 weight rows per workgroup, 64 columns a stage (mfma_tile.h), 8 wavefronts (2 along
-// x, 4 along the weights) of 64 x 64.  Every group's sum is formed by itself and folded into the totals
-// with its scale, one fma per output and group: that needs two sets of sums, which is why a wavefront
-// has 64 x 64 outputs and not 128 x 64.
+// 128 rows of x by 256 weight rows per workgroup, 64 columns a stage (mfma_tile.h).  A wavefront takes all of
+// the rows of x by 32 weight rows: a 32 x 16 fragment of W is one word per lane, converted by the only
+// wavefront that multiplies by it, a step ahead.  Conversions and matrix instructions of the two wavefronts on a SIMD hardly
+// overlap, and a stage is 16 of these (1024 clocks a SIMD) and about 120 others (944) for either; 64 x 64 outputs per
+// wavefront halve the reads of x from LDS (128 KB a stage, 1024 clocks) but convert every word twice: XXX us against YYY at
+// 8192 rows, 7168 -> 4096.  Converted once, into LDS, words cost 16 KB of writes and 64 KB of reads a stage.
+// Every group's sum is formed by itself and folded into the totals with its scale, one fma per output and
+// group: that needs two sets of sums, which is why a wavefront has 64 x 64 outputs' worth and not twice that.
 // x and the packed words go to LDS without registers, four stages ahead, the words in runs of 64 bytes
 // (two stages: a lane's own 16 bytes of its weight row, straight into registers, are a request each, and
-// 16 such loads a stage keep the address unit busy longer than the matrix pipe).  A 32 x 16 fragment
-// of W is one word per lane, converted by the wavefront that multiplies by it, a step ahead.  Both
-// wavefronts along x convert the same words; converted once, into LDS, they would cost 16 KB of writes
-// and 64 KB of reads a stage beside x's 64 KB, and the LDS was then the limit.
+// 16 such loads a stage keep the address unit busy longer than the matrix pipe).
 // Where groups end is fixed at compile time: 128 columns (two stages) hold FOLDS folds (1: groups of
 // 128 k or a single one; 2: of 64 k; 4: of 32 k).  The first product of a group starts from the
 // constant zero.
@@ -177,7 +178,6 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles,
     // (the epilogue takes half of the tile's 128 KB in f32 at a time)
     __shared__ __attribute__((aligned(1024))) char X0[kXBytes], X1[kXBytes], X2[kXBytes], X3[kXBytes], W0[256 * 64], W1[256 * 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wp = wave >> 2, wq = wave & 3;
     const int tile = xcd_tile(blockIdx.x, r_tiles * m_tiles);
     if (tile >= r_tiles * m_tiles) return;
     // runs of 8 tiles of x by all weight tiles
@@ -190,9 +190,9 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles,
     InnerLoader<2> lx;
     lx.init(lane, a.ldx, wave * 16);
     InnerFragment fx;
-    fx.init(lane, wp * 2);
+    fx.init(lane, 0);
 
-    const uint32_t sat = (uint32_t)((wq * 64 + lane) * a.G * 4); // lanes 0 .. 31: the first 32 weight rows' scales, 32 .. 63: the others'
+    const uint32_t sat = (uint32_t)((wave * 32 + (lane & 31)) * a.G * 4);
     // Words of two stages: row r at 64 r, its 16-byte piece c (2 (stage % 2) + lane / 32 of the reader) at
     // c ^ (r / 4 % 4).  What lies behind the row is a neighbour's (its x is zero) or outside the array: the
     // range check is per word, so a load across the array's end still gets the words inside.
@@ -201,30 +201,23 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles,
 #pragma unroll
         for (int j = 0; j < 2; ++j) load_to_lds(dw, W + (wave * 2 + j) * 1024, wat + (uint32_t)(j * 64 * a.words) + pair * 64);
     };
-    const uint32_t wfrom = (uint32_t)((wq * 64 + (lane & 31)) * 64);
-    auto read_words = [&](u32x4 (&w)[2], const char* W, int odd) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-            w[n] = *reinterpret_cast<const u32x4*>(W + wfrom + n * 2048 + (((odd * 2 + (lane >> 5)) ^ ((lane >> 2) & 3)) * 16));
+    const uint32_t wfrom = (uint32_t)((wave * 32 + (lane & 31)) * 64);
+    auto read_words = [&](u32x4& w, const char* W, int odd) {
+        w = *reinterpret_cast<const u32x4*>(W + wfrom + (((odd * 2 + (lane >> 5)) ^ ((lane >> 2) & 3)) * 16));
     };
     // words 0 .. 3 | 4 .. 7 of the two lanes to 0 2 4 6 | 1 3 5 7: word of step s is then 2 s + lane / 32
-    auto spread = [&](u32x4 (&w)[2]) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            auto p = __builtin_amdgcn_permlane32_swap(w[n][0], w[n][1], false, false);
-            auto q = __builtin_amdgcn_permlane32_swap(w[n][2], w[n][3], false, false);
-            w[n][0] = p[0]; w[n][2] = p[1];
-            w[n][1] = q[0]; w[n][3] = q[1];
-        }
+    auto spread = [&](u32x4& w) {
+        auto p = __builtin_amdgcn_permlane32_swap(w[0], w[1], false, false);
+        auto q = __builtin_amdgcn_permlane32_swap(w[2], w[3], false, false);
+        w[0] = p[0]; w[2] = p[1];
+        w[1] = q[0]; w[3] = q[1];
     };
 
-    f32x16_t total[2][2], acc[2][2];
+    f32x16_t total[4], acc[4];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) total[t][n][v] = 0.0f;
+        for (int v = 0; v < 16; ++v) total[t][v] = 0.0f;
     // The scales of the four stages of a turn's folds, each asked for when the turn before has used its
     // place: loads come back in order, so a wait for a young one is a wait for all x and words before it
     // (asked for two stages ahead they cost half of the kernel's time).
@@ -240,35 +233,29 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles,
         }
     };
     auto fold = [&](int i) {
-        const auto both = __builtin_amdgcn_permlane32_swap(sc[i], sc[i], false, false);
-        const float s2[2] = {__uint_as_float(both[0]), __uint_as_float(both[1])};
+        const float scale = __uint_as_float(sc[i]);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 4; ++t) {
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-#pragma unroll
-                for (int v = 0; v < 16; ++v) total[t][n][v] = __builtin_fmaf(s2[n], acc[t][n][v], total[t][n][v]);
-                // here and now: put off, several groups' sums would be alive at once, 64 registers each
-                asm volatile("" : "+v"(total[t][n]));
-            }
+            for (int v = 0; v < 16; ++v) total[t][v] = __builtin_fmaf(scale, acc[t][v], total[t][v]);
+            // here and now: put off, several groups' sums would be alive at once, 64 registers each
+            asm volatile("" : "+v"(total[t]));
+        }
         scales(i);
     };
     struct Step {
-        bf16x8_t p[2], q[2];
+        bf16x8_t p[4], q;
     };
-    auto prepare = [&](Step& f, const char* X, int s, const u32x4 (&w)[2]) {
+    auto prepare = [&](Step& f, const char* X, int s, const u32x4& w) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) f.p[t] = fx.read(X, t, s);
-#pragma unroll
-        for (int n = 0; n < 2; ++n) f.q[n] = nibbles(w[n][s]);
+        for (int t = 0; t < 4; ++t) f.p[t] = fx.read(X, t, s);
+        f.q = nibbles(w[s]);
     };
     auto multiply = [&](auto first, const Step& f) {
         const f32x16_t zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-                acc[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.p[t], f.q[n], decltype(first)::value ? zero : acc[t][n], 0, 0, 0);
+        for (int t = 0; t < 4; ++t)
+            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.p[t], f.q, decltype(first)::value ? zero : acc[t], 0, 0, 0);
         // a step's matrix instructions among the next step's reads (and conversions, as the compiler likes)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -280,7 +267,7 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles,
     Step f, h;
     // Stage s, the I-th of its turn; the next one's x in Xn.  w: its words (spread), wn: the next stage's;
     // W: this pair of stages' words, Wn: the next pair's
-    auto one_stage = [&](auto i, int s, char* X, const char* Xn, char* W, const char* Wn, u32x4 (&w)[2], u32x4 (&wn)[2]) {
+    auto one_stage = [&](auto i, int s, char* X, const char* Xn, char* W, const char* Wn, u32x4& w, u32x4& wn) {
         constexpr int I = decltype(i)::value;
         constexpr bool kFirst = I % 2 == 0 || FOLDS > 1, kLast = I % 2 == 1 || FOLDS > 1;
         prepare(h, X, 1, w);
@@ -309,7 +296,7 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles,
         multiply(std::false_type{}, h);
         if (kLast) fold(FOLDS == 1 ? I / 2 : FOLDS == 2 ? I : 2 * I + 1);
     };
-    u32x4 w0[2], w1[2];                                         // words of even and odd stages
+    u32x4 w0, w1;                                               // words of even and odd stages
     // in the loop's own order
     lx.stage(dx, X0, wave, a.ldx, 0, a.C);
     __builtin_amdgcn_sched_barrier(0);
@@ -344,22 +331,18 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles,
     }
     wait_loads<0>();
     __syncthreads();
-    // The tile goes through LDS as f32, 64 rows of x (one row of wavefronts) at a time, so that bias,
+    // The tile goes through LDS as f32, 64 rows of x at a time, so that bias,
     // residual and y are read and written in runs of 8 columns.  16 rows of 1 KB a buffer.
     // Register v of a tile: row 8 (v / 4) + 4 (lane / 32) + v % 4 of x, weight row lane & 31.
     auto quarter = [&](int i) { return reinterpret_cast<float*>(i == 0 ? X0 : i == 1 ? X1 : i == 2 ? X2 : X3); };
 #pragma unroll
     for (int pass = 0; pass < 2; ++pass) {
-        if (wp == pass) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int v = 0; v < 16; ++v)
-                        quarter(t * 2 + (v >> 3))[(8 * ((v >> 2) & 1) + 4 * (lane >> 5) + (v & 3)) * 256 + (wq * 2 + n) * 32 +
-                                                  (lane & 31)] = total[t][n][v] * kNibbleUnit;
-        }
+            for (int v = 0; v < 16; ++v)
+                quarter(t * 2 + (v >> 3))[(8 * ((v >> 2) & 1) + 4 * (lane >> 5) + (v & 3)) * 256 + wave * 32 + (lane & 31)] =
+                    total[pass * 2 + t][v] * kNibbleUnit;
         __syncthreads();
         // 32 threads a row, 16 rows at a time
         const int c = (threadIdx.x & 31) * 8, r = r0 + c;
