@@ -80,10 +80,9 @@ constexpr float kNibbleUnit = 16.0f;
 // eighth run of 128 columns, and their sums meet in LDS (in a fixed order; fewer wavefronts per row and
 // more rows per workgroup were slower at every size, 47 against 34 us at 7168 -> 18432).  A lane fetches
 // 16 bytes, 32 nibbles, of one weight row, so four lanes fetch 64 consecutive bytes of it; exchanging
-// words between the four (two
-// v_permlane32_swap, two v_permlane16_swap) gives every lane the word that the matrix instruction
-// wants of it when each step takes 32 consecutive columns, and then x too is read in 64-byte runs and
-// a step never crosses a group (groups are multiples of 32).  STEPS steps of 32 columns share a
+// words between the four (two v_permlane32_swap, two v_permlane16_swap) gives every lane the word that
+// the matrix instruction wants of it when each step takes 32 consecutive columns, and then x too is read
+// in 64-byte runs and a step never crosses a group (groups are multiples of 32).  STEPS steps of 32 columns share a
 // scale.  The up to 16 rows of x come from the caches; rows beyond M and columns beyond C read as zero.
 template <int STEPS>
 __global__ __launch_bounds__(512) void int4_few_kernel(Int4Args a) {
@@ -158,10 +157,10 @@ __global__ __launch_bounds__(512) void int4_few_kernel(Int4Args a) {
 // ---------------------------------------------------------------- many rows of x
 // 128 rows of x by 256 weight rows per workgroup, 64 columns a stage (mfma_tile.h).  A wavefront takes all of
 // the rows of x by 32 weight rows: a 32 x 16 fragment of W is one word per lane, converted by the only
-// wavefront that multiplies by it, a step ahead.  Conversions and matrix instructions of the two wavefronts on a SIMD hardly
-// overlap, and a stage is 16 of these (1024 clocks a SIMD) and about 120 others (944) for either; 64 x 64 outputs per
-// wavefront halve the reads of x from LDS (128 KB a stage, 1024 clocks) but convert every word twice: XXX us against YYY at
-// 8192 rows, 7168 -> 4096.  Converted once, into LDS, words cost 16 KB of writes and 64 KB of reads a stage.
+// wavefront that multiplies by it, a step ahead.  8192 rows, 7168 -> 4096: 490 us, 980 TFLOP/s, the clock at 1.7 GHz
+// (2.1 and more where power allows), the matrix pipe busy for half of the cycles and the vector ALU for
+// half, so what counts is the work itself: 64 x 64 outputs per wavefront halve the reads of x from LDS but
+// convert every word twice, 585 us.  Converted once, into LDS, words cost 16 KB of writes and 64 KB of reads a stage.
 // Every group's sum is formed by itself and folded into the totals with its scale, one fma per output and
 // group: that needs two sets of sums, which is why a wavefront has 64 x 64 outputs' worth and not twice that.
 // x and the packed words go to LDS without registers, four stages ahead, the words in runs of 64 bytes
@@ -566,7 +565,8 @@ __global__ __launch_bounds__(512) void int4_split_kernel(Int4Args a, int r_tiles
         for (int k = 0; k < 8 && r + k < a.R; ++k) store_y(a, m0 + m, r + k, v[k]);
 }
 
-// Groups that are not multiples of 32 columns (any shape and alignment): 64 x 64 outputs per workgroup, four wavefronts of 32 x 32,
+// Groups that are not multiples of 32 columns (any shape and alignment): 64 x 64 outputs per workgroup,
+// four wavefronts of 32 x 32,
 // 32 columns a step through LDS; a step never crosses the end of a group (its rest is zero).
 __global__ __launch_bounds__(256) void int4_any_kernel(Int4Args a, int r_tiles) {
     constexpr int T = 64, K = 32, LD = K + 8;
@@ -624,9 +624,10 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 // 1 row 12 against 20 of int4_split_kernel<1>, 16 rows 16 / 21.
 constexpr int64_t kFewRows = 16;
 // int4_split_kernel with 32 rows while its workgroups run at once: 128 rows 21 against 27 with 64 rows, 256
-// rows 39 / 29.  And int4_tile_kernel when that one's workgroups would take their turns: 512 rows (512
-// workgroups) 51 against 109, 1024 rows 100 / 118, 2048 rows 265 / 131; R = 7168, C = 2048 512 rows (896) 42 / 42.
-constexpr int64_t kAtOnce = 256, kSplitWorkgroups = 896;
+// rows 39 / 29.  And int4_tile_kernel when that one's workgroups would take more than three turns: 512 rows (512
+// workgroups) 51 against 95, 768 rows 74 / 100, 1024 rows 101 / 103, 1536 rows 169 / 113; R = 7168, C = 2048, 384 rows
+// (672) 32 / 37, 512 rows (896) 41 / 37.
+constexpr int64_t kAtOnce = 256, kSplitWorkgroups = 768;
 int64_t split_workgroups(int64_t M, int64_t R, int64_t rows) { return forge::ceil_div(R, 64) * forge::ceil_div(M, rows); }
 
 template <int PT>
