@@ -196,6 +196,11 @@ def _pieces(t) -> bool:
             and all(s % 8 == 0 for s in t.stride()[:-1]) and t.stride(-2) < 1 << 21)
 
 
+def _like(t):
+    """An empty dense tensor of t's shape and type (the quickest way there is, for single tokens)"""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _need_one_device(first, *tensors):
     """All on one GPU; returns it."""
     dev = first.device
@@ -227,7 +232,7 @@ class _HipKernels:
         """fn(*args, current stream of dev), with dev as the current device.  The operators that also
         serve single tokens go through here: a device guard and a Stream object cost several times what
         the launch does."""
-        if dev.index == torch.cuda.current_device():
+        if dev.index == torch._C._cuda_getDevice():
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
         else:
             with torch.cuda.device(dev):
@@ -945,10 +950,10 @@ class _HipKernels:
         T, C = x.shape
         ldx, ldr, rp, out, op = x.stride(0), 0, 0, None, 0
         assert x.stride(1) == 1 and weight.is_contiguous() and weight.numel() == C
-        y = torch.empty((T, C), dtype=x.dtype, device=dev)
+        y = _like(x)
         if residual is not None:
             assert residual.dtype == x.dtype and residual.shape == x.shape and residual.stride(1) == 1
-            out = torch.empty((T, C), dtype=x.dtype, device=dev)
+            out = _like(x)
             ldr, rp, op = max(residual.stride(0), C), residual.data_ptr(), out.data_ptr()
         self._launch(dev, self._lib.forge_rms_norm, x.data_ptr(), _dtype_code(x), max(ldx, C), rp, ldr,
                      weight.data_ptr(), _dtype_code(weight), T, C, float(eps), y.data_ptr(), op)
@@ -964,7 +969,7 @@ class _HipKernels:
         scale_inv = torch.empty((T, (C + 127) // 128), dtype=torch.float32, device=dev)
         if residual is not None:
             assert residual.dtype == x.dtype and residual.shape == x.shape and residual.stride(1) == 1
-            out = torch.empty((T, C), dtype=x.dtype, device=dev)
+            out = _like(x)
             ldr, rp, op = max(residual.stride(0), C), residual.data_ptr(), out.data_ptr()
         self._launch(dev, self._lib.forge_rms_norm_fp8, x.data_ptr(), _dtype_code(x), max(ldx, C), rp, ldr,
                      weight.data_ptr(), _dtype_code(weight), T, C, float(eps), codes.data_ptr(),
@@ -1078,7 +1083,7 @@ class _HipKernels:
         if group_size % 8 == 0 and not _pieces(x):
             x = self.pad_rows(x)                     # zeros: they meet the last word's spare nibbles
             C = x.shape[1]
-        y = torch.empty((M, R), dtype=torch.bfloat16, device=dev)
+        y = x.new_empty((M, R))
         self._launch(dev, self._lib.forge_linear_int4, x.data_ptr(), max(x.stride(0), C), packed.data_ptr(),
                      scale.data_ptr(), int(group_size), bp, rp, ldr, M, C, R, _act_code(activation),
                      y.data_ptr())
