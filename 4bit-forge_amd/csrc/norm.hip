@@ -81,6 +81,8 @@ __device__ __forceinline__ int cvt_fp8x2(float a, float b, int old, bool hi) {
               : __builtin_amdgcn_cvt_pk_fp8_f32(a, b, old, false);
 }
 
+// Bound by HBM: 8192 x 7168 bf16 with a residual 96 us, 4.9 TB/s (a copy reaches 4.8); 4099 x 2048 to 8 bits 13.0 us,
+// 4.5 TB/s; one row 3.9 us, the launch and one round trip.
 // LANES lanes per row, NCH runs of 8 columns per lane: lane t holds columns 8 (j LANES + t) .. + 7.
 // C a multiple of 8, at most 8 LANES NCH; 16-byte aligned rows.
 template <typename T, int LANES, int NCH, bool FP8>
