@@ -196,6 +196,17 @@ def _pieces(t) -> bool:
             and all(s % 8 == 0 for s in t.stride()[:-1]) and t.stride(-2) < 1 << 21)
 
 
+def _pitch(t) -> int:
+    """Distance of t's rows [..., R, C] in elements.  Rows that lie over each other are refused: the kernels
+    would read or write behind them."""
+    pitch, C = t.stride(-2), t.shape[-1]
+    if pitch >= C:
+        return pitch
+    if t.shape[-2] > 1:
+        raise RuntimeError(f"rows of {C} elements every {pitch} overlap: pass a contiguous copy")
+    return C
+
+
 def _like(t):
     """An empty dense tensor of t's shape and type (the quickest way there is, for single tokens)"""
     return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
@@ -948,14 +959,14 @@ class _HipKernels:
         without residual), both [T,C] of x's dtype."""
         dev = _need_one_device(x, weight, residual)
         T, C = x.shape
-        ldx, ldr, rp, out, op = x.stride(0), 0, 0, None, 0
+        ldx, ldr, rp, out, op = _pitch(x), 0, 0, None, 0
         assert x.stride(1) == 1 and weight.is_contiguous() and weight.numel() == C
         y = _like(x)
         if residual is not None:
             assert residual.dtype == x.dtype and residual.shape == x.shape and residual.stride(1) == 1
             out = _like(x)
-            ldr, rp, op = max(residual.stride(0), C), residual.data_ptr(), out.data_ptr()
-        self._launch(dev, self._lib.forge_rms_norm, x.data_ptr(), _dtype_code(x), max(ldx, C), rp, ldr,
+            ldr, rp, op = _pitch(residual), residual.data_ptr(), out.data_ptr()
+        self._launch(dev, self._lib.forge_rms_norm, x.data_ptr(), _dtype_code(x), ldx, rp, ldr,
                      weight.data_ptr(), _dtype_code(weight), T, C, float(eps), y.data_ptr(), op)
         return y, out
 
@@ -963,15 +974,15 @@ class _HipKernels:
         """The same with codes [T,C] float8_e4m3fn and scale_inv [T,ceil(C/128)] f32 in y's place."""
         dev = _need_one_device(x, weight, residual)
         T, C = x.shape
-        ldx, ldr, rp, out, op = x.stride(0), 0, 0, None, 0
+        ldx, ldr, rp, out, op = _pitch(x), 0, 0, None, 0
         assert x.stride(1) == 1 and weight.is_contiguous() and weight.numel() == C
         codes = torch.empty((T, C), dtype=torch.float8_e4m3fn, device=dev)
         scale_inv = torch.empty((T, (C + 127) // 128), dtype=torch.float32, device=dev)
         if residual is not None:
             assert residual.dtype == x.dtype and residual.shape == x.shape and residual.stride(1) == 1
             out = _like(x)
-            ldr, rp, op = max(residual.stride(0), C), residual.data_ptr(), out.data_ptr()
-        self._launch(dev, self._lib.forge_rms_norm_fp8, x.data_ptr(), _dtype_code(x), max(ldx, C), rp, ldr,
+            ldr, rp, op = _pitch(residual), residual.data_ptr(), out.data_ptr()
+        self._launch(dev, self._lib.forge_rms_norm_fp8, x.data_ptr(), _dtype_code(x), ldx, rp, ldr,
                      weight.data_ptr(), _dtype_code(weight), T, C, float(eps), codes.data_ptr(),
                      scale_inv.data_ptr(), op)
         return codes, scale_inv, out
@@ -988,7 +999,7 @@ class _HipKernels:
         B, R, C = t3.shape
         Rp, Cp = R if rows is None else int(rows), -(-C // 8) * 8
         out = torch.empty((B, Rp, Cp), dtype=t.dtype, device=dev)
-        self._launch(dev, self._lib.forge_pad_rows, t3.data_ptr(), t3.stride(0), max(t3.stride(1), C),
+        self._launch(dev, self._lib.forge_pad_rows, t3.data_ptr(), t3.stride(0), _pitch(t3),
                      out.data_ptr(), B, R, C, Rp, Cp, 0 if offsets is None else offsets.data_ptr())
         return out[0] if t.dim() == 2 else out
 
@@ -1015,14 +1026,13 @@ class _HipKernels:
         assert offsets.dtype == torch.int32 and offsets.is_contiguous() and offsets.numel() == E + 1
         assert rows.stride(1) == w_gate.stride(2) == w_up.stride(2) == 1 and w_up.shape == w_gate.shape
         rows, w_gate, w_up = self.gated_operands(rows, offsets, w_gate, w_up)
-        ws, ldw, _ = w_gate.stride()
         Ip, Hp = w_gate.shape[1:]
         h = torch.empty((N, Ip), dtype=torch.bfloat16, device=dev)
         g = u = None
         if keep:
             g, u = torch.empty((2, N, Ip), dtype=torch.float32, device=dev)
-        self._launch(dev, self._lib.forge_gated_rows, rows.data_ptr(), max(rows.stride(0), Hp),
-                     offsets.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), max(ldw, Hp), ws, N, E, Hp, Ip,
+        self._launch(dev, self._lib.forge_gated_rows, rows.data_ptr(), _pitch(rows),
+                     offsets.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _pitch(w_gate), w_gate.stride(0), N, E, Hp, Ip,
                      _act_code(activation), h.data_ptr(), g.data_ptr() if keep else 0,
                      u.data_ptr() if keep else 0)
         if Ip != I:
@@ -1045,7 +1055,6 @@ class _HipKernels:
         rows, w_gate, w_up = self.gated_operands(rows, offsets, w_gate, w_up)
         if not dh.is_contiguous() or Ip != I or dh.data_ptr() % 16:
             dh = self.pad_rows(_unit_rows(dh))
-        ws, ldw, _ = w_gate.stride()
         Hp = w_gate.shape[2]
         dx = torch.empty((N, Hp), dtype=torch.bfloat16, device=dev) if need[0] else None
         dwg = torch.empty((E, Ip, Hp), dtype=torch.bfloat16, device=dev) if need[1] else None
@@ -1054,8 +1063,8 @@ class _HipKernels:
         work = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
         ptr = lambda t: 0 if t is None else t.data_ptr()   # noqa: E731
         self._launch(dev, self._lib.forge_gated_rows_backward, dh.data_ptr(), g.data_ptr(), u.data_ptr(),
-                     rows.data_ptr(), max(rows.stride(0), Hp), offsets.data_ptr(), w_gate.data_ptr(),
-                     w_up.data_ptr(), max(ldw, Hp), ws, N, E, Hp, Ip, _act_code(activation), ptr(dx), ptr(dwg),
+                     rows.data_ptr(), _pitch(rows), offsets.data_ptr(), w_gate.data_ptr(),
+                     w_up.data_ptr(), _pitch(w_gate), w_gate.stride(0), N, E, Hp, Ip, _act_code(activation), ptr(dx), ptr(dwg),
                      ptr(dwu), work.data_ptr(), nbytes)
         if Hp != H or Ip != I:
             dx = None if dx is None else dx[:, :H]
@@ -1079,12 +1088,12 @@ class _HipKernels:
         if residual is not None:
             assert residual.dtype == torch.bfloat16 and residual.stride(1) == 1
             assert residual.shape[0] == M and residual.shape[1] == R
-            ldr, rp = max(residual.stride(0), R), residual.data_ptr()
+            ldr, rp = _pitch(residual), residual.data_ptr()
         if group_size % 8 == 0 and not _pieces(x):
             x = self.pad_rows(x)                     # zeros: they meet the last word's spare nibbles
             C = x.shape[1]
         y = x.new_empty((M, R))
-        self._launch(dev, self._lib.forge_linear_int4, x.data_ptr(), max(x.stride(0), C), packed.data_ptr(),
+        self._launch(dev, self._lib.forge_linear_int4, x.data_ptr(), _pitch(x), packed.data_ptr(),
                      scale.data_ptr(), int(group_size), bp, rp, ldr, M, C, R, _act_code(activation),
                      y.data_ptr())
         return y

@@ -131,7 +131,7 @@ class _GatedRows(torch.autograd.Function):
         h, g, u = kernels.gated_rows(rows, offsets, w_gate, w_up, activation, keep=True)
         ctx.save_for_backward(rows, offsets, w_gate, w_up, g, u)
         ctx.activation, ctx.sizes = activation, (H, I)
-        return h if h.shape[1] == I else h[:, :I]
+        return h if h.shape[1] == I else h[:, :I].contiguous()
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -199,7 +199,7 @@ def expert_gated_rows(rows: torch.Tensor, offsets: Union[torch.Tensor, Sequence[
     w_gate, w_up = _unit_rows(w_gate), _unit_rows(w_up)
     if torch.is_grad_enabled() and (rows.requires_grad or w_gate.requires_grad or w_up.requires_grad):
         return _GatedRows.apply(rows, off, w_gate, w_up, activation)
-    return kernels.gated_rows(rows, off, w_gate, w_up, activation)
+    return kernels.gated_rows(rows, off, w_gate, w_up, activation).contiguous()
 
 
 def linear_int4(x: torch.Tensor, packed: Dict[str, torch.Tensor], bias: Optional[torch.Tensor] = None,

@@ -173,3 +173,56 @@ def test_more_experts_than_a_workgroup_has_threads(hip, per):
     within(h[:n], want, bound)
     for got, (w, b) in zip((grads[0][:n], *grads[1:]), wants):
         within(got, w, b)
+
+
+def test_pitch_of_rows():
+    from forge.backend.hip import _pitch
+    t = torch.zeros(4, 24)
+    assert _pitch(t) == 24 and _pitch(t[:, 3:11]) == 24 and _pitch(t[::2]) == 48
+    assert _pitch(t[:1].as_strided((1, 24), (3, 1))) == 24 and _pitch(t[:0]) == 24
+    assert _pitch(torch.zeros(2, 4, 24)[:, :, :8]) == 24
+    for bad in (t[:1].expand(4, 24), t.as_strided((4, 24), (23, 1)), torch.zeros(2, 1, 8).expand(2, 3, 8)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            _pitch(bad)
+
+
+@pytest.mark.gpu
+def test_rows_over_each_other_are_refused_or_copied(hip):
+    """the kernels' calls refuse them, the engine's copy them"""
+    one = torch.randn(1, 64, device=DEV).bfloat16()
+    rows, w = one.expand(9, 64), torch.randn(1, 40, 64, device=DEV).bfloat16()
+    offs = torch.tensor([0, 9], dtype=torch.int32, device=DEV)
+    norm_w = torch.ones(64, device=DEV).bfloat16()
+    packed = torch.zeros(8, 8, dtype=torch.int32, device=DEV)
+    scale = torch.ones(8, 1, device=DEV)
+    dense = rows.contiguous()
+    h, g, u = hip.gated_rows(dense, offs, w, w, "silu", keep=True)
+    for call in (lambda: hip.rms_norm(rows, norm_w, 1e-6), lambda: hip.rms_norm(dense, norm_w, 1e-6, rows),
+                 lambda: hip.rms_norm_fp8(rows, norm_w, 1e-6), lambda: hip.gated_rows(rows, offs, w, w),
+                 lambda: hip.gated_rows_backward(h, g, u, rows, offs, w, w), lambda: hip.pad_rows(rows),
+                 lambda: hip.gated_rows(dense, offs, *2 * (w[:, :1].expand(1, 40, 64),)),
+                 lambda: hip.linear_int4(rows, packed, scale, 64),
+                 lambda: hip.linear_int4(dense, packed, scale, 64, None, None, one[:, :8].expand(9, 8))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            call()
+    assert torch.equal(engine.expert_gated_rows(rows, [0, 9], w, w), h)
+    assert torch.equal(engine.rms_norm(rows, norm_w), engine.rms_norm(dense, norm_w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("I", [40, 41])
+def test_the_result_is_a_tensor_of_its_own(hip, I):
+    """dense and free to be changed in place, whatever its width"""
+    g = torch.Generator(device=DEV).manual_seed(I)
+    mk = lambda *sh: (0.3 * torch.randn(*sh, generator=g, device=DEV)).bfloat16()   # noqa: E731
+    x, wg, wu = mk(10, 24), mk(2, I, 24), mk(2, I, 24)
+    plain = engine.expert_gated_rows(x, [0, 4, 10], wg, wu)
+    assert plain.is_contiguous() and plain.shape == (10, I)
+    leaf = x.clone().requires_grad_(True)
+    h = engine.expert_gated_rows(leaf, [0, 4, 10], wg, wu)
+    assert h.is_contiguous() and torch.equal(h, plain)
+    h.mul_(2)
+    h.sum().backward()
+    again = x.clone().requires_grad_(True)
+    engine.expert_gated_rows(again, [0, 4, 10], wg, wu).backward(torch.full_like(plain, 2.0))
+    assert torch.equal(leaf.grad, again.grad)
