@@ -78,7 +78,7 @@ constexpr float kNibbleUnit = 16.0f;
 // ---------------------------------------------------------------- few rows of x
 // Bound by the packed words, which are read once: a workgroup takes 16 weight rows, its 8 wavefronts every
 // eighth run of 128 columns, and their sums meet in LDS (in a fixed order; fewer wavefronts per row and
-// more rows per workgroup were slower at every size, 47 against 34 us at 7168 -> 18432).  A lane fetches
+// more rows per workgroup were slower at every size, 47 against 34 us then at 7168 -> 18432).  A lane fetches
 // 16 bytes, 32 nibbles, of one weight row, so four lanes fetch 64 consecutive bytes of it; exchanging
 // words between the four (two v_permlane32_swap, two v_permlane16_swap) gives every lane the word that
 // the matrix instruction wants of it when each step takes 32 consecutive columns, and then x too is read
@@ -88,7 +88,6 @@ template <int STEPS>
 __global__ __launch_bounds__(512) void int4_few_kernel(Int4Args a) {
     using namespace forge;
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    constexpr int U = 4;                                        // runs in flight per wavefront
     __shared__ float part[8][256];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, kb = lane >> 4;
@@ -98,47 +97,41 @@ __global__ __launch_bounds__(512) void int4_few_kernel(Int4Args a) {
     const __amdgpu_buffer_rsrc_t dx = descriptor(a.x, (uint32_t)(((a.M - 1) * a.ldx + a.C) * 2));
     f32x4_t total = {0.0f, 0.0f, 0.0f, 0.0f};
     const int runs = (a.C + 127) / 128;
-    for (int c0 = wave; c0 < runs; c0 += 8 * U) {
-        u32x4 w[U], x[U][4];
-        float sc[U][4 / STEPS];
+    // One run at a time: the other wavefronts' are on their way meanwhile (two or four of each asked for at once
+    // keep wavefronts off the CU: 2048 -> 7168, 1 row 7.8 us with one, 9.5 with four; 7168 -> 18432 28.8 / 31.5)
+    for (int c = wave; c < runs; c += 8) {
+        u32x4 x[4];
+        float sc[4 / STEPS];
+        // (words behind the row are a neighbour's, their x is zero, or outside the array)
+        u32x4 q = __builtin_amdgcn_raw_buffer_load_b128(dw, (n * a.words + c * 16 + kb * 4) * 4, 0, 0);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int c = c0 + 8 * u;
-            // (words behind the row are a neighbour's, their x is zero, or outside the array)
-            w[u] = __builtin_amdgcn_raw_buffer_load_b128(dw, (n * a.words + c * 16 + kb * 4) * 4, 0, 0);
-#pragma unroll
-            for (int i = 0; i < 4 / STEPS; ++i) {
-                const int k = c * 128 + i * STEPS * 32;
-                sc[u][i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
-                    ds, k < a.C ? (n * a.G + k / a.gs) * 4 : (int)kOutside, 0, 0));
-            }
-#pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                const int k = c * 128 + d * 32 + kb * 8;
-                x[u][d] = __builtin_amdgcn_raw_buffer_load_b128(
-                    dx, k < a.C && n < a.M ? (int)((n * a.ldx + k) * 2) : (int)kOutside, 0, 0);
-            }
+        for (int i = 0; i < 4 / STEPS; ++i) {
+            const int k = c * 128 + i * STEPS * 32;
+            sc[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                ds, k < a.C ? (n * a.G + k / a.gs) * 4 : (int)kOutside, 0, 0));
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            u32x4& q = w[u];
-            auto s = __builtin_amdgcn_permlane32_swap(q[0], q[2], false, false);
-            q[0] = s[0]; q[2] = s[1];
-            s = __builtin_amdgcn_permlane32_swap(q[1], q[3], false, false);
-            q[1] = s[0]; q[3] = s[1];
-            s = __builtin_amdgcn_permlane16_swap(q[0], q[1], false, false);
-            q[0] = s[0]; q[1] = s[1];
-            s = __builtin_amdgcn_permlane16_swap(q[2], q[3], false, false);
-            q[2] = s[0]; q[3] = s[1];
-            f32x4_t acc;
+        for (int d = 0; d < 4; ++d) {
+            const int k = c * 128 + d * 32 + kb * 8;
+            x[d] = __builtin_amdgcn_raw_buffer_load_b128(
+                dx, k < a.C && n < a.M ? (int)((n * a.ldx + k) * 2) : (int)kOutside, 0, 0);
+        }
+        auto s = __builtin_amdgcn_permlane32_swap(q[0], q[2], false, false);
+        q[0] = s[0]; q[2] = s[1];
+        s = __builtin_amdgcn_permlane32_swap(q[1], q[3], false, false);
+        q[1] = s[0]; q[3] = s[1];
+        s = __builtin_amdgcn_permlane16_swap(q[0], q[1], false, false);
+        q[0] = s[0]; q[1] = s[1];
+        s = __builtin_amdgcn_permlane16_swap(q[2], q[3], false, false);
+        q[2] = s[0]; q[3] = s[1];
+        f32x4_t acc;
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                if (d % STEPS == 0) acc = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x[u][d]), nibbles(q[d]), acc, 0, 0, 0);
-                if (d % STEPS == STEPS - 1)
+        for (int d = 0; d < 4; ++d) {
+            if (d % STEPS == 0) acc = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x[d]), nibbles(q[d]), acc, 0, 0, 0);
+            if (d % STEPS == STEPS - 1)
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) total[v] = __builtin_fmaf(sc[u][d / STEPS], acc[v], total[v]);
-            }
+                for (int v = 0; v < 4; ++v) total[v] = __builtin_fmaf(sc[d / STEPS], acc[v], total[v]);
         }
     }
     // register v: row 4 (lane / 16) + v of x, weight row lane & 15
@@ -621,7 +614,7 @@ __global__ __launch_bounds__(256) void int4_any_kernel(Int4Args a, int r_tiles) 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Which kernel (us, C = 7168, R = 4096; 256 workgroups run at a time).  int4_few_kernel, for a few rows of x:
-// 1 row 12 against 20 of int4_split_kernel<1>, 16 rows 16 / 21.
+// 1 row 10.5 against 20 of int4_split_kernel<1>, 16 rows 14 / 21.
 constexpr int64_t kFewRows = 16;
 // int4_split_kernel with 32 rows while its workgroups run at once: 128 rows 21 against 27 with 64 rows, 256
 // rows 39 / 29.  And int4_tile_kernel when that one's workgroups would take more than three turns: 512 rows (512
