@@ -183,28 +183,35 @@ def _unit_rows(t):
     another without overlapping); anything else is copied."""
     stride, shape = t.stride(), t.shape
     if stride[-1] == 1:
+        if t.is_contiguous():
+            return t
         for i in range(len(shape) - 1):
             if stride[i] < stride[i + 1] * shape[i + 1]:
                 return t.contiguous()
         return t
-    return t.contiguous()
+    # (a single column may have any stride and still count as contiguous)
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _pieces(t) -> bool:
     """Rows that start on 16-byte boundaries and are whole 16-byte pieces long (16-bit elements)."""
-    return (t.shape[-1] % 8 == 0 and t.data_ptr() % 16 == 0 and t.stride(-1) == 1
-            and all(s % 8 == 0 for s in t.stride()[:-1]) and t.stride(-2) < 1 << 21)
+    if t.shape[-1] % 8 or t.data_ptr() % 16:
+        return False
+    if t.is_contiguous():
+        return t.shape[-1] < 1 << 21
+    stride = t.stride()
+    return stride[-1] == 1 and stride[-2] < 1 << 21 and not any(s % 8 for s in stride[:-1])
 
 
 def _pitch(t) -> int:
     """Distance of t's rows [..., R, C] in elements.  Rows that lie over each other are refused: the kernels
     would read or write behind them."""
     pitch, C = t.stride(-2), t.shape[-1]
-    if pitch >= C:
-        return pitch
-    if t.shape[-2] > 1:
+    if t.shape[-2] <= 1:
+        return C
+    if pitch < C:
         raise RuntimeError(f"rows of {C} elements every {pitch} overlap: pass a contiguous copy")
-    return C
+    return pitch
 
 
 def _like(t):
@@ -215,11 +222,15 @@ def _like(t):
 def _need_one_device(first, *tensors):
     """All on one GPU; returns it."""
     dev = first.device
-    if dev.type != "cuda" or any(t is not None and t.device != dev for t in tensors):
-        _need_cuda(first, *tensors)
-        raise RuntimeError("tensors on different devices: "
-                           f"{sorted({str(t.device) for t in (first, *tensors) if t is not None})}")
-    return dev
+    one = dev.type == "cuda"
+    for t in tensors:
+        if t is not None and t.device != dev:
+            one = False
+    if one:
+        return dev
+    _need_cuda(first, *tensors)
+    raise RuntimeError("tensors on different devices: "
+                       f"{sorted({str(t.device) for t in (first, *tensors) if t is not None})}")
 
 
 def _need_cuda(*tensors):

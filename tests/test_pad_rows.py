@@ -186,6 +186,32 @@ def test_pitch_of_rows():
             _pitch(bad)
 
 
+def test_unit_rows():
+    from forge.backend.hip import _pieces, _unit_rows
+    t = torch.zeros(4, 24, dtype=torch.bfloat16)
+    assert _unit_rows(t) is t and _unit_rows(t[:, 3:11]).data_ptr() == t[:, 3:11].data_ptr()
+    for odd in (t.t(), t[:1].expand(4, 24), torch.zeros(1, 5).t(), torch.zeros(1, 5, 7).transpose(0, 2)[..., :1]):
+        u = _unit_rows(odd)
+        assert u.stride(-1) == 1 and u.is_contiguous() and torch.equal(u, odd)
+    assert _pieces(t) and not _pieces(t[:, :23]) and not _pieces(t[:, 1:17]) and _pieces(t[:, 8:16])
+    assert not _pieces(torch.zeros(4, 27, dtype=torch.bfloat16)[:, :8])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 5])
+def test_a_single_column_of_any_stride(hip, rows):
+    mk = lambda *sh: torch.randn(*sh, device=DEV).bfloat16()   # noqa: E731
+    x, w = mk(1, rows).t(), mk(3, 1, 1).transpose(1, 2)
+    norm_w = mk(1)
+    assert torch.equal(engine.rms_norm(x, norm_w), engine.rms_norm(x.clone(memory_format=torch.contiguous_format), norm_w))
+    offs = [0, rows, rows, rows]
+    assert torch.equal(engine.expert_gated_rows(x, offs, w, w),
+                       engine.expert_gated_rows(x.clone(memory_format=torch.contiguous_format), offs, w, w))
+    rec = dict(weight_packed=torch.full((8, 1), 0x7, dtype=torch.int32, device=DEV),
+               weight_scale=torch.ones(8, 1, device=DEV), weight_shape=torch.tensor([8, 1]))
+    assert torch.equal(engine.linear_int4(x, rec), (-x).expand(rows, 8))
+
+
 @pytest.mark.gpu
 def test_rows_over_each_other_are_refused_or_copied(hip):
     """the kernels' calls refuse them, the engine's copy them"""
