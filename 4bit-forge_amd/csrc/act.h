@@ -45,6 +45,21 @@ __device__ __forceinline__ float act_f32(int act, float v) {
     }
 }
 
+// out = act(v) * times, N values: the activation is looked at once, so that the values' chains overlap
+template <int N, typename V>
+__device__ __forceinline__ void act_times(int act, const V& v, const V& times, float (&out)[N]) {
+    auto all = [&](int fixed) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) out[i] = act_f32(fixed, v[i]) * times[i];
+    };
+    switch (act) {
+        case FORGE_ACT_SILU: all(FORGE_ACT_SILU); break;
+        case FORGE_ACT_GELU: all(FORGE_ACT_GELU); break;
+        case FORGE_ACT_RELU: all(FORGE_ACT_RELU); break;
+        default: all(FORGE_ACT_NONE);
+    }
+}
+
 // the activation and its derivative
 __device__ __forceinline__ void act_grad_f32(int act, float v, float& a, float& da) {
     switch (act) {

@@ -160,30 +160,34 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
         asm volatile("" : "+v"(lane_e));
         const int q = row0 + (lane_e & 31);
         lds_char* row = buffer(row0 / kRows) + (q % kRows) * (kCols * 2) + (lane_e >> 5) * 8;
+        float h[16];
+        if constexpr (MODE == FORWARD) {
+            if (a.g && q < r.rows) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float h[4];
-            if constexpr (MODE == FORWARD) {
-                f32x4_t g, u;
+                for (int j = 0; j < 4; ++j) {
+                    f32x4_t g, u;
 #pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    g[v] = x[4 * j + v];
-                    u[v] = y[4 * j + v];
-                    h[v] = act_f32(a.act, g[v]) * u[v];
-                }
-                const int i = p0 + block * 32 + 8 * j + 4 * (lane_e >> 5);
-                if (a.g && q < r.rows && i < a.I) {
+                    for (int v = 0; v < 4; ++v) {
+                        g[v] = x[4 * j + v];
+                        u[v] = y[4 * j + v];
+                    }
+                    const int i = p0 + block * 32 + 8 * j + 4 * (lane_e >> 5);
                     const int64_t at = (int64_t)(r.row0 + q) * a.I + i;
-                    *reinterpret_cast<f32x4_t*>(a.g + at) = g;
-                    *reinterpret_cast<f32x4_t*>(a.u + at) = u;
+                    if (i < a.I) {
+                        *reinterpret_cast<f32x4_t*>(a.g + at) = g;
+                        *reinterpret_cast<f32x4_t*>(a.u + at) = u;
+                    }
                 }
-            } else {
-#pragma unroll
-                for (int v = 0; v < 4; ++v) h[v] = x[4 * j + v];
             }
-            *(__attribute__((address_space(3))) u32x2*)(row + (((block * 4 + j) ^ (q % kPieces)) * 16)) =
-                u32x2{pack_bf16(h[0], h[1]), pack_bf16(h[2], h[3])};
+            act_times(a.act, x, y, h);
+        } else {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) h[v] = x[v];
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            *(__attribute__((address_space(3))) u32x2*)(row + (((block * 4 + j) ^ (q % kPieces)) * 16)) =
+                u32x2{pack_bf16(h[4 * j], h[4 * j + 1]), pack_bf16(h[4 * j + 2], h[4 * j + 3])};
     };
     auto clear = [](auto& acc, int n_p, int n_q) {
 #pragma unroll
