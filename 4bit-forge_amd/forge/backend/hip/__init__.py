@@ -1037,18 +1037,23 @@ class _HipKernels:
         assert offsets.dtype == torch.int32 and offsets.is_contiguous() and offsets.numel() == E + 1
         assert rows.stride(1) == w_gate.stride(2) == w_up.stride(2) == 1 and w_up.shape == w_gate.shape
         rows, w_gate, w_up = self.gated_operands(rows, offsets, w_gate, w_up)
-        Ip, Hp = w_gate.shape[1:]
+        h, g, u = self.gated_rows_of_operands(dev, rows, offsets, w_gate, w_up, _act_code(activation), keep)
+        if w_gate.shape[1] != I:
+            h = h[:, :I]
+        return (h, g, u) if keep else h
+
+    def gated_rows_of_operands(self, dev, rows, offsets, w_gate, w_up, act, keep):
+        """gated_rows on what gated_operands returned: (h, g, u), g and u None without keep."""
+        E, Ip, Hp = w_gate.shape
+        N = rows.shape[0]
         h = torch.empty((N, Ip), dtype=torch.bfloat16, device=dev)
         g = u = None
         if keep:
             g, u = torch.empty((2, N, Ip), dtype=torch.float32, device=dev)
         self._launch(dev, self._lib.forge_gated_rows, rows.data_ptr(), _pitch(rows),
-                     offsets.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _pitch(w_gate), w_gate.stride(0), N, E, Hp, Ip,
-                     _act_code(activation), h.data_ptr(), g.data_ptr() if keep else 0,
-                     u.data_ptr() if keep else 0)
-        if Ip != I:
-            h = h[:, :I]
-        return (h, g, u) if keep else h
+                     offsets.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _pitch(w_gate), w_gate.stride(0),
+                     N, E, Hp, Ip, act, h.data_ptr(), g.data_ptr() if keep else 0, u.data_ptr() if keep else 0)
+        return h, g, u
 
     def gated_rows_backward(self, dh, g, u, rows, offsets, w_gate, w_up, activation="silu",
                             need=(True, True, True)):
@@ -1064,22 +1069,30 @@ class _HipKernels:
         assert rows.stride(1) == w_gate.stride(2) == w_up.stride(2) == 1
         assert w_up.shape == w_gate.shape and tuple(rows.shape) == (N, H)
         rows, w_gate, w_up = self.gated_operands(rows, offsets, w_gate, w_up)
-        if not dh.is_contiguous() or Ip != I or dh.data_ptr() % 16:
+        if Ip != I:
             dh = self.pad_rows(_unit_rows(dh))
-        Hp = w_gate.shape[2]
-        dx = torch.empty((N, Hp), dtype=torch.bfloat16, device=dev) if need[0] else None
-        dwg = torch.empty((E, Ip, Hp), dtype=torch.bfloat16, device=dev) if need[1] else None
-        dwu = torch.empty((E, Ip, Hp), dtype=torch.bfloat16, device=dev) if need[2] else None
-        nbytes = int(self._lib.forge_gated_rows_backward_workspace_bytes(N, Ip))
-        work = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-        ptr = lambda t: 0 if t is None else t.data_ptr()   # noqa: E731
-        self._launch(dev, self._lib.forge_gated_rows_backward, dh.data_ptr(), g.data_ptr(), u.data_ptr(),
-                     rows.data_ptr(), _pitch(rows), offsets.data_ptr(), w_gate.data_ptr(),
-                     w_up.data_ptr(), _pitch(w_gate), w_gate.stride(0), N, E, Hp, Ip, _act_code(activation), ptr(dx), ptr(dwg),
-                     ptr(dwu), work.data_ptr(), nbytes)
-        if Hp != H or Ip != I:
+        dx, dwg, dwu = self.gated_gradients_of_operands(dev, dh, g, u, rows, offsets, w_gate, w_up,
+                                                        _act_code(activation), need)
+        if w_gate.shape[2] != H or Ip != I:
             dx = None if dx is None else dx[:, :H]
             dwg, dwu = (None if d is None else d[:, :I, :H] for d in (dwg, dwu))
+        return dx, dwg, dwu
+
+    def gated_gradients_of_operands(self, dev, dh, g, u, rows, offsets, w_gate, w_up, act, need):
+        """gated_rows_backward on what gated_operands returned, dh as wide as g."""
+        if not dh.is_contiguous() or dh.data_ptr() % 16:
+            dh = self.pad_rows(_unit_rows(dh))
+        E, Ip, Hp = w_gate.shape
+        N = rows.shape[0]
+        dx = _like(rows) if need[0] else None
+        dwg = _like(w_gate) if need[1] else None
+        dwu = _like(w_up) if need[2] else None
+        nbytes = self._lib.forge_gated_rows_backward_workspace_bytes(N, Ip)
+        work = torch.empty(nbytes or 16, dtype=torch.uint8, device=dev)
+        self._launch(dev, self._lib.forge_gated_rows_backward, dh.data_ptr(), g.data_ptr(), u.data_ptr(),
+                     rows.data_ptr(), _pitch(rows), offsets.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
+                     _pitch(w_gate), w_gate.stride(0), N, E, Hp, Ip, act, dx.data_ptr() if need[0] else 0,
+                     dwg.data_ptr() if need[1] else 0, dwu.data_ptr() if need[2] else 0, work.data_ptr(), nbytes)
         return dx, dwg, dwu
 
     def linear_int4(self, x, packed, scale, group_size, bias=None, activation=None, residual=None):

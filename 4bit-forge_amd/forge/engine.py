@@ -10,7 +10,7 @@ from typing import Dict, Optional, Sequence, Tuple, Union
 
 import torch
 
-from forge.backend.hip import kernels, _unit_rows, ACTIVATIONS
+from forge.backend.hip import kernels, _need_one_device, _unit_rows, ACTIVATIONS
 
 
 @torch.no_grad()
@@ -126,23 +126,27 @@ class _GatedRows(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, offsets, w_gate, w_up, activation):
         I, H = w_gate.shape[1:]
+        dev = _need_one_device(rows, offsets, w_gate, w_up)
         # odd sizes: the padded copies are kept, so that the backward pass need not make them again
         rows, w_gate, w_up = kernels.gated_operands(rows, offsets, w_gate, w_up)
-        h, g, u = kernels.gated_rows(rows, offsets, w_gate, w_up, activation, keep=True)
+        act = ACTIVATIONS[activation]
+        h, g, u = kernels.gated_rows_of_operands(dev, rows, offsets, w_gate, w_up, act, True)
         ctx.save_for_backward(rows, offsets, w_gate, w_up, g, u)
-        ctx.activation, ctx.sizes = activation, (H, I)
+        ctx.sizes = dev, act, H, I
         return h if h.shape[1] == I else h[:, :I].contiguous()
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
+        if torch.is_grad_enabled():
+            # (once_differentiable would let a graph pass whose saved tensors alone ask for gradients)
+            raise RuntimeError("expert_gated_rows has no gradients of its gradients (create_graph=True)")
         rows, offsets, w_gate, w_up, g, u = ctx.saved_tensors
-        H, I = ctx.sizes
-        need = (ctx.needs_input_grad[0], ctx.needs_input_grad[2], ctx.needs_input_grad[3])
+        dev, act, H, I = ctx.sizes
+        need = ctx.needs_input_grad
         if g.shape[1] != I:
             dh = kernels.pad_rows(_unit_rows(dh))
-        dx, dwg, dwu = kernels.gated_rows_backward(dh, g, u, rows, offsets, w_gate, w_up,
-                                                   ctx.activation, need)
+        dx, dwg, dwu = kernels.gated_gradients_of_operands(dev, dh, g, u, rows, offsets, w_gate, w_up, act,
+                                                           (need[0], need[2], need[3]))
         if rows.shape[1] != H or g.shape[1] != I:
             dx = None if dx is None else dx[:, :H]
             dwg, dwu = (None if d is None else d[:, :I, :H] for d in (dwg, dwu))
@@ -162,7 +166,7 @@ def expert_gated_rows(rows: torch.Tensor, offsets: Union[torch.Tensor, Sequence[
     from offsets[E] on) get 0.  activation: "silu", "gelu" (tanh form), "relu" or None.
     Sums in f32, h [N, I] bf16 rounded once.
 
-    Differentiable in rows, w_gate and w_up (once); gradients are bf16, with dg and du rounded to
+    Differentiable in rows, w_gate and w_up (once: create_graph is refused); gradients are bf16, with dg and du rounded to
     bf16 between the products.  A HIP graph of a training step captures ``kernels.gated_rows(...,
     keep=True)`` and ``kernels.gated_rows_backward`` directly, not autograd's engine."""
     if activation not in ACTIVATIONS:

@@ -67,3 +67,22 @@ def test_weights_behind_two_to_the_31st_element(hip):
     for got, (w, b) in zip((dx, dwg[-1:], dwu[-1:]), wants):
         within(got, w, b)
     assert not dwg[:-1].any() and not dwu[:-1].any()
+
+
+@pytest.mark.parametrize("I", [40, 41])
+def test_gradients_of_gradients_are_refused(hip, I):
+    g = torch.Generator(device=DEV).manual_seed(I)
+    mk = lambda *sh: (0.3 * torch.randn(*sh, generator=g, device=DEV)).bfloat16()   # noqa: E731
+    x, wg, wu = (t.requires_grad_(True) for t in (mk(10, 24), mk(2, I, 24), mk(2, I, 24)))
+    h = engine.expert_gated_rows(x, [0, 4, 10], wg, wu)
+    for leaf in (x, wg, wu):                          # also where the incoming gradient asks for none
+        with pytest.raises(RuntimeError, match="gradients of its gradients"):
+            torch.autograd.grad(h.sum(), leaf, create_graph=True)
+    torch.autograd.grad(h.sum(), (x, wg, wu))
+
+
+def test_tensors_on_different_devices_are_refused_in_training(hip):
+    x = torch.randn(4, 16, device=DEV).bfloat16().requires_grad_(True)
+    w = torch.randn(1, 8, 16).bfloat16()
+    with pytest.raises(RuntimeError):
+        engine.expert_gated_rows(x, [0, 4], w, w)
