@@ -306,8 +306,9 @@ __global__ __launch_bounds__(512) void gated_dweights_kernel(GatedArgs a, int p_
     __shared__ int slot[2];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wp = wave >> 2, wq = wave & 3;
-    // Every XCD takes an eighth of every expert's tiles: those of up to 8 tiles of Q by some of P, which share
-    // their panels in its L2.  Q counts the gate's tiles, then the up projection's.
+    // Every XCD takes an eighth of every expert's tiles: those of up to 4 tiles of Q by some of P, which share
+    // their panels in its L2 (by 8 or 16 of Q a panel is met again too late: 541 against 528 us with 8168 rows of
+    // 16 experts).  Q counts the gate's tiles, then the up projection's.
     const int tiles = p_tiles * q_tiles, per = (tiles + 7) / 8, t0 = (blockIdx.x % 8) * per;
     const int here = min(tiles - t0, per), items = here > 0 ? here * a.E : 0, workers = gridDim.x / 8;
     const int first = blockIdx.x / 8;
@@ -321,9 +322,9 @@ __global__ __launch_bounds__(512) void gated_dweights_kernel(GatedArgs a, int p_
     auto tile_at = [&](int item) {
         Tile t;
         t.expert = item / here;
-        const int c = t0 + item - t.expert * here, group = c / (8 * p_tiles), in_group = c - group * 8 * p_tiles;
-        const int wide = min(q_tiles - group * 8, 8), up_from = (a.I + kTile - 1) / kTile;
-        const int q = group * 8 + in_group % wide;
+        const int c = t0 + item - t.expert * here, group = c / (4 * p_tiles), in_group = c - group * 4 * p_tiles;
+        const int wide = min(q_tiles - group * 4, 4), up_from = (a.I + kTile - 1) / kTile;
+        const int q = group * 4 + in_group % wide;
         t.which = q >= up_from;
         t.p0 = in_group / wide * kTile;
         t.q0 = (t.which ? q - up_from : q) * kTile;
@@ -738,7 +739,7 @@ int few_tile(int64_t N, int64_t E) { return N <= 32 || N <= 16 * E ? 16 : N <= 6
 
 // From so many rows per expert on a workgroup per tile does better than one per CU (gated_dweights_kernel), whose
 // stages are fetched less far ahead: 7168 x 2048, us, per CU against per tile: 16 experts of 64 rows 212 / 256, 16
-// with 8168 rows by popularity 545 / 630, of 1024 rows 905 / 975, 8 of 2048 rows 831 / 811, 4 of 4096 rows 790 / 742,
+// with 8168 rows by popularity 528 / 630, of 1024 rows 905 / 975, 8 of 2048 rows 831 / 811, 4 of 4096 rows 790 / 742,
 // one of 8192 411 / 365
 constexpr int64_t kLongExperts = 2048;
 

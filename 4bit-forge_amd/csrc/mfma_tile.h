@@ -148,15 +148,12 @@ struct Fragments {
 #pragma unroll
         for (int t = 0; t < NP; ++t) p[t] = fp.read(P, t * SKIP, s);
     }
-    // FIRST: the sums start from zero, which the matrix instruction takes as a constant
-    template <bool FIRST = false>
     __device__ __forceinline__ void multiply(f32x16_t (&acc)[NP][NQ]) const {
-        const f32x16_t zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
         for (int t = 0; t < NP; ++t)
 #pragma unroll
             for (int n = 0; n < NQ; ++n)
-                acc[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[t], q[n], FIRST ? zero : acc[t][n], 0, 0, 0);
+                acc[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[t], q[n], acc[t][n], 0, 0, 0);
     }
 };
 
