@@ -579,8 +579,9 @@ int forge_gated_rows(const void* rows, int64_t ldx, const int32_t* offsets, cons
  *   drows = dg Wg + du Wu [N, H],  dWg[e] = dg_e^T x_e,  dWu[e] = du_e^T x_e [E, I, H]
  * all bf16 contiguous, sums in f32; any of the three may be NULL.  Rows of no expert: drows = 0 (what
  * dh holds there is not read into any gradient); experts without rows: dW = 0.  Alignment as above.
- * ws: device workspace of forge_gated_rows_backward_workspace_bytes(N, I), 16-byte aligned.  Results
- * do not depend on the order in which workgroups run. */
+ * ws: device workspace of forge_gated_rows_backward_workspace_bytes(N, I), 16-byte aligned, of no
+ * initial value, this call's alone until its launches have ended.  Results do not depend on the order in
+ * which workgroups run. */
 int forge_gated_rows_backward(const void* dh, const float* g, const float* u, const void* rows,
                               int64_t ldx, const int32_t* offsets, const void* Wg, const void* Wu,
                               int64_t ldw, int64_t w_stride, int64_t N, int64_t E, int64_t H,
