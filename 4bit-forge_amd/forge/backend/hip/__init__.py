@@ -968,32 +968,42 @@ class _HipKernels:
     def rms_norm(self, x, weight, eps, residual=None):
         """x, residual [T,C] bf16/f32 (unit column stride), weight [C] -> y, residual out (None
         without residual), both [T,C] of x's dtype."""
+        self._check_norm(x, weight, residual)
+        return self.rms_norm_of_checked(x, weight, eps, residual)
+
+    def _check_norm(self, x, weight, residual):
+        assert x.stride(1) == 1 and weight.is_contiguous() and weight.numel() == x.shape[1]
+        assert residual is None or (residual.dtype == x.dtype and residual.shape == x.shape
+                                    and residual.stride(1) == 1)
+
+    def rms_norm_of_checked(self, x, weight, eps, residual):
+        """rms_norm on arguments whose shapes and strides are known to fit."""
         dev = _need_one_device(x, weight, residual)
         T, C = x.shape
-        ldx, ldr, rp, out, op = _pitch(x), 0, 0, None, 0
-        assert x.stride(1) == 1 and weight.is_contiguous() and weight.numel() == C
-        y = _like(x)
+        y, out, ldr, rp, op = _like(x), None, 0, 0, 0
         if residual is not None:
-            assert residual.dtype == x.dtype and residual.shape == x.shape and residual.stride(1) == 1
             out = _like(x)
             ldr, rp, op = _pitch(residual), residual.data_ptr(), out.data_ptr()
-        self._launch(dev, self._lib.forge_rms_norm, x.data_ptr(), _dtype_code(x), ldx, rp, ldr,
+        self._launch(dev, self._lib.forge_rms_norm, x.data_ptr(), _dtype_code(x), _pitch(x), rp, ldr,
                      weight.data_ptr(), _dtype_code(weight), T, C, float(eps), y.data_ptr(), op)
         return y, out
 
     def rms_norm_fp8(self, x, weight, eps, residual=None):
         """The same with codes [T,C] float8_e4m3fn and scale_inv [T,ceil(C/128)] f32 in y's place."""
+        self._check_norm(x, weight, residual)
+        return self.rms_norm_fp8_of_checked(x, weight, eps, residual)
+
+    def rms_norm_fp8_of_checked(self, x, weight, eps, residual):
+        """rms_norm_fp8 on arguments whose shapes and strides are known to fit."""
         dev = _need_one_device(x, weight, residual)
         T, C = x.shape
-        ldx, ldr, rp, out, op = _pitch(x), 0, 0, None, 0
-        assert x.stride(1) == 1 and weight.is_contiguous() and weight.numel() == C
         codes = torch.empty((T, C), dtype=torch.float8_e4m3fn, device=dev)
         scale_inv = torch.empty((T, (C + 127) // 128), dtype=torch.float32, device=dev)
+        out, ldr, rp, op = None, 0, 0, 0
         if residual is not None:
-            assert residual.dtype == x.dtype and residual.shape == x.shape and residual.stride(1) == 1
             out = _like(x)
             ldr, rp, op = _pitch(residual), residual.data_ptr(), out.data_ptr()
-        self._launch(dev, self._lib.forge_rms_norm_fp8, x.data_ptr(), _dtype_code(x), ldx, rp, ldr,
+        self._launch(dev, self._lib.forge_rms_norm_fp8, x.data_ptr(), _dtype_code(x), _pitch(x), rp, ldr,
                      weight.data_ptr(), _dtype_code(weight), T, C, float(eps), codes.data_ptr(),
                      scale_inv.data_ptr(), op)
         return codes, scale_inv, out
@@ -1098,28 +1108,26 @@ class _HipKernels:
     def linear_int4(self, x, packed, scale, group_size, bias=None, activation=None, residual=None):
         """x [M,C] bf16, packed [R,ceil(C/8)] int32, scale [R,G] f32 (pack_int4's words and its
         groups' scales) -> act(x W^T + bias) + residual [M,R] bf16."""
-        dev = _need_one_device(x, packed, scale, bias, residual)
-        M, C = x.shape
-        R, words = packed.shape
-        ldr, bp, rp = 0, 0, 0
+        C, (R, words) = x.shape[1], packed.shape
         assert x.dtype == torch.bfloat16 and x.stride(1) == 1
         assert packed.dtype == torch.int32 and packed.is_contiguous() and words == (C + 7) // 8
         assert scale.dtype == torch.float32 and scale.is_contiguous()
         assert scale.shape[0] == R and scale.shape[1] == (C + group_size - 1) // group_size
-        if bias is not None:
-            assert bias.dtype == torch.bfloat16 and bias.is_contiguous() and bias.numel() == R
-            bp = bias.data_ptr()
-        if residual is not None:
-            assert residual.dtype == torch.bfloat16 and residual.stride(1) == 1
-            assert residual.shape[0] == M and residual.shape[1] == R
-            ldr, rp = _pitch(residual), residual.data_ptr()
+        assert bias is None or (bias.dtype == torch.bfloat16 and bias.is_contiguous() and bias.numel() == R)
+        assert residual is None or (residual.dtype == torch.bfloat16 and residual.stride(1) == 1
+                                    and tuple(residual.shape) == (x.shape[0], R))
+        return self.linear_int4_of_checked(x, packed, scale, int(group_size), bias, _act_code(activation), residual)
+
+    def linear_int4_of_checked(self, x, packed, scale, group_size, bias, act, residual):
+        """linear_int4 on arguments whose types, shapes and strides are known to fit."""
+        dev = _need_one_device(x, packed, scale, bias, residual)
         if group_size % 8 == 0 and not _pieces(x):
             x = self.pad_rows(x)                     # zeros: they meet the last word's spare nibbles
-            C = x.shape[1]
+        (M, C), R = x.shape, packed.shape[0]
         y = x.new_empty((M, R))
-        self._launch(dev, self._lib.forge_linear_int4, x.data_ptr(), _pitch(x), packed.data_ptr(),
-                     scale.data_ptr(), int(group_size), bp, rp, ldr, M, C, R, _act_code(activation),
-                     y.data_ptr())
+        self._launch(dev, self._lib.forge_linear_int4, x.data_ptr(), _pitch(x), packed.data_ptr(), scale.data_ptr(),
+                     group_size, 0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(),
+                     0 if residual is None else _pitch(residual), M, C, R, act, y.data_ptr())
         return y
 
 

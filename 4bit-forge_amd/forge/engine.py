@@ -100,7 +100,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     Everything in f32 with one rounding at the end; the statistics come from the unrounded s.
     weight [C] bf16 or f32.  New tensors; no backward pass (refused where one is asked for)."""
     x2, w, r2 = _norm_arguments("rms_norm", x, weight, eps, residual)
-    y, out = kernels.rms_norm(x2, w, eps, r2)
+    y, out = kernels.rms_norm_of_checked(x2, w, eps, r2)
     if x.dim() != 2:
         y, out = y.view(x.shape), None if out is None else out.view(x.shape)
     return y if residual is None else (y, out)
@@ -112,7 +112,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     [, s]), one scale = max(max |y|, 1e-12) / 448 per 128 columns, so that y = codes * scale_inv as
     ``kernels.fp8_block_dequant`` reads block-scaled weights."""
     x2, w, r2 = _norm_arguments("rms_norm_fp8", x, weight, eps, residual)
-    codes, scale_inv, out = kernels.rms_norm_fp8(x2, w, eps, r2)
+    codes, scale_inv, out = kernels.rms_norm_fp8_of_checked(x2, w, eps, r2)
     if x.dim() != 2:
         codes, scale_inv = codes.view(x.shape), scale_inv.view(*x.shape[:-1], scale_inv.shape[1])
         out = None if out is None else out.view(x.shape)
@@ -168,7 +168,7 @@ def expert_gated_rows(rows: torch.Tensor, offsets: Union[torch.Tensor, Sequence[
 
     Differentiable in rows, w_gate and w_up (once: create_graph is refused); gradients are bf16, with dg and du rounded to
     bf16 between the products.  A HIP graph of a training step captures ``kernels.gated_rows(...,
-    keep=True)`` and ``kernels.gated_rows_backward`` directly, not autograd's engine."""
+    keep=True)`` and ``kernels.gated_rows_backward`` directly; under autograd a capture is refused."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"expert_gated_rows: unknown activation {activation!r} (one of {list(ACTIVATIONS)})")
     for n, t in (("rows", rows), ("w_gate", w_gate), ("w_up", w_up)):
@@ -199,9 +199,13 @@ def expert_gated_rows(rows: torch.Tensor, offsets: Union[torch.Tensor, Sequence[
             raise ValueError(f"expert_gated_rows: offsets must be {E + 1} ascending numbers within "
                              f"[0, {N}]")
         off = torch.tensor(off, dtype=torch.int32).to(rows.device)
-    rows = _unit_rows(rows)
-    w_gate, w_up = _unit_rows(w_gate), _unit_rows(w_up)
+    rows, w_gate, w_up = _unit_rows(rows), _unit_rows(w_gate), _unit_rows(w_up)
     if torch.is_grad_enabled() and (rows.requires_grad or w_gate.requires_grad or w_up.requires_grad):
+        if torch.cuda.is_current_stream_capturing():
+            # its engine waits for the streams that leaves were used on before: the capture would fail in
+            # one of its threads, and the process with it
+            raise RuntimeError("expert_gated_rows under autograd cannot be captured: capture kernels.gated_rows(..., "
+                               "keep=True) and kernels.gated_rows_backward")
         return _GatedRows.apply(rows, off, w_gate, w_up, activation)
     return kernels.gated_rows(rows, off, w_gate, w_up, activation).contiguous()
 
@@ -243,7 +247,7 @@ def linear_int4(x: torch.Tensor, packed: Dict[str, torch.Tensor], bias: Optional
     if residual is not None and (residual.dtype != torch.bfloat16 or residual.shape != shape):
         raise ValueError(f"linear_int4: residual {tuple(residual.shape)} {residual.dtype}, expected "
                          f"{shape} bfloat16")
-    y = kernels.linear_int4(_rows_of(x), w.contiguous(), scale.float().contiguous(), group_size,
-                            None if bias is None else bias.contiguous(), activation,
-                            None if residual is None else _rows_of(residual))
+    y = kernels.linear_int4_of_checked(_rows_of(x), w.contiguous(), scale.float().contiguous(), int(group_size),
+                                       None if bias is None else bias.contiguous(), ACTIVATIONS[activation],
+                                       None if residual is None else _rows_of(residual))
     return y if len(shape) == 2 else y.view(shape)

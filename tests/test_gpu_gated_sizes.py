@@ -86,3 +86,25 @@ def test_tensors_on_different_devices_are_refused_in_training(hip):
     w = torch.randn(1, 8, 16).bfloat16()
     with pytest.raises(RuntimeError):
         engine.expert_gated_rows(x, [0, 4], w, w)
+
+
+def test_training_is_not_captured_through_autograd(hip):
+    """refused, with the leaves' eager graph alive; without gradients the same call is captured"""
+    g = torch.Generator(device=DEV).manual_seed(9)
+    mk = lambda *sh: (0.3 * torch.randn(*sh, generator=g, device=DEV)).bfloat16()   # noqa: E731
+    x, wg, wu = (t.requires_grad_(True) for t in (mk(10, 24), mk(2, 40, 24), mk(2, 40, 24)))
+    offs = torch.tensor([0, 4, 10], dtype=torch.int32, device=DEV)
+    alive = engine.expert_gated_rows(x, offs, wg, wu)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            engine.expert_gated_rows(x, offs, wg, wu)
+        with torch.no_grad():
+            h = engine.expert_gated_rows(x, offs, wg, wu)
+    for _ in range(3):
+        h.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(h, alive)
+    alive.sum().backward()
+    assert x.grad is not None and wg.grad is not None
