@@ -9,6 +9,7 @@
 #include "common.h"
 #include "mfma_tile.h"
 #include "ragged.h"
+#include <type_traits>
 
 namespace {
 using forge::act_f32;
@@ -142,24 +143,24 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
         if constexpr (MODE == DWEIGHTS) load_q_by(lq_out, s, Q); else load_q_by(lq_in, s, Q);
     };
     // Registers 4 j .. 4 j + 3 of a tile: rows 8 j + 4 (lane / 32) .. + 3 of P, column lane & 31 of Q, i.e.
-    // 8 bytes of 32 rows of the output at a time.  The tile goes through LDS, [row of Q][column of P] with
-    // 16-byte piece c of row q at c ^ (q % 32), and leaves in runs of a whole row.
-    // (32 KB of the tile per buffer: 64 rows of 512 bytes, or 128 of FORWARD's 256 bytes.)
-    constexpr int kCols = MODE == FORWARD ? kTile / 2 : kTile, kPieces = kCols / 8, kRows = kStageBytes / (kCols * 2);
-    auto buffer = [&](int i) {
-        lds_char *b0 = (lds_char*)P0, *b1 = (lds_char*)P1, *b2 = (lds_char*)P2, *b3 = (lds_char*)Q0;
-        return i == 0 ? b0 : i == 1 ? b1 : i == 2 ? b2 : b3;
-    };
+    // 8 bytes of 32 rows of the output at a time.  Every wavefront's part goes through 16 KB of LDS of its own,
+    // [row of Q][KB pieces of 16 bytes], with the pieces of a row in an order that keeps the banks apart, and
+    // leaves in whole rows of it.
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    // 32 columns (block) x 32 rows (from row0 on) of the output; FORWARD: g and u
-    auto put = [&](int row0, int block, const f32x16_t& x, const f32x16_t& y) {
+    lds_char* mine = (wave < 4 ? wave < 2 ? (lds_char*)P0 : (lds_char*)P1 : wave < 6 ? (lds_char*)P2 : (lds_char*)Q0) + (wave & 1) * 16384;
+    auto place = [](auto pieces, int row, int piece) {
+        constexpr int K = decltype(pieces)::value, kShift = K == 16 ? 0 : K == 8 ? 1 : 2;
+        return row * (K * 16) + ((piece ^ ((row >> kShift) & (K - 1))) * 16);
+    };
+    // 32 columns (block, of the wavefront's) x 32 rows (from `row0` of the wavefront's, which are the tile's from
+    // q0 on) of the output; FORWARD: g and u
+    auto put = [&](auto pieces, int q0w, int row0, int block, int col0, const f32x16_t& x, const f32x16_t& y) {
         // an opaque copy: addresses made from it are not formed before the inner loop, where they would
         // cost registers
         int lane_e = lane;
         asm volatile("" : "+v"(lane_e));
-        const int q = row0 + (lane_e & 31);
-        lds_char* row = buffer(row0 / kRows) + (q % kRows) * (kCols * 2) + (lane_e >> 5) * 8;
+        const int row = row0 + (lane_e & 31), q = q0w + row;
         float h[16];
         if constexpr (MODE == FORWARD) {
             if (a.g && q < r.rows) {
@@ -171,7 +172,7 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
                         g[v] = x[4 * j + v];
                         u[v] = y[4 * j + v];
                     }
-                    const int i = p0 + block * 32 + 8 * j + 4 * (lane_e >> 5);
+                    const int i = p0 + col0 + block * 32 + 8 * j + 4 * (lane_e >> 5);
                     const int64_t at = (int64_t)(r.row0 + q) * a.I + i;
                     if (i < a.I) {
                         *reinterpret_cast<f32x4_t*>(a.g + at) = g;
@@ -186,8 +187,34 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            *(__attribute__((address_space(3))) u32x2*)(row + (((block * 4 + j) ^ (q % kPieces)) * 16)) =
+            *(__attribute__((address_space(3))) u32x2*)(mine + place(pieces, row, block * 4 + j) + (lane_e >> 5) * 8) =
                 u32x2{pack_bf16(h[4 * j], h[4 * j + 1]), pack_bf16(h[4 * j + 2], h[4 * j + 3])};
+    };
+    // the wavefront's rows, the tile's from q0w on, at its columns from col0 on
+    auto leave = [&](auto pieces, int n_rows, int q0w, int col0) {
+        constexpr int K = decltype(pieces)::value;
+        uint16_t* out;
+        int64_t pitch;
+        int rows, cols;
+        if constexpr (MODE == FORWARD) {
+            out = a.h + (int64_t)r.row0 * a.I + p0;
+            pitch = a.I; rows = r.rows; cols = a.I - p0;
+        } else if constexpr (MODE == DROWS) {
+            out = a.dx + (int64_t)r.row0 * a.H + p0;
+            pitch = a.H; rows = r.rows; cols = a.H - p0;
+        } else {
+            out = (which ? a.dwu : a.dwg) + ((int64_t)r.expert * a.I + q0) * a.H + p0;
+            pitch = a.H; rows = a.I - q0; cols = a.H - p0;
+        }
+        const int piece = lane % K, col = col0 + piece * 8;
+        if (col >= cols) return;
+#pragma unroll 4
+        for (int i = 0; i < n_rows * K / 64; ++i) {
+            const int row = i * (64 / K) + lane / K;
+            if (q0w + row >= rows) break;
+            *reinterpret_cast<u32x4*>(out + (q0w + row) * pitch + col) =
+                *(__attribute__((address_space(3))) u32x4*)(mine + place(pieces, row, piece));
+        }
     };
     auto clear = [](auto& acc, int n_p, int n_q) {
 #pragma unroll
@@ -214,14 +241,18 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
                 fp.init(lane, (block >> 1) * 4 + (block & 1));
                 multiply_light_stages<2>(stages, P0, P1, P2, Q0, Q1, load_p, load_light, fp, fq_in, acc);
                 __syncthreads();
-                put(row0, block, acc[0][0], acc[1][0]);
+                constexpr std::integral_constant<int, 4> kPieces{};
+                put(kPieces, row0, 0, 0, block * 32, acc[0][0], acc[1][0]);
+                leave(kPieces, 32, row0, block * 32);
             } else {
                 OuterFragment<2> fp;
                 fp.init(lane, block * 2);
                 multiply_light_stages<1>(stages, P0, P1, P2, Q0, Q1, load_p, load_light, fp, fq_in, acc);
                 __syncthreads();
-                put(row0, block * 2, acc[0][0], acc[0][0]);
-                put(row0, block * 2 + 1, acc[1][0], acc[1][0]);
+                constexpr std::integral_constant<int, 8> kPieces{};
+                put(kPieces, row0, 0, 0, block * 64, acc[0][0], acc[0][0]);
+                put(kPieces, row0, 0, 1, block * 64, acc[1][0], acc[1][0]);
+                leave(kPieces, 32, row0, block * 64);
             }
         }
     } else if (wq * 64 < (MODE == DWEIGHTS ? a.I - q0 : r.rows)) {
@@ -245,44 +276,17 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
             }
         }
         __syncthreads();
+        constexpr int kTiles = MODE == FORWARD ? 2 : 4;
+        constexpr std::integral_constant<int, kTiles * 4> kPieces{};
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int t = 0; t < (MODE == FORWARD ? 2 : 4); ++t) {
-                if constexpr (MODE == FORWARD) put(wq * 64 + n * 32, wp * 2 + t, acc[t][n], acc[t + 2][n]);
-                else put(wq * 64 + n * 32, wp * 4 + t, acc[t][n], acc[t][n]);
-            }
+            for (int t = 0; t < kTiles; ++t)
+                put(kPieces, wq * 64, n * 32, t, wp * kTiles * 32, acc[t][n], acc[MODE == FORWARD ? t + 2 : t][n]);
+        leave(kPieces, 64, wq * 64, wp * kTiles * 32);
     } else {
         load_stages(stages, P0, P1, P2, Q0, Q1, load_p, load_q);
         __syncthreads();
-    }
-    __syncthreads();
-    uint16_t* out;
-    int64_t pitch;
-    int rows, cols;
-    if constexpr (MODE == FORWARD) {
-        out = a.h + (int64_t)r.row0 * a.I + p0;
-        pitch = a.I; rows = r.rows; cols = a.I - p0;
-    } else if constexpr (MODE == DROWS) {
-        out = a.dx + (int64_t)r.row0 * a.H + p0;
-        pitch = a.H; rows = r.rows; cols = a.H - p0;
-    } else {
-        out = (which ? a.dwu : a.dwg) + ((int64_t)r.expert * a.I + q0) * a.H + p0;
-        pitch = a.H; rows = a.I - q0; cols = a.H - p0;
-    }
-    // every wavefront writes 32 rows, or 8 of a light tile's
-    const int own = light ? 8 : 32;
-    lds_char* from = buffer(wave * own / kRows);
-    const int piece = lane % kPieces;
-    if (piece * 8 < cols) {
-#pragma unroll 4
-        for (int i = 0; i < own * kPieces / 64; ++i) {
-            const int q = wave * own + i * (64 / kPieces) + lane / kPieces;
-            if (q >= rows) break;
-            const u32x4 v = *(__attribute__((address_space(3))) u32x4*)(from + (q % kRows) * (kCols * 2) +
-                                                                        ((piece ^ (q % kPieces)) * 16));
-            *reinterpret_cast<u32x4*>(out + q * pitch + piece * 8) = v;
-        }
     }
 }
 
