@@ -144,7 +144,7 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
     };
     // Registers 4 j .. 4 j + 3 of a tile: rows 8 j + 4 (lane / 32) .. + 3 of P, column lane & 31 of Q, i.e.
     // 8 bytes of 32 rows of the output at a time.  Every wavefront's part goes through 16 KB of LDS of its own,
-    // [row of Q][KB pieces of 16 bytes], with the pieces of a row in an order that keeps the banks apart, and
+    // [row of Q][K pieces of 16 bytes], with the pieces of a row in an order that keeps the banks apart, and
     // leaves in whole rows of it.
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -153,33 +153,14 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
         constexpr int K = decltype(pieces)::value, kShift = K == 16 ? 0 : K == 8 ? 1 : 2;
         return row * (K * 16) + ((piece ^ ((row >> kShift) & (K - 1))) * 16);
     };
-    // 32 columns (block, of the wavefront's) x 32 rows (from `row0` of the wavefront's, which are the tile's from
-    // q0 on) of the output; FORWARD: g and u
-    auto put = [&](auto pieces, int q0w, int row0, int block, int col0, const f32x16_t& x, const f32x16_t& y) {
+    // 32 columns (block) x 32 rows (from row0 on) of the wavefront's part of the output; FORWARD: from g and u
+    auto put = [&](auto pieces, int row0, int block, const f32x16_t& x, const f32x16_t& y) {
         // an opaque copy: addresses made from it are not formed before the inner loop, where they would
         // cost registers
         int lane_e = lane;
         asm volatile("" : "+v"(lane_e));
-        const int row = row0 + (lane_e & 31), q = q0w + row;
         float h[16];
         if constexpr (MODE == FORWARD) {
-            if (a.g && q < r.rows) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    f32x4_t g, u;
-#pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        g[v] = x[4 * j + v];
-                        u[v] = y[4 * j + v];
-                    }
-                    const int i = p0 + col0 + block * 32 + 8 * j + 4 * (lane_e >> 5);
-                    const int64_t at = (int64_t)(r.row0 + q) * a.I + i;
-                    if (i < a.I) {
-                        *reinterpret_cast<f32x4_t*>(a.g + at) = g;
-                        *reinterpret_cast<f32x4_t*>(a.u + at) = u;
-                    }
-                }
-            }
             act_times(a.act, x, y, h);
         } else {
 #pragma unroll
@@ -187,8 +168,29 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            *(__attribute__((address_space(3))) u32x2*)(mine + place(pieces, row, block * 4 + j) + (lane_e >> 5) * 8) =
+            *(__attribute__((address_space(3))) u32x2*)(mine + place(pieces, row0 + (lane_e & 31), block * 4 + j) + (lane_e >> 5) * 8) =
                 u32x2{pack_bf16(h[4 * j], h[4 * j + 1]), pack_bf16(h[4 * j + 2], h[4 * j + 3])};
+    };
+    // the same of g or u alone, in f32 (twice as many pieces)
+    auto put_f32 = [&](auto pieces, int row0, int block, const f32x16_t& x) {
+        int lane_e = lane;
+        asm volatile("" : "+v"(lane_e));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            *(__attribute__((address_space(3))) f32x4_t*)(mine + place(pieces, row0 + (lane_e & 31), block * 8 + j * 2 + (lane_e >> 5))) =
+                f32x4_t{x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]};
+    };
+    auto leave_f32 = [&](auto pieces, float* out, int n_rows, int q0w, int col0) {
+        constexpr int K = decltype(pieces)::value;
+        const int piece = lane % K, col = p0 + col0 + piece * 4;
+        if (col >= a.I) return;
+#pragma unroll 4
+        for (int i = 0; i < n_rows * K / 64; ++i) {
+            const int row = i * (64 / K) + lane / K;
+            if (q0w + row >= r.rows) break;
+            *reinterpret_cast<f32x4_t*>(out + (int64_t)(r.row0 + q0w + row) * a.I + col) =
+                *(__attribute__((address_space(3))) f32x4_t*)(mine + place(pieces, row, piece));
+        }
     };
     // the wavefront's rows, the tile's from q0w on, at its columns from col0 on
     auto leave = [&](auto pieces, int n_rows, int q0w, int col0) {
@@ -242,7 +244,14 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
                 multiply_light_stages<2>(stages, P0, P1, P2, Q0, Q1, load_p, load_light, fp, fq_in, acc);
                 __syncthreads();
                 constexpr std::integral_constant<int, 4> kPieces{};
-                put(kPieces, row0, 0, 0, block * 32, acc[0][0], acc[1][0]);
+                if (a.g) {
+                    constexpr std::integral_constant<int, 8> kWide{};
+                    put_f32(kWide, 0, 0, acc[0][0]);
+                    leave_f32(kWide, a.g, 32, row0, block * 32);
+                    put_f32(kWide, 0, 0, acc[1][0]);
+                    leave_f32(kWide, a.u, 32, row0, block * 32);
+                }
+                put(kPieces, 0, 0, acc[0][0], acc[1][0]);
                 leave(kPieces, 32, row0, block * 32);
             } else {
                 OuterFragment<2> fp;
@@ -250,8 +259,8 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
                 multiply_light_stages<1>(stages, P0, P1, P2, Q0, Q1, load_p, load_light, fp, fq_in, acc);
                 __syncthreads();
                 constexpr std::integral_constant<int, 8> kPieces{};
-                put(kPieces, row0, 0, 0, block * 64, acc[0][0], acc[0][0]);
-                put(kPieces, row0, 0, 1, block * 64, acc[1][0], acc[1][0]);
+                put(kPieces, 0, 0, acc[0][0], acc[0][0]);
+                put(kPieces, 0, 1, acc[1][0], acc[1][0]);
                 leave(kPieces, 32, row0, block * 64);
             }
         }
@@ -278,11 +287,24 @@ __global__ __launch_bounds__(512) void gated_tile_kernel(GatedArgs a, int p_tile
         __syncthreads();
         constexpr int kTiles = MODE == FORWARD ? 2 : 4;
         constexpr std::integral_constant<int, kTiles * 4> kPieces{};
+        if constexpr (MODE == FORWARD) {
+            if (a.g) {
+                constexpr std::integral_constant<int, 16> kWide{};
+#pragma unroll
+                for (int of = 0; of < 2; ++of) {
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) put_f32(kWide, n * 32, t, acc[2 * of + t][n]);
+                    leave_f32(kWide, of ? a.u : a.g, 64, wq * 64, wp * 64);
+                }
+            }
+        }
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
-                put(kPieces, wq * 64, n * 32, t, wp * kTiles * 32, acc[t][n], acc[MODE == FORWARD ? t + 2 : t][n]);
+                put(kPieces, n * 32, t, acc[t][n], acc[MODE == FORWARD ? t + 2 : t][n]);
         leave(kPieces, 64, wq * 64, wp * kTiles * 32);
     } else {
         load_stages(stages, P0, P1, P2, Q0, Q1, load_p, load_q);
