@@ -60,6 +60,21 @@ __device__ __forceinline__ void act_times(int act, const V& v, const V& times, f
     }
 }
 
+// the same in place, without the product
+template <int N>
+__device__ __forceinline__ void act_all(int act, float (&v)[N]) {
+    auto all = [&](int fixed) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = act_f32(fixed, v[i]);
+    };
+    switch (act) {
+        case FORGE_ACT_SILU: all(FORGE_ACT_SILU); break;
+        case FORGE_ACT_GELU: all(FORGE_ACT_GELU); break;
+        case FORGE_ACT_RELU: all(FORGE_ACT_RELU); break;
+        default: break;
+    }
+}
+
 // the activation and its derivative
 __device__ __forceinline__ void act_grad_f32(int act, float v, float& a, float& da) {
     switch (act) {

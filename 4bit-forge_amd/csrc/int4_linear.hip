@@ -34,18 +34,28 @@ __device__ __forceinline__ void store_y(const Int4Args& a, int m, int r, float v
     a.y[(int64_t)m * a.R + r] = f32_to_bf16_bits(v);
 }
 
-// the same for 8 columns (R, ldr and the pointers allow 16-byte accesses)
-__device__ __forceinline__ void store_y8(const Int4Args& a, int m, int r, float (&v)[8]) {
-    uint32_t b[4] = {0, 0, 0, 0}, e[4] = {0, 0, 0, 0}, y[4];
-    if (a.bias) *reinterpret_cast<uint4*>(b) = *reinterpret_cast<const uint4*>(a.bias + r);
-    if (a.res) *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(a.res + (int64_t)m * a.ldr + r);
+// the same for 8 columns (R, ldr and the pointers allow 16-byte accesses), whose bias and residual the caller has
+// loaded beforehand
+__device__ __forceinline__ uint4 load_bias8(const Int4Args& a, int r) {
+    return a.bias ? *reinterpret_cast<const uint4*>(a.bias + r) : make_uint4(0, 0, 0, 0);
+}
+__device__ __forceinline__ uint4 load_residual8(const Int4Args& a, int m, int r) {
+    return a.res ? *reinterpret_cast<const uint4*>(a.res + (int64_t)m * a.ldr + r) : make_uint4(0, 0, 0, 0);
+}
+__device__ __forceinline__ void store_y8(const Int4Args& a, int m, int r, float (&v)[8], const uint4& bias, const uint4& residual) {
+    const uint32_t b[4] = {bias.x, bias.y, bias.z, bias.w}, e[4] = {residual.x, residual.y, residual.z, residual.w};
+    uint32_t y[4];
+    if (a.bias) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        if (a.bias) v[k] += __uint_as_float(k & 1 ? b[k / 2] & 0xFFFF0000u : b[k / 2] << 16);
-        v[k] = act_f32(a.act, v[k]);
-        if (a.res) v[k] += __uint_as_float(k & 1 ? e[k / 2] & 0xFFFF0000u : e[k / 2] << 16);
-        if (k & 1) y[k / 2] = forge::pack_bf16(v[k - 1], v[k]);
+        for (int k = 0; k < 8; ++k) v[k] += __uint_as_float(k & 1 ? b[k / 2] & 0xFFFF0000u : b[k / 2] << 16);
     }
+    forge::act_all(a.act, v);
+    if (a.res) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] += __uint_as_float(k & 1 ? e[k / 2] & 0xFFFF0000u : e[k / 2] << 16);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] = forge::pack_bf16(v[2 * k], v[2 * k + 1]);
     *reinterpret_cast<uint4*>(a.y + (int64_t)m * a.R + r) = make_uint4(y[0], y[1], y[2], y[3]);
 }
 
@@ -327,8 +337,18 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles,
     // residual and y are read and written in runs of 8 columns.  16 rows of 1 KB a buffer.
     // Register v of a tile: row 8 (v / 4) + 4 (lane / 32) + v % 4 of x, weight row lane & 31.
     auto quarter = [&](int i) { return reinterpret_cast<float*>(i == 0 ? X0 : i == 1 ? X1 : i == 2 ? X2 : X3); };
+    // 32 threads a row, 16 rows at a time; what is added is asked for before the tile is in LDS
+    const int c = (threadIdx.x & 31) * 8, r = r0 + c;
+    const bool pieces = vec && r < a.R;
+    const uint4 none = make_uint4(0, 0, 0, 0), bias = pieces ? load_bias8(a, r) : none;
 #pragma unroll
     for (int pass = 0; pass < 2; ++pass) {
+        uint4 residual[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int m = m0 + pass * 64 + i * 16 + (threadIdx.x >> 5);
+            residual[i] = pieces && m < a.M ? load_residual8(a, m, r) : none;
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -336,8 +356,6 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles,
                 quarter(t * 2 + (v >> 3))[(8 * ((v >> 2) & 1) + 4 * (lane >> 5) + (v & 3)) * 256 + wave * 32 + (lane & 31)] =
                     total[pass * 2 + t][v] * kNibbleUnit;
         __syncthreads();
-        // 32 threads a row, 16 rows at a time
-        const int c = (threadIdx.x & 31) * 8, r = r0 + c;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int m = m0 + pass * 64 + i * 16 + (threadIdx.x >> 5);
@@ -347,7 +365,7 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles,
                 float v[8];
                 *reinterpret_cast<f32x4_t*>(v) = *reinterpret_cast<const f32x4_t*>(from);
                 *reinterpret_cast<f32x4_t*>(v + 4) = *reinterpret_cast<const f32x4_t*>(from + 4);
-                store_y8(a, m, r, v);
+                store_y8(a, m, r, v, bias, residual[i]);
             } else {
                 for (int k = 0; k < 8 && r + k < a.R; ++k) store_y(a, m, r + k, from[k]);
             }
@@ -553,7 +571,7 @@ __global__ __launch_bounds__(512) void int4_split_kernel(Int4Args a, int r_tiles
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] *= kNibbleUnit;
-    if (vec) store_y8(a, m0 + m, r, v);
+    if (vec) store_y8(a, m0 + m, r, v, load_bias8(a, r), load_residual8(a, m0 + m, r));
     else
         for (int k = 0; k < 8 && r + k < a.R; ++k) store_y(a, m0 + m, r + k, v[k]);
 }
