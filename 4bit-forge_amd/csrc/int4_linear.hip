@@ -160,10 +160,11 @@ __global__ __launch_bounds__(512) void int4_few_kernel(Int4Args a) {
 // ---------------------------------------------------------------- many rows of x
 // 128 rows of x by 256 weight rows per workgroup, 64 columns a stage (mfma_tile.h).  A wavefront takes all of
 // the rows of x by 32 weight rows: a 32 x 16 fragment of W is one word per lane, converted by the only
-// wavefront that multiplies by it, a step ahead.  8192 rows, 7168 -> 4096: 490 us, 980 TFLOP/s, the clock at 1.7 GHz
-// (2.1 and more where power allows), the matrix pipe busy for half of the cycles and the vector ALU for
-// half, so what counts is the work itself: 64 x 64 outputs per wavefront halve the reads of x from LDS but
-// convert every word twice, 585 us.  Converted once, into LDS, words cost 16 KB of writes and 64 KB of reads a stage.
+// wavefront that multiplies by it, a step ahead.  8192 rows, 7168 -> 4096: 450 us, 1070 TFLOP/s, the clock at 1.6 to
+// 1.7 GHz (2.1 and more where power allows), the matrix pipe busy for half of the cycles and the vector ALU
+// for half, so what counts is the work itself: 64 x 64 outputs per wavefront halve the reads of x from LDS
+// but convert every word twice (585 us against 490 at that time).  Converted once, into LDS, words cost 16 KB of
+// writes and 64 KB of reads a stage.
 // Every group's sum is formed by itself and folded into the totals with its scale, one fma per output and
 // group: that needs two sets of sums, which is why a wavefront has 64 x 64 outputs' worth and not twice that.
 // x and the packed words go to LDS without registers, four stages ahead, the words in runs of 64 bytes
