@@ -7,7 +7,6 @@ framework's entry points (``forge.engine``).  Sizes are those of the Qwen3-style
 layers of ``forge.synth`` (2048 x 768, 128 experts; 7168 x 2048, top-8 routing with Zipf popularity),
 and generic odd ones.
 """
-import functools
 import math
 import sys
 from pathlib import Path
@@ -22,7 +21,6 @@ FP8_MAX = 448.0          # largest e4m3 value
 FP8_GROUP = 128          # columns that share an 8-bit scale
 
 
-@functools.lru_cache(maxsize=None)
 def _engine():
     pkg = str(Path(__file__).resolve().parents[1] / "4bit-forge_amd")
     if pkg not in sys.path:
