@@ -1,7 +1,9 @@
 // Product with packed int4 weights:  y = act(x W^T + bias) + residual,
-// W[r][c] = (nibble - 8) * scale[r][c / gs].
+// W[r][c] = (code - zero[r][c / gs]) * scale[r][c / gs].
 //
-// The nibbles minus 8 are integers of at most 4 bits, exact in bf16, so the matrix instruction's
+// A nibble is code - zero + 8 modulo 16.  Without zero points (they are all 8, symmetric grids) it is the code, and
+// nibble - 8 is a signed 4-bit integer; with them code - zero takes five bits, so the code is formed
+// again from the nibble and the zero point (ZERO).  Either is exact in bf16, so the matrix instruction's
 // products are exact; the scale is applied to every group's f32 sum.
 #include "act.h"
 #include "common.h"
@@ -20,6 +22,7 @@ struct Int4Args {
     const uint16_t* x;       // [M, C], pitch ldx
     const uint32_t* w;       // [R, words]
     const float* scale;      // [R, G]
+    const int32_t* zero;     // [R, G], null without zero points
     const uint16_t* bias;    // [R], may be null
     const uint16_t* res;     // [M, R], pitch ldr, may be null
     uint16_t* y;             // [M, R]
@@ -85,6 +88,36 @@ __device__ __forceinline__ bf16x8_t nibbles(uint32_t word) {
 }
 constexpr float kNibbleUnit = 16.0f;
 
+// A group's zero point as nibbles() takes it: in all eight nibbles of a word, and (8 - zero) / 16
+struct Zero {
+    uint32_t add;
+    float off;
+};
+__device__ __forceinline__ Zero zero_of(uint32_t z) {
+    return {(z & 15u) * 0x11111111u, __builtin_fmaf(-0.0625f, (float)(int)z, 0.5f)};
+}
+// Eight times code - zero as bf16, divided by 16.  nibble + zero modulo 16 is code - 8 as a signed 4-bit integer
+// (added in the low three bits of every nibble, the top bit by exclusive or: nothing carries into a
+// neighbour); (code - 8) / 16 + (8 - zero) / 16 is exact, in the upper 16 bits too (zero within -240 .. 255).
+__device__ __forceinline__ bf16x8_t nibbles(uint32_t word, const Zero& z) {
+    const uint32_t a = ((word & 0x77777777u) + (z.add & 0x77777777u)) ^ ((word ^ z.add) & 0x88888888u), b = a >> 4;
+    auto value = [&](uint32_t v) { return __float_as_uint(__uint_as_float(v) + z.off); };
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    const u32x4 v = {__builtin_amdgcn_perm(value(nibble_of_byte<0>(b)), value(nibble_of_byte<0>(a)), 0x07060302u),
+                     __builtin_amdgcn_perm(value(nibble_of_byte<1>(b)), value(nibble_of_byte<1>(a)), 0x07060302u),
+                     __builtin_amdgcn_perm(value(nibble_of_byte<2>(b)), value(nibble_of_byte<2>(a)), 0x07060302u),
+                     __builtin_amdgcn_perm(value(nibble_of_byte<3>(b)), value(nibble_of_byte<3>(a)), 0x07060302u)};
+    return __builtin_bit_cast(bf16x8_t, v);
+}
+template <bool ZERO>
+__device__ __forceinline__ bf16x8_t weights(uint32_t word, const Zero& z) {
+    if constexpr (ZERO) return nibbles(word, z);
+    else return nibbles(word);
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t zero_descriptor(const Int4Args& a, int r0, int rows) {
+    return forge::descriptor(a.zero + (int64_t)r0 * a.G, (uint32_t)(rows * a.G * 4));
+}
+
 // ---------------------------------------------------------------- few rows of x
 // Bound by the packed words, which are read once: a workgroup takes 16 weight rows, its 8 wavefronts every
 // eighth run of 128 columns, and their sums meet in LDS (in a fixed order; fewer wavefronts per row and
@@ -94,7 +127,7 @@ constexpr float kNibbleUnit = 16.0f;
 // the matrix instruction wants of it when each step takes 32 consecutive columns, and then x too is read
 // in 64-byte runs and a step never crosses a group (groups are multiples of 32).  STEPS steps of 32 columns share a
 // scale.  The up to 16 rows of x come from the caches; rows beyond M and columns beyond C read as zero.
-template <int STEPS>
+template <int STEPS, bool ZERO>
 __global__ __launch_bounds__(512) void int4_few_kernel(Int4Args a) {
     using namespace forge;
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -105,6 +138,8 @@ __global__ __launch_bounds__(512) void int4_few_kernel(Int4Args a) {
     const __amdgpu_buffer_rsrc_t dw = descriptor(a.w + (int64_t)r0 * a.words, (uint32_t)(rows * a.words * 4));
     const __amdgpu_buffer_rsrc_t ds = descriptor(a.scale + (int64_t)r0 * a.G, (uint32_t)(rows * a.G * 4));
     const __amdgpu_buffer_rsrc_t dx = descriptor(a.x, (uint32_t)(((a.M - 1) * a.ldx + a.C) * 2));
+    __amdgpu_buffer_rsrc_t dz;
+    if constexpr (ZERO) dz = zero_descriptor(a, r0, rows);
     f32x4_t total = {0.0f, 0.0f, 0.0f, 0.0f};
     const int runs = (a.C + 127) / 128;
     // One run at a time: the other wavefronts' are on their way meanwhile (two or four of each asked for at once
@@ -112,13 +147,15 @@ __global__ __launch_bounds__(512) void int4_few_kernel(Int4Args a) {
     for (int c = wave; c < runs; c += 8) {
         u32x4 x[4];
         float sc[4 / STEPS];
+        Zero z[4 / STEPS] = {};
         // (words behind the row are a neighbour's, their x is zero, or outside the array)
         u32x4 q = __builtin_amdgcn_raw_buffer_load_b128(dw, (n * a.words + c * 16 + kb * 4) * 4, 0, 0);
 #pragma unroll
         for (int i = 0; i < 4 / STEPS; ++i) {
             const int k = c * 128 + i * STEPS * 32;
-            sc[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
-                ds, k < a.C ? (n * a.G + k / a.gs) * 4 : (int)kOutside, 0, 0));
+            const int at = k < a.C ? (n * a.G + k / a.gs) * 4 : (int)kOutside;
+            sc[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ds, at, 0, 0));
+            if constexpr (ZERO) z[i] = zero_of(__builtin_amdgcn_raw_buffer_load_b32(dz, at, 0, 0));
         }
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
@@ -138,7 +175,7 @@ __global__ __launch_bounds__(512) void int4_few_kernel(Int4Args a) {
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
             if (d % STEPS == 0) acc = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x[d]), nibbles(q[d]), acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x[d]), weights<ZERO>(q[d], z[d / STEPS]), acc, 0, 0, 0);
             if (d % STEPS == STEPS - 1)
 #pragma unroll
                 for (int v = 0; v < 4; ++v) total[v] = __builtin_fmaf(sc[d / STEPS], acc[v], total[v]);
@@ -173,7 +210,7 @@ __global__ __launch_bounds__(512) void int4_few_kernel(Int4Args a) {
 // Where groups end is fixed at compile time: 128 columns (two stages) hold FOLDS folds (1: groups of
 // 128 k or a single one; 2: of 64 k; 4: of 32 k).  The first product of a group starts from the
 // constant zero.
-template <int FOLDS>
+template <int FOLDS, bool ZERO>
 __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles, int m_tiles, bool vec) {
     using namespace forge;
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -190,6 +227,8 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles,
     const __amdgpu_buffer_rsrc_t dx = descriptor(a.x + (int64_t)m0 * a.ldx, (uint32_t)(((xrows - 1) * a.ldx + a.C) * 2));
     const __amdgpu_buffer_rsrc_t dw = descriptor(a.w + (int64_t)r0 * a.words, (uint32_t)(rows * a.words * 4));
     const __amdgpu_buffer_rsrc_t ds = descriptor(a.scale + (int64_t)r0 * a.G, (uint32_t)(rows * a.G * 4));
+    __amdgpu_buffer_rsrc_t dz;
+    if constexpr (ZERO) dz = zero_descriptor(a, r0, rows);
     InnerLoader<2> lx;
     lx.init(lane, a.ldx, wave * 16);
     InnerFragment fx;
@@ -235,6 +274,24 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles,
             k_end += a.gs;
         }
     };
+    // Zero points the same way, but a group's is wanted before its first conversion, which is before the
+    // group in front of it is folded: they are asked for one group further ahead, and the place of
+    // fold i + 1 is free when fold i is made.
+    constexpr int kAsked = ZERO ? 2 : 1;                        // loads per fold
+    uint32_t zr[kFolds];
+    Zero zero = {};
+    int gz = 0, kz_next = 0, kz_end = a.gs;
+    auto zeros = [&](uint32_t& to) {
+        to = __builtin_amdgcn_raw_buffer_load_b32(dz, (int)(sat + gz * 4), 0, 0);
+        kz_next += 128 / FOLDS;
+        if (kz_next >= kz_end && gz + 1 < a.G) {
+            ++gz;
+            kz_end += a.gs;
+        }
+    };
+    auto group = [&](int i) {                                   // the words that follow belong to fold i
+        if constexpr (ZERO) zero = zero_of(zr[i]);
+    };
     auto fold = [&](int i) {
         const float scale = __uint_as_float(sc[i]);
 #pragma unroll
@@ -245,6 +302,7 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles,
             asm volatile("" : "+v"(total[t]));
         }
         scales(i);
+        if constexpr (ZERO) zeros(zr[(i + 1) % kFolds]);
     };
     struct Step {
         bf16x8_t p[4], q;
@@ -252,7 +310,7 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles,
     auto prepare = [&](Step& f, const char* X, int s, const u32x4& w) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) f.p[t] = fx.read(X, t, s);
-        f.q = nibbles(w[s]);
+        f.q = weights<ZERO>(w[s], zero);
     };
     auto multiply = [&](auto first, const Step& f) {
         const f32x16_t zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
@@ -275,16 +333,17 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles,
         constexpr bool kFirst = I % 2 == 0 || FOLDS > 1, kLast = I % 2 == 1 || FOLDS > 1;
         prepare(h, X, 1, w);
         multiply(std::integral_constant<bool, kFirst>{}, f);
+        if (FOLDS == 4) group(2 * I + 1);
         prepare(f, X, 2, w);
         multiply(std::false_type{}, h);
         if (FOLDS == 4) fold(2 * I);
         prepare(h, X, 3, w);
         multiply(std::integral_constant<bool, FOLDS == 4>{}, f);
         // The next stage's x (and words, if a pair begins) have arrived once no more loads are on their way
-        // than were issued behind them: x of two stages, one pair's words, and the scales of three stages
-        // (FOLDS 1: of every other).
+        // than were issued behind them: x of two stages, one pair's words, and the scales (and zero points) of
+        // three stages (FOLDS 1: of every other).
         constexpr int kScales = FOLDS == 1 ? (I % 2 == 0 ? 2 : 1) : FOLDS == 2 ? 3 : 6;
-        wait_loads_barrier<2 * 2 + 2 + kScales>();
+        wait_loads_barrier<2 * 2 + 2 + kAsked * kScales>();
         lx.stage(dx, X, wave, a.ldx, (s + 4) * kStage, a.C);
         __builtin_amdgcn_sched_barrier(0);
         if (I % 2 == 0) {
@@ -295,11 +354,15 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles,
             read_words(w, Wn, 1);
         }
         spread(wn);
+        if (kLast) group(FOLDS == 1 ? (I + 1) / 2 % 2 : (I + 1) * (FOLDS / 2) % kFolds);
         prepare(f, Xn, 0, wn);
         multiply(std::false_type{}, h);
         if (kLast) fold(FOLDS == 1 ? I / 2 : FOLDS == 2 ? I : 2 * I + 1);
     };
     u32x4 w0, w1;                                               // words of even and odd stages
+    uint32_t first_zero;
+    if constexpr (ZERO) zeros(first_zero);
+    __builtin_amdgcn_sched_barrier(0);
     // in the loop's own order
     lx.stage(dx, X0, wave, a.ldx, 0, a.C);
     __builtin_amdgcn_sched_barrier(0);
@@ -313,11 +376,15 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles,
     lx.stage(dx, X3, wave, a.ldx, 3 * kStage, a.C);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < kFolds; ++i) scales(i);
-    wait_loads_barrier<8 + kFolds>();
+    for (int i = 0; i < kFolds; ++i) {
+        scales(i);
+        if constexpr (ZERO) zeros(zr[(i + 1) % kFolds]);
+    }
+    wait_loads_barrier<8 + kAsked * kFolds>();
     read_words(w0, W0, 0);
     read_words(w1, W0, 1);
     spread(w0);
+    if constexpr (ZERO) zero = zero_of(first_zero);
     prepare(f, X0, 0, w0);
     // (columns behind C are zeros of x times a neighbour's words)
     const int stages = (a.C + 2 * kStage - 1) / (2 * kStage) * 2;
@@ -381,7 +448,7 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Args a, int r_tiles,
 // wavefronts forms all of that tile over every eighth 128 columns (a pair of stages), on LDS buffers of
 // its own, without a barrier; their sums meet in LDS in a fixed order.  The wavefront's inner loop is
 // that of the tiles: x a stage ahead, words a pair ahead, fragments a step ahead.
-template <int PT, int FOLDS>
+template <int PT, int FOLDS, bool ZERO>
 __global__ __launch_bounds__(512) void int4_split_kernel(Int4Args a, int r_tiles, int m_tiles, bool vec) {
     using namespace forge;
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -395,6 +462,8 @@ __global__ __launch_bounds__(512) void int4_split_kernel(Int4Args a, int r_tiles
     const __amdgpu_buffer_rsrc_t dx = descriptor(a.x + (int64_t)m0 * a.ldx, (uint32_t)(((xrows - 1) * a.ldx + a.C) * 2));
     const __amdgpu_buffer_rsrc_t dw = descriptor(a.w + (int64_t)r0 * a.words, (uint32_t)(rows * a.words * 4));
     const __amdgpu_buffer_rsrc_t ds = descriptor(a.scale + (int64_t)r0 * a.G, (uint32_t)(rows * a.G * 4));
+    __amdgpu_buffer_rsrc_t dz;
+    if constexpr (ZERO) dz = zero_descriptor(a, r0, rows);
     InnerLoader<4 * PT> lx;                                     // as wavefront 0 of a tile of its own
     lx.init(lane, a.ldx, 0);
     InnerFragment fx;
@@ -431,17 +500,24 @@ __global__ __launch_bounds__(512) void int4_split_kernel(Int4Args a, int r_tiles
 #pragma unroll
             for (int v = 0; v < 16; ++v) total[t][n][v] = 0.0f;
     const uint32_t sat = (uint32_t)(lane * a.G * 4);
-    auto scales = [&](uint32_t (&sc)[FOLDS], int pair) {
+    auto scales = [&](__amdgpu_buffer_rsrc_t d, uint32_t (&sc)[FOLDS], int pair) {
         int g = pair * 128 / a.gs, into = pair * 128 - g * a.gs;
 #pragma unroll
         for (int i = 0; i < FOLDS; ++i) {
-            sc[i] = __builtin_amdgcn_raw_buffer_load_b32(ds, (int)(sat + min(g, a.G - 1) * 4), 0, 0);
+            sc[i] = __builtin_amdgcn_raw_buffer_load_b32(d, (int)(sat + min(g, a.G - 1) * 4), 0, 0);
             into += 128 / FOLDS;
             if (into >= a.gs) {
                 into -= a.gs;
                 ++g;
             }
         }
+    };
+    // the zero points of the words that follow, from what was loaded like the scales
+    Zero zero[2] = {};
+    auto group = [&](uint32_t z) {
+        const auto both = __builtin_amdgcn_permlane32_swap(z, z, false, false);
+        zero[0] = zero_of(both[0]);
+        zero[1] = zero_of(both[1]);
     };
     auto fold = [&](uint32_t s) {
         const auto both = __builtin_amdgcn_permlane32_swap(s, s, false, false);
@@ -462,7 +538,7 @@ __global__ __launch_bounds__(512) void int4_split_kernel(Int4Args a, int r_tiles
 #pragma unroll
         for (int t = 0; t < PT; ++t) f.p[t] = fx.read(X, t, s);
 #pragma unroll
-        for (int n = 0; n < 2; ++n) f.q[n] = nibbles(w[n][s]);
+        for (int n = 0; n < 2; ++n) f.q[n] = weights<ZERO>(w[n][s], zero[n]);
     };
     auto multiply = [&](auto first, const Step& f) {
         const f32x16_t zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
@@ -484,12 +560,13 @@ __global__ __launch_bounds__(512) void int4_split_kernel(Int4Args a, int r_tiles
     };
     Step f, h;
     u32x4 w0[2], w1[2];
-    uint32_t sc[FOLDS], sn[FOLDS];
+    uint32_t sc[FOLDS], sn[FOLDS], zc[FOLDS], zn[FOLDS];
     const int pairs = (a.C + 127) / 128;
     if (wave < pairs) {
         load_words(wave);
         __builtin_amdgcn_sched_barrier(0);
-        scales(sc, wave);
+        scales(ds, sc, wave);
+        if constexpr (ZERO) scales(dz, zc, wave);
         __builtin_amdgcn_sched_barrier(0);
         load_x(xa, wave * 128);
         __builtin_amdgcn_sched_barrier(0);
@@ -498,11 +575,13 @@ __global__ __launch_bounds__(512) void int4_split_kernel(Int4Args a, int r_tiles
         read_words(w0, 0);
         read_words(w1, 1);
         spread(w0);
+        if constexpr (ZERO) group(zc[0]);
         prepare(f, xa, 0, w0);
         // (what lies behind the last pair is fetched as zeros of x)
         for (int p = wave; p < pairs; p += 8) {
             prepare(h, xa, 1, w0);
             multiply(std::true_type{}, f);
+            if constexpr (ZERO && FOLDS == 4) group(zc[1]);
             prepare(f, xa, 2, w0);
             multiply(std::false_type{}, h);
             if (FOLDS == 4) fold(sc[0]);
@@ -511,16 +590,19 @@ __global__ __launch_bounds__(512) void int4_split_kernel(Int4Args a, int r_tiles
             arrived(std::integral_constant<int, 63>{});         // the reads: words and xa are free
             load_words(p + 8);
             __builtin_amdgcn_sched_barrier(0);
-            scales(sn, p + 8);
+            scales(ds, sn, p + 8);
+            if constexpr (ZERO) scales(dz, zn, p + 8);
             __builtin_amdgcn_sched_barrier(0);
             load_x(xa, (p + 8) * 128);
-            arrived(std::integral_constant<int, 4 + FOLDS + 4 * PT>{});      // xb
+            arrived(std::integral_constant<int, 4 + (ZERO ? 2 : 1) * FOLDS + 4 * PT>{});      // xb
             spread(w1);
+            if constexpr (ZERO && FOLDS > 1) group(zc[FOLDS / 2]);
             prepare(f, xb, 0, w1);
             multiply(std::false_type{}, h);
             if (FOLDS > 1) fold(sc[FOLDS == 2 ? 0 : 1]);
             prepare(h, xb, 1, w1);
             multiply(std::integral_constant<bool, (FOLDS > 1)>{}, f);
+            if constexpr (ZERO && FOLDS == 4) group(zc[3]);
             prepare(f, xb, 2, w1);
             multiply(std::false_type{}, h);
             if (FOLDS == 4) fold(sc[FOLDS / 2]);
@@ -532,11 +614,15 @@ __global__ __launch_bounds__(512) void int4_split_kernel(Int4Args a, int r_tiles
             read_words(w0, 0);
             read_words(w1, 1);
             spread(w0);
+            if constexpr (ZERO) group(zn[0]);
             prepare(f, xa, 0, w0);
             multiply(std::false_type{}, h);
             fold(sc[FOLDS - 1]);
 #pragma unroll
-            for (int i = 0; i < FOLDS; ++i) sc[i] = sn[i];
+            for (int i = 0; i < FOLDS; ++i) {
+                sc[i] = sn[i];
+                if constexpr (ZERO) zc[i] = zn[i];
+            }
         }
         wait_loads<0>();
     }
@@ -580,6 +666,7 @@ __global__ __launch_bounds__(512) void int4_split_kernel(Int4Args a, int r_tiles
 // Groups that are not multiples of 32 columns (any shape and alignment): 64 x 64 outputs per workgroup,
 // four wavefronts of 32 x 32,
 // 32 columns a step through LDS; a step never crosses the end of a group (its rest is zero).
+template <bool ZERO>
 __global__ __launch_bounds__(256) void int4_any_kernel(Int4Args a, int r_tiles) {
     constexpr int T = 64, K = 32, LD = K + 8;
     __shared__ uint16_t X[T][LD], W[T][LD];
@@ -604,7 +691,9 @@ __global__ __launch_bounds__(256) void int4_any_kernel(Int4Args a, int r_tiles) 
                     if (m0 + row < a.M) xv = a.x[(int64_t)(m0 + row) * a.ldx + c];
                     if (r0 + row < a.R) {
                         const uint32_t word = a.w[(int64_t)(r0 + row) * a.words + c / 8];
-                        wv = f32_to_bf16_bits((float)((int)((word >> (4 * (c % 8))) & 15u) - 8));
+                        const int nibble = (int)((word >> (4 * (c % 8))) & 15u);
+                        const int z = ZERO ? a.zero[(int64_t)(r0 + row) * a.G + g] : 8;
+                        wv = f32_to_bf16_bits((float)(((nibble + z + 8) & 15) - z));     // code - zero
                     }
                 }
                 X[row][k] = xv;
@@ -642,65 +731,86 @@ constexpr int64_t kFewRows = 16;
 constexpr int64_t kAtOnce = 256, kSplitWorkgroups = 768;
 int64_t split_workgroups(int64_t M, int64_t R, int64_t rows) { return forge::ceil_div(R, 64) * forge::ceil_div(M, rows); }
 
-template <int PT>
+template <int PT, bool ZERO>
 void launch_split(const Int4Args& a, bool one_group, bool vec, hipStream_t st) {
     const int r_tiles = (int)forge::ceil_div(a.R, 64), m_tiles = (int)forge::ceil_div(a.M, 32 * PT);
     const dim3 grid((unsigned)(forge::ceil_div((int64_t)r_tiles * m_tiles, 8) * 8));
-    if (a.gs % 128 == 0 || one_group) int4_split_kernel<PT, 1><<<grid, 512, 0, st>>>(a, r_tiles, m_tiles, vec);
-    else if (a.gs % 64 == 0) int4_split_kernel<PT, 2><<<grid, 512, 0, st>>>(a, r_tiles, m_tiles, vec);
-    else int4_split_kernel<PT, 4><<<grid, 512, 0, st>>>(a, r_tiles, m_tiles, vec);
+    if (a.gs % 128 == 0 || one_group) int4_split_kernel<PT, 1, ZERO><<<grid, 512, 0, st>>>(a, r_tiles, m_tiles, vec);
+    else if (a.gs % 64 == 0) int4_split_kernel<PT, 2, ZERO><<<grid, 512, 0, st>>>(a, r_tiles, m_tiles, vec);
+    else int4_split_kernel<PT, 4, ZERO><<<grid, 512, 0, st>>>(a, r_tiles, m_tiles, vec);
 }
 
+template <bool ZERO>
 void launch_few(const Int4Args& a, bool one_group, hipStream_t st) {
     const dim3 grid((unsigned)forge::ceil_div(a.R, 16));
-    if (a.gs % 128 == 0 || one_group) int4_few_kernel<4><<<grid, 512, 0, st>>>(a);
-    else if (a.gs % 64 == 0) int4_few_kernel<2><<<grid, 512, 0, st>>>(a);
-    else int4_few_kernel<1><<<grid, 512, 0, st>>>(a);
+    if (a.gs % 128 == 0 || one_group) int4_few_kernel<4, ZERO><<<grid, 512, 0, st>>>(a);
+    else if (a.gs % 64 == 0) int4_few_kernel<2, ZERO><<<grid, 512, 0, st>>>(a);
+    else int4_few_kernel<1, ZERO><<<grid, 512, 0, st>>>(a);
 }
-}  // namespace
 
-extern "C" int forge_linear_int4(const void* x, int64_t ldx, const int32_t* packed, const float* scale,
-                                 int64_t gs, const void* bias, const void* residual, int64_t ldr, int64_t M,
-                                 int64_t C, int64_t R, int act, void* y, forge_stream_t stream) {
-    const char* name = "forge_linear_int4";
+template <bool ZERO>
+int launch(const char* name, const Int4Args& a, bool pieces, bool one_group, bool vec, hipStream_t st) {
+    const int64_t M = a.M, R = a.R;
+    if (!pieces) {
+        const int64_t r_tiles = forge::ceil_div(R, 64), blocks = r_tiles * forge::ceil_div(M, 64);
+        FORGE_REQUIRE(blocks <= INT32_MAX, "%s: %lld workgroups", name, (long long)blocks);
+        int4_any_kernel<ZERO><<<dim3((unsigned)blocks), 256, 0, st>>>(a, (int)r_tiles);
+    } else if (M <= kFewRows) {
+        launch_few<ZERO>(a, one_group, st);
+    } else if (split_workgroups(M, R, 32) <= kAtOnce) {
+        launch_split<1, ZERO>(a, one_group, vec, st);
+    } else if (split_workgroups(M, R, 64) <= kSplitWorkgroups) {
+        launch_split<2, ZERO>(a, one_group, vec, st);
+    } else {
+        const int64_t r_tiles = forge::ceil_div(R, 256), m_tiles = forge::ceil_div(M, 128);
+        const int64_t blocks = forge::ceil_div(r_tiles * m_tiles, 8) * 8;
+        FORGE_REQUIRE(blocks <= INT32_MAX, "%s: %lld workgroups", name, (long long)blocks);
+        const dim3 grid((unsigned)blocks);
+        if (a.gs % 128 == 0 || one_group) int4_tile_kernel<1, ZERO><<<grid, 512, 0, st>>>(a, (int)r_tiles, (int)m_tiles, vec);
+        else if (a.gs % 64 == 0) int4_tile_kernel<2, ZERO><<<grid, 512, 0, st>>>(a, (int)r_tiles, (int)m_tiles, vec);
+        else int4_tile_kernel<4, ZERO><<<grid, 512, 0, st>>>(a, (int)r_tiles, (int)m_tiles, vec);
+    }
+    FORGE_LAUNCH_CHECK();
+    return FORGE_OK;
+}
+
+int linear_int4(const char* name, const void* x, int64_t ldx, const int32_t* packed, const float* scale,
+                const int32_t* zero, bool zeros, int64_t gs, const void* bias, const void* residual, int64_t ldr,
+                int64_t M, int64_t C, int64_t R, int act, void* y, forge_stream_t stream) {
     FORGE_REQUIRE(M >= 0 && C >= 1 && R >= 1 && gs >= 1, "%s: M=%lld C=%lld R=%lld gs=%lld", name, (long long)M,
                   (long long)C, (long long)R, (long long)gs);
     FORGE_REQUIRE(M <= (1 << 30) && C <= (1 << 24) && R <= (1 << 24), "%s: M=%lld C=%lld R=%lld: too large "
                   "(M up to 2^30, C and R up to 2^24)", name, (long long)M, (long long)C, (long long)R);
     FORGE_REQUIRE(act >= FORGE_ACT_NONE && act <= FORGE_ACT_RELU, "%s: act=%d", name, act);
     if (M == 0) return FORGE_OK;
-    FORGE_REQUIRE(x && packed && scale && y, "%s: null pointer", name);
+    FORGE_REQUIRE(x && packed && scale && y && (zero || !zeros), "%s: null pointer", name);
     FORGE_REQUIRE(ldx >= C && (!residual || ldr >= R), "%s: row pitch %lld / %lld below C=%lld / R=%lld", name,
                   (long long)ldx, (long long)ldr, (long long)C, (long long)R);
     if (gs > C) gs = C;
-    Int4Args a{(const uint16_t*)x, (const uint32_t*)packed, scale, (const uint16_t*)bias,
+    Int4Args a{(const uint16_t*)x, (const uint32_t*)packed, scale, zero, (const uint16_t*)bias,
                (const uint16_t*)residual, (uint16_t*)y, ldx, ldr, (int)M, (int)C, (int)R,
                (int)forge::ceil_div(C, gs), (int)gs, (int)forge::ceil_div(C, 8), act};
     hipStream_t st = (hipStream_t)stream;
-    forge::KernelTiming timing("linear_int4", st, 2.0 * M * C * R, forge::WORK_FLOPS);
+    forge::KernelTiming timing(name + 6, st, 2.0 * M * C * R, forge::WORK_FLOPS);
     const bool one_group = a.G == 1;
     const bool pieces = C % 8 == 0 && ldx % 8 == 0 && ldx < (1 << 21) && aligned16(x) &&
                         (gs % 32 == 0 || one_group);
     const bool vec = R % 8 == 0 && aligned16(y) && aligned16(bias) && aligned16(residual) && (!residual || ldr % 8 == 0);
-    if (!pieces) {
-        const int64_t r_tiles = forge::ceil_div(R, 64), blocks = r_tiles * forge::ceil_div(M, 64);
-        FORGE_REQUIRE(blocks <= INT32_MAX, "%s: %lld workgroups", name, (long long)blocks);
-        int4_any_kernel<<<dim3((unsigned)blocks), 256, 0, st>>>(a, (int)r_tiles);
-    } else if (M <= kFewRows) {
-        launch_few(a, one_group, st);
-    } else if (split_workgroups(M, R, 32) <= kAtOnce) {
-        launch_split<1>(a, one_group, vec, st);
-    } else if (split_workgroups(M, R, 64) <= kSplitWorkgroups) {
-        launch_split<2>(a, one_group, vec, st);
-    } else {
-        const int64_t r_tiles = forge::ceil_div(R, 256), m_tiles = forge::ceil_div(M, 128);
-        const int64_t blocks = forge::ceil_div(r_tiles * m_tiles, 8) * 8;
-        FORGE_REQUIRE(blocks <= INT32_MAX, "%s: %lld workgroups", name, (long long)blocks);
-        const dim3 grid((unsigned)blocks);
-        if (gs % 128 == 0 || one_group) int4_tile_kernel<1><<<grid, 512, 0, st>>>(a, (int)r_tiles, (int)m_tiles, vec);
-        else if (gs % 64 == 0) int4_tile_kernel<2><<<grid, 512, 0, st>>>(a, (int)r_tiles, (int)m_tiles, vec);
-        else int4_tile_kernel<4><<<grid, 512, 0, st>>>(a, (int)r_tiles, (int)m_tiles, vec);
-    }
-    FORGE_LAUNCH_CHECK();
-    return FORGE_OK;
+    return zeros ? launch<true>(name, a, pieces, one_group, vec, st) : launch<false>(name, a, pieces, one_group, vec, st);
+}
+}  // namespace
+
+extern "C" int forge_linear_int4(const void* x, int64_t ldx, const int32_t* packed, const float* scale,
+                                 int64_t gs, const void* bias, const void* residual, int64_t ldr, int64_t M,
+                                 int64_t C, int64_t R, int act, void* y, forge_stream_t stream) {
+    return linear_int4("forge_linear_int4", x, ldx, packed, scale, nullptr, false, gs, bias, residual, ldr, M, C, R,
+                       act, y, stream);
+}
+
+extern "C" int forge_linear_int4_zeros(const void* x, int64_t ldx, const int32_t* packed, const float* scale,
+                                       const int32_t* zero, int64_t gs, const void* bias, const void* residual,
+                                       int64_t ldr, int64_t M, int64_t C, int64_t R, int act, void* y,
+                                       forge_stream_t stream) {
+    return linear_int4("forge_linear_int4_zeros", x, ldx, packed, scale, zero, true, gs, bias, residual, ldr, M, C,
+                       R, act, y, stream);
 }

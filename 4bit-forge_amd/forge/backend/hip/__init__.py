@@ -106,6 +106,7 @@ def _declare(lib: ctypes.CDLL) -> ctypes.CDLL:
                                        vp, vp, vp, vp, i64, vp], i32),
         "forge_gated_rows_backward_workspace_bytes": ([i64, i64], i64),
         "forge_linear_int4": ([vp, i64, vp, vp, i64, vp, vp, i64, i64, i64, i64, i32, vp, vp], i32),
+        "forge_linear_int4_zeros": ([vp, i64, vp, vp, vp, i64, vp, vp, i64, i64, i64, i64, i32, vp, vp], i32),
     }
     for name, (args, res) in sigs.items():
         fn = getattr(lib, name)          # AttributeError here = library/header mismatch
@@ -140,7 +141,7 @@ EXPORTED_SYMBOLS = (
     "forge_gptq_sweep_rows_blocked", "forge_gptq_sweep_rows_workspace_bytes",
     "forge_rows_operands", "forge_rows_diagonal",
     "forge_rms_norm", "forge_rms_norm_fp8", "forge_gated_rows", "forge_gated_rows_backward",
-    "forge_gated_rows_backward_workspace_bytes", "forge_linear_int4", "forge_pad_rows",
+    "forge_gated_rows_backward_workspace_bytes", "forge_linear_int4", "forge_linear_int4_zeros", "forge_pad_rows",
 )
 
 # FORGE_ACT_* of include/forge_hip.h
@@ -1105,27 +1106,33 @@ class _HipKernels:
                      dwg.data_ptr() if need[1] else 0, dwu.data_ptr() if need[2] else 0, work.data_ptr(), nbytes)
         return dx, dwg, dwu
 
-    def linear_int4(self, x, packed, scale, group_size, bias=None, activation=None, residual=None):
+    def linear_int4(self, x, packed, scale, group_size, bias=None, activation=None, residual=None, zero=None):
         """x [M,C] bf16, packed [R,ceil(C/8)] int32, scale [R,G] f32 (pack_int4's words and its
-        groups' scales) -> act(x W^T + bias) + residual [M,R] bf16."""
+        groups' scales), zero [R,G] int32 (the groups' zero points; None: all 8) ->
+        act(x W^T + bias) + residual [M,R] bf16."""
         C, (R, words) = x.shape[1], packed.shape
         assert x.dtype == torch.bfloat16 and x.stride(1) == 1
         assert packed.dtype == torch.int32 and packed.is_contiguous() and words == (C + 7) // 8
         assert scale.dtype == torch.float32 and scale.is_contiguous()
         assert scale.shape[0] == R and scale.shape[1] == (C + group_size - 1) // group_size
+        assert zero is None or (zero.dtype == torch.int32 and zero.is_contiguous() and zero.shape == scale.shape)
         assert bias is None or (bias.dtype == torch.bfloat16 and bias.is_contiguous() and bias.numel() == R)
         assert residual is None or (residual.dtype == torch.bfloat16 and residual.stride(1) == 1
                                     and tuple(residual.shape) == (x.shape[0], R))
-        return self.linear_int4_of_checked(x, packed, scale, int(group_size), bias, _act_code(activation), residual)
+        return self.linear_int4_of_checked(x, packed, scale, zero, int(group_size), bias, _act_code(activation),
+                                           residual)
 
-    def linear_int4_of_checked(self, x, packed, scale, group_size, bias, act, residual):
+    def linear_int4_of_checked(self, x, packed, scale, zero, group_size, bias, act, residual):
         """linear_int4 on arguments whose types, shapes and strides are known to fit."""
-        dev = _need_one_device(x, packed, scale, bias, residual)
+        dev = _need_one_device(x, packed, scale, zero, bias, residual)
         if group_size % 8 == 0 and not _pieces(x):
             x = self.pad_rows(x)                     # zeros: they meet the last word's spare nibbles
         (M, C), R = x.shape, packed.shape[0]
         y = x.new_empty((M, R))
-        self._launch(dev, self._lib.forge_linear_int4, x.data_ptr(), _pitch(x), packed.data_ptr(), scale.data_ptr(),
+        fn, zeros = self._lib.forge_linear_int4, ()
+        if zero is not None:
+            fn, zeros = self._lib.forge_linear_int4_zeros, (zero.data_ptr(),)
+        self._launch(dev, fn, x.data_ptr(), _pitch(x), packed.data_ptr(), scale.data_ptr(), *zeros,
                      group_size, 0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(),
                      0 if residual is None else _pitch(residual), M, C, R, act, y.data_ptr())
         return y

@@ -214,8 +214,10 @@ def linear_int4(x: torch.Tensor, packed: Dict[str, torch.Tensor], bias: Optional
                 activation: Optional[str] = None, residual: Optional[torch.Tensor] = None,
                 group_size: Optional[int] = None) -> torch.Tensor:
     """A layer's product with its packed weights, as ``export.pack_weight`` returns them:
-    act(x W^T + bias) + residual with W[r, c] = (nibble - 8) * weight_scale[r, c / group_size] (the
-    zero points are in the nibbles).  x [..., C] bf16, bias [R] bf16, residual [..., R] bf16;
+    act(x W^T + bias) + residual with W[r, c] = (code - zero) * weight_scale[r, c / group_size], the layer's
+    dequantised weight.  The record's nibbles are code - zero + 8 modulo 16: with a ``weight_zero_point`` (whole
+    numbers of an integer type, one per group) the codes are formed from both, without one every zero
+    is 8 (symmetric records).  x [..., C] bf16, bias [R] bf16, residual [..., R] bf16;
     activation "silu", "gelu" (tanh form), "relu" or None; result [..., R] bf16, rounded once.
     group_size may be left out when the groups divide C evenly (or there is one).  The weights stay
     4 bits wide in memory; no layout of them is kept.  No backward pass (refused where one is asked
@@ -241,13 +243,20 @@ def linear_int4(x: torch.Tensor, packed: Dict[str, torch.Tensor], bias: Optional
         group_size = C // G
     if group_size < 1 or (C + group_size - 1) // group_size != G:
         raise ValueError(f"linear_int4: group_size={group_size} does not give {G} groups of {C} columns")
+    zero = packed.get("weight_zero_point")
+    if zero is not None:
+        if zero.dtype.is_floating_point or zero.dtype.is_complex or zero.dtype == torch.bool:
+            raise ValueError(f"linear_int4: weight_zero_point is {zero.dtype}, expected an integer type")
+        if zero.shape != scale.shape:
+            raise ValueError(f"linear_int4: weight_zero_point {tuple(zero.shape)}, weight_scale {tuple(scale.shape)}")
+        zero = zero.to(torch.int32).contiguous()
     if bias is not None and (bias.dtype != torch.bfloat16 or bias.shape != (R,)):
         raise ValueError(f"linear_int4: bias {tuple(bias.shape)} {bias.dtype}, expected [{R}] bfloat16")
     shape = (*x.shape[:-1], R)
     if residual is not None and (residual.dtype != torch.bfloat16 or residual.shape != shape):
         raise ValueError(f"linear_int4: residual {tuple(residual.shape)} {residual.dtype}, expected "
                          f"{shape} bfloat16")
-    y = kernels.linear_int4_of_checked(_rows_of(x), w.contiguous(), scale.float().contiguous(), int(group_size),
+    y = kernels.linear_int4_of_checked(_rows_of(x), w.contiguous(), scale.float().contiguous(), zero, int(group_size),
                                        None if bias is None else bias.contiguous(), ACTIVATIONS[activation],
                                        None if residual is None else _rows_of(residual))
     return y if len(shape) == 2 else y.view(shape)

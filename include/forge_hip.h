@@ -589,8 +589,8 @@ int forge_gated_rows_backward(const void* dh, const float* g, const float* u, co
                               int64_t ws_bytes, forge_stream_t stream);
 int64_t forge_gated_rows_backward_workspace_bytes(int64_t N, int64_t I);
 
-/* Product with forge_pack_int4's weights:  y = act(x W^T + bias) + residual,
- * W[r][c] = (nibble c of row r - 8) * scale[r][c / gs]; the zero points are in the nibbles already.
+/* Product with forge_pack_int4's weights where every zero point is 8 (symmetric grids, or none given to
+ * forge_pack_int4):  y = act(x W^T + bias) + residual, W[r][c] = (nibble c of row r - 8) * scale[r][c / gs].
  * x [M, C] bf16 with row pitch ldx, packed [R, ceil(C/8)] int32, scale [R, ceil(C/gs)] f32, bias
  * [R] bf16 (NULL: none), residual [M, R] bf16 with row pitch ldr (NULL: none), y [M, R] bf16
  * contiguous.  The nibbles enter the products as integers (exact in bf16); every group's sum is
@@ -598,6 +598,14 @@ int64_t forge_gated_rows_backward_workspace_bytes(int64_t N, int64_t I);
 int forge_linear_int4(const void* x, int64_t ldx, const int32_t* packed, const float* scale,
                       int64_t gs, const void* bias, const void* residual, int64_t ldr, int64_t M,
                       int64_t C, int64_t R, int act, void* y, forge_stream_t stream);
+/* The same with zero points: a nibble is code - zero + 8 modulo 16, which code it stands for shows only
+ * with its zero point:  W[r][c] = (code - zero[r][c / gs]) * scale[r][c / gs], code = (nibble + zero + 8) modulo 16
+ * in 0 .. 15.  zero [R, ceil(C/gs)] int32, those that forge_pack_int4 was given, within -240 .. 255 (0 .. 15 on the
+ * solver's grids).  code - zero enters the products as an integer, exact in bf16. */
+int forge_linear_int4_zeros(const void* x, int64_t ldx, const int32_t* packed, const float* scale,
+                            const int32_t* zero, int64_t gs, const void* bias, const void* residual,
+                            int64_t ldr, int64_t M, int64_t C, int64_t R, int act, void* y,
+                            forge_stream_t stream);
 
 #ifdef __cplusplus
 }
