@@ -146,11 +146,13 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void rms_norm_kernel(Nor
 #pragma unroll
             for (int k = 8; k; k >>= 1) m = nan_max(m, __shfl_xor(m, k));
             const float sc = (m < 1e-12f ? 1e-12f : m) / kFp8Max;
-            const float inv = 1.0f / sc;
             if (in) {
+                // divided, not multiplied by a reciprocal: that puts values near the middle of two codes on the other side
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = y[i] / sc;
                 uint2 q;
-                q.x = (uint32_t)cvt_fp8x2(y[2] * inv, y[3] * inv, cvt_fp8x2(y[0] * inv, y[1] * inv, 0, false), true);
-                q.y = (uint32_t)cvt_fp8x2(y[6] * inv, y[7] * inv, cvt_fp8x2(y[4] * inv, y[5] * inv, 0, false), true);
+                q.x = (uint32_t)cvt_fp8x2(y[2], y[3], cvt_fp8x2(y[0], y[1], 0, false), true);
+                q.y = (uint32_t)cvt_fp8x2(y[6], y[7], cvt_fp8x2(y[4], y[5], 0, false), true);
                 *reinterpret_cast<uint2*>((uint8_t*)a.y + row * a.C + c) = q;
                 if ((t & 15) == 0) a.scale_inv[row * ((a.C + kGroup - 1) / kGroup) + c / kGroup] = sc;
             }
@@ -198,8 +200,7 @@ __global__ __launch_bounds__(256) void rms_norm_any_kernel(NormArgs a) {
 #pragma unroll
             for (int k = 32; k; k >>= 1) m = nan_max(m, __shfl_xor(m, k));
             const float sc = (m < 1e-12f ? 1e-12f : m) / kFp8Max;
-            const float inv = 1.0f / sc;
-            const int q = cvt_fp8x2(y[0] * inv, y[1] * inv, 0, false);
+            const int q = cvt_fp8x2(y[0] / sc, y[1] / sc, 0, false);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int64_t c = g * kGroup + i * 64 + lane;

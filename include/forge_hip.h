@@ -544,8 +544,8 @@ int forge_rms_norm(const void* x, int dtype, int64_t ldx, const void* residual, 
                    const void* weight, int w_dtype, int64_t T, int64_t C, float eps, void* y,
                    void* residual_out, forge_stream_t stream);
 /* The same with y in 8 bits: per row and run of 128 columns (the last one may be shorter)
- * scale_inv = max(max |y|, 1e-12) / 448 and codes = float8 e4m3fn nearest to y / scale_inv, y
- * unrounded: the form forge_fp8_e4m3_block_dequant reads with so = 1, si = 128.  A NaN in a run
+ * scale_inv = max(max |y|, 1e-12) / 448 and codes = float8 e4m3fn nearest to y / scale_inv (the
+ * f32 quotient, ties to even), y unrounded: the form forge_fp8_e4m3_block_dequant reads with so = 1, si = 128.  A NaN in a run
  * makes its scale NaN.  codes [T, C] bytes, scale_inv [T, ceil(C/128)] f32, contiguous. */
 int forge_rms_norm_fp8(const void* x, int dtype, int64_t ldx, const void* residual, int64_t ldr,
                        const void* weight, int w_dtype, int64_t T, int64_t C, float eps,
