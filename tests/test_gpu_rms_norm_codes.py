@@ -31,3 +31,21 @@ def test_codes_are_the_nearest(hip, T, C, dtype, residual):
     assert torch.equal(scale, top / torch.full_like(top, 448.0))
     want = (y / per).cpu().to(torch.float8_e4m3fn)
     assert torch.equal(codes.cpu().view(torch.uint8), want.view(torch.uint8))
+
+
+@pytest.mark.parametrize("C", [256, 257])
+def test_codes_of_extreme_rows(hip, C):
+    """the same where a run's largest value is tiny, huge or infinite"""
+    g = torch.Generator(device=DEV).manual_seed(C)
+    x = torch.randn(6, C, generator=g, device=DEV)
+    w = torch.ones(6, C, device=DEV)
+    w[0], w[1], w[2], w[3] = 1e-20, 1e30, 1e37, 1e-11
+    for k in range(6):
+        x[5, 3] = float("inf") if k == 5 else 1.0
+        codes, scale = engine.rms_norm_fp8(x[k:k + 1], w[k], 1e-6)
+        y = engine.rms_norm(x[k:k + 1], w[k], 1e-6)
+        want = (y / scale.repeat_interleave(128, 1)[:, :C]).cpu().to(torch.float8_e4m3fn).float()
+        got = codes.cpu().float()
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(got.nan_to_num(), want.nan_to_num())
+    assert torch.isnan(got).any() and (got == 0).any()
