@@ -9,6 +9,7 @@ from __future__ import annotations
 from typing import Dict, Optional, Sequence, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from forge.backend.hip import kernels, _need_one_device, _unit_rows, ACTIVATIONS
 
@@ -61,7 +62,17 @@ def routed_rows(x: torch.Tensor, router_indices: torch.Tensor,
     return rows, offsets
 
 
+def _no_tangent(name: str, *tensors):
+    # (a dual tensor asks for no gradient; the level is looked at first because it costs nothing)
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no forward-mode derivative: call it on the primal tensors")
+
+
 def _no_gradient(name: str, *tensors):
+    _no_tangent(name, *tensors)
     if not torch.is_grad_enabled():
         return
     for t in tensors:
@@ -166,7 +177,7 @@ def expert_gated_rows(rows: torch.Tensor, offsets: Union[torch.Tensor, Sequence[
     from offsets[E] on) get 0.  activation: "silu", "gelu" (tanh form), "relu" or None.
     Sums in f32, h [N, I] bf16 rounded once.
 
-    Differentiable in rows, w_gate and w_up (once: create_graph is refused); gradients are bf16, with dg and du rounded to
+    Differentiable in rows, w_gate and w_up (once: create_graph and forward mode are refused); gradients are bf16, with dg and du rounded to
     bf16 between the products.  A HIP graph of a training step captures ``kernels.gated_rows(...,
     keep=True)`` and ``kernels.gated_rows_backward`` directly; under autograd a capture is refused."""
     if activation not in ACTIVATIONS:
@@ -199,6 +210,7 @@ def expert_gated_rows(rows: torch.Tensor, offsets: Union[torch.Tensor, Sequence[
             raise ValueError(f"expert_gated_rows: offsets must be {E + 1} ascending numbers within "
                              f"[0, {N}]")
         off = torch.tensor(off, dtype=torch.int32).to(rows.device)
+    _no_tangent("expert_gated_rows", rows, w_gate, w_up)
     rows, w_gate, w_up = _unit_rows(rows), _unit_rows(w_gate), _unit_rows(w_up)
     if torch.is_grad_enabled() and (rows.requires_grad or w_gate.requires_grad or w_up.requires_grad):
         if torch.cuda.is_current_stream_capturing():
