@@ -203,7 +203,8 @@ def expert_gated_rows(rows: torch.Tensor, offsets: Union[torch.Tensor, Sequence[
         if offsets.dtype not in (torch.int32, torch.int64) or tuple(offsets.shape) != (E + 1,):
             raise ValueError(f"expert_gated_rows: offsets {tuple(offsets.shape)} {offsets.dtype}, expected "
                              f"[{E + 1}] int32 or int64")
-        off = offsets.to(torch.int32).contiguous()
+        # (clamped while they are wide: behind 2^31 they would come back as others within [0, N])
+        off = (offsets.clamp(0, N) if offsets.dtype == torch.int64 else offsets).to(torch.int32).contiguous()
     else:
         off = [int(v) for v in offsets]
         if len(off) != E + 1 or off[0] < 0 or off[-1] > N or any(a > b for a, b in zip(off, off[1:])):
