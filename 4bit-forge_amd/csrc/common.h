@@ -28,6 +28,8 @@ int fail(int code, const char* fmt, ...);
 #define FORGE_LAUNCH_CHECK() FORGE_HIP_CHECK(hipGetLastError())
 
 static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// A launch has fewer than 2^32 threads along x: so many workgroups of `threads` at most.
+static inline int64_t max_workgroups(int64_t threads) { return UINT32_MAX / threads; }
 
 // Library-wide settings (forge_set_option / forge_get_option in forge_hip.h).  Each starts from
 // an environment variable read ONCE, when the library is loaded; after that only

@@ -832,7 +832,7 @@ extern "C" int forge_pad_rows(const void* in, int64_t stride, int64_t ld, void* 
     FORGE_REQUIRE(batch >= 0 && R >= 0 && C >= 1 && Rp >= R && Cp >= C && Cp % 8 == 0,
                   "%s: batch=%lld R=%lld C=%lld Rp=%lld Cp=%lld", name, (long long)batch, (long long)R, (long long)C,
                   (long long)Rp, (long long)Cp);
-    FORGE_REQUIRE(batch <= 65535 && Rp < (1 << 30) && Cp < (1 << 24) && Rp * Cp / 8 <= (int64_t)INT32_MAX * 256,
+    FORGE_REQUIRE(batch <= 65535 && Rp < (1 << 30) && Cp < (1 << 24) && forge::ceil_div(Rp * Cp / 8, 256) <= forge::max_workgroups(256),
                   "%s: batch=%lld Rp=%lld Cp=%lld: too large", name, (long long)batch, (long long)Rp, (long long)Cp);
     if (batch == 0 || Rp == 0) return FORGE_OK;
     FORGE_REQUIRE(in && out, "%s: null pointer", name);
@@ -870,7 +870,7 @@ extern "C" int forge_gated_rows(const void* rows, int64_t ldx, const int32_t* of
     const int64_t p_tiles = forge::ceil_div(I, few ? 128 / split : 128);
     const int q_tile = few ? few_tile(N, E) : 256;
     const int64_t blocks = forge::ceil_div(p_tiles * forge::ragged_tiles(N, E, q_tile), 8) * 8 + 8;
-    FORGE_REQUIRE(blocks <= INT32_MAX, "%s: %lld workgroups", name, (long long)blocks);
+    FORGE_REQUIRE(blocks <= forge::max_workgroups(512), "%s: %lld workgroups, too many for one launch", name, (long long)blocks);
     const dim3 grid((unsigned)blocks);
     if (!few) gated_tile_kernel<FORWARD><<<grid, 512, 0, st>>>(a, (int)p_tiles, 1);
     else if (q_tile == 16) gated_few_kernel<1><<<grid, 512, 0, st>>>(a, (int)p_tiles, split);
@@ -909,7 +909,9 @@ extern "C" int forge_gated_rows_backward(const void* dh, const float* g, const f
     const bool few = few_rows_back(N, E, H);
     const int64_t h_tiles = forge::ceil_div(H, 256), i_tiles = forge::ceil_div(I, 256), p_tiles = few ? forge::ceil_div(H, 128) : h_tiles;
     const int64_t row_blocks = forge::ceil_div(p_tiles * forge::ragged_tiles(N, E, few ? 32 : 256), 8) * 8 + 8;
-    FORGE_REQUIRE(row_blocks <= INT32_MAX && 16 * forge::ceil_div(h_tiles * i_tiles, 8) * E <= INT32_MAX && N * I / 8 / 256 < INT32_MAX, "%s: too many workgroups", name);
+    FORGE_REQUIRE(row_blocks <= forge::max_workgroups(512) && 16 * forge::ceil_div(h_tiles * i_tiles, 8) * E <= INT32_MAX &&
+                      forge::ceil_div(N * I / 8, 256) <= forge::max_workgroups(256),
+                  "%s: too many workgroups for one launch", name);
     if (N > 0) {
         forge::KernelTiming timing("gated_grad", st, 14.0 * N * I, forge::WORK_BYTES);
         gated_grad_kernel<<<dim3((unsigned)forge::ceil_div(N * I / 8, 256)), 256, 0, st>>>(
@@ -929,6 +931,7 @@ extern "C" int forge_gated_rows_backward(const void* dh, const float* g, const f
         if (!dWg) { a.dg = du; a.dwg = a.dwu; }
         if (N >= kLongExperts * E) {
             const int64_t blocks = forge::ceil_div(h_tiles * i_tiles, 8) * 8 * E * both;
+            FORGE_REQUIRE(blocks <= forge::max_workgroups(512), "%s: %lld workgroups, too many for one launch", name, (long long)blocks);
             gated_tile_kernel<DWEIGHTS><<<dim3((unsigned)blocks), 512, 0, st>>>(a, (int)h_tiles, (int)i_tiles);
         } else {
             const int64_t items = forge::ceil_div(h_tiles * i_tiles * both, 8) * E;    // of an XCD

@@ -753,7 +753,7 @@ int launch(const char* name, const Int4Args& a, bool pieces, bool one_group, boo
     const int64_t M = a.M, R = a.R;
     if (!pieces) {
         const int64_t r_tiles = forge::ceil_div(R, 64), blocks = r_tiles * forge::ceil_div(M, 64);
-        FORGE_REQUIRE(blocks <= INT32_MAX, "%s: %lld workgroups", name, (long long)blocks);
+        FORGE_REQUIRE(blocks <= forge::max_workgroups(256), "%s: %lld workgroups, too many for one launch", name, (long long)blocks);
         int4_any_kernel<ZERO><<<dim3((unsigned)blocks), 256, 0, st>>>(a, (int)r_tiles);
     } else if (M <= kFewRows) {
         launch_few<ZERO>(a, one_group, st);
@@ -764,7 +764,7 @@ int launch(const char* name, const Int4Args& a, bool pieces, bool one_group, boo
     } else {
         const int64_t r_tiles = forge::ceil_div(R, 256), m_tiles = forge::ceil_div(M, 128);
         const int64_t blocks = forge::ceil_div(r_tiles * m_tiles, 8) * 8;
-        FORGE_REQUIRE(blocks <= INT32_MAX, "%s: %lld workgroups", name, (long long)blocks);
+        FORGE_REQUIRE(blocks <= forge::max_workgroups(512), "%s: %lld workgroups, too many for one launch", name, (long long)blocks);
         const dim3 grid((unsigned)blocks);
         if (a.gs % 128 == 0 || one_group) int4_tile_kernel<1, ZERO><<<grid, 512, 0, st>>>(a, (int)r_tiles, (int)m_tiles, vec);
         else if (a.gs % 64 == 0) int4_tile_kernel<2, ZERO><<<grid, 512, 0, st>>>(a, (int)r_tiles, (int)m_tiles, vec);

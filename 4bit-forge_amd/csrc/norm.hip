@@ -228,15 +228,25 @@ __global__ __launch_bounds__(256) void rms_norm_any_kernel(NormArgs a) {
 }
 
 template <typename T, bool FP8>
-void launch(const NormArgs& a, bool vec, hipStream_t st) {
-    if (vec && a.C <= 64 * 8 * 4)
-        rms_norm_kernel<T, 64, 4, FP8><<<dim3((unsigned)forge::ceil_div(a.T, 4)), 256, 0, st>>>(a);
-    else if (vec && a.C <= 256 * 8 * 4)
-        rms_norm_kernel<T, 256, 4, FP8><<<dim3((unsigned)a.T), 256, 0, st>>>(a);
-    else if (vec && a.C <= 1024 * 8 * 2)
-        rms_norm_kernel<T, 1024, 2, FP8><<<dim3((unsigned)a.T), 1024, 0, st>>>(a);
-    else
-        rms_norm_any_kernel<T, FP8><<<dim3((unsigned)a.T), 256, 0, st>>>(a);
+void launch(NormArgs a, bool vec, hipStream_t st) {
+    // as many rows at a time as a launch can have threads for
+    const int width = !vec ? 0 : a.C <= 64 * 8 * 4 ? 64 : a.C <= 256 * 8 * 4 ? 256 : a.C <= 1024 * 8 * 2 ? 1024 : 0;
+    const int64_t T0 = a.T, most = width == 64 ? forge::max_workgroups(256) * 4 : forge::max_workgroups(width == 1024 ? 1024 : 256);
+    for (int64_t done = 0; done < T0; done += a.T) {
+        a.T = T0 - done < most ? T0 - done : most;
+        const dim3 grid((unsigned)(width == 64 ? forge::ceil_div(a.T, 4) : a.T));
+        if (width == 64) rms_norm_kernel<T, 64, 4, FP8><<<grid, 256, 0, st>>>(a);
+        else if (width == 256) rms_norm_kernel<T, 256, 4, FP8><<<grid, 256, 0, st>>>(a);
+        else if (width == 1024) rms_norm_kernel<T, 1024, 2, FP8><<<grid, 1024, 0, st>>>(a);
+        else rms_norm_any_kernel<T, FP8><<<grid, 256, 0, st>>>(a);
+        a.x = (const T*)a.x + a.T * a.ldx;
+        if (a.res) {
+            a.res = (const T*)a.res + a.T * a.ldr;
+            a.res_out = (T*)a.res_out + a.T * a.C;
+        }
+        a.y = (char*)a.y + a.T * a.C * (FP8 ? 1 : sizeof(T));
+        if (FP8) a.scale_inv += a.T * forge::ceil_div(a.C, kGroup);
+    }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
