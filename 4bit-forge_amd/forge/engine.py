@@ -232,7 +232,8 @@ def linear_int4(x: torch.Tensor, packed: Dict[str, torch.Tensor], bias: Optional
     numbers of an integer type, one per group) the codes are formed from both, without one every zero
     is 8 (symmetric records).  x [..., C] bf16, bias [R] bf16, residual [..., R] bf16;
     activation "silu", "gelu" (tanh form), "relu" or None; result [..., R] bf16, rounded once.
-    group_size may be left out when the groups divide C evenly (or there is one).  The weights stay
+    group_size may be left out when the groups divide C evenly (or there is one) and no power of two gives as
+    many groups, the last one shorter.  The weights stay
     4 bits wide in memory; no layout of them is kept.  No backward pass (refused where one is asked
     for)."""
     w, scale = packed["weight_packed"], packed["weight_scale"]
@@ -254,6 +255,10 @@ def linear_int4(x: torch.Tensor, packed: Dict[str, torch.Tensor], bias: Optional
         if C % G:
             raise ValueError(f"linear_int4: {G} groups do not divide {C} columns evenly: pass group_size")
         group_size = C // G
+        # another usual size may give as many groups, the last one shorter: 2 of 192 columns are 96 + 96 or 128 + 64
+        usual = 1 << (group_size - 1).bit_length()
+        if G > 1 and usual != group_size and (C + usual - 1) // usual == G:
+            raise ValueError(f"linear_int4: {G} groups of {C} columns may be of {group_size} or of {usual}: pass group_size")
     if group_size < 1 or (C + group_size - 1) // group_size != G:
         raise ValueError(f"linear_int4: group_size={group_size} does not give {G} groups of {C} columns")
     zero = packed.get("weight_zero_point")
