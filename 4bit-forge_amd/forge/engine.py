@@ -170,7 +170,8 @@ def expert_gated_rows(rows: torch.Tensor, offsets: Union[torch.Tensor, Sequence[
     """The rows that reach each expert's down projection, for all experts at once:
     h_i = act(w_gate[e] x_i) * (w_up[e] x_i) for the rows x_i of expert e, i.e. what
     ``ExpertGroupGPTQ.update`` of the down projections takes.  rows [N, H] bf16 grouped by expert
-    and offsets [E + 1] as ``routed_rows`` returns them; offsets may also be an int32 or int64 tensor on
+    and offsets [E + 1] as ``routed_rows`` returns them (a list: copied to the device, which waits for the work
+    queued there, and refused in a capture); offsets may also be an int32 or int64 tensor on
     the rows' device, which is taken without looking at it on the host (ascending within [0, N] is
     then the caller's duty; values outside are clamped).  w_gate, w_up [E, I, H] bf16, or [I, H]
     for a dense layer (offsets None: all rows are its own).  Rows of no expert (before offsets[0],
@@ -198,7 +199,8 @@ def expert_gated_rows(rows: torch.Tensor, offsets: Union[torch.Tensor, Sequence[
     if offsets is None:
         if E != 1:
             raise ValueError(f"expert_gated_rows: {E} experts need offsets")
-        offsets = [0, N]
+        # made on the device where the rows are on one: nothing to copy, nothing to wait for
+        offsets = torch.arange(0, N + 1, N, dtype=torch.int32, device=rows.device) if rows.is_cuda and N else [0, N]
     if isinstance(offsets, torch.Tensor) and offsets.is_cuda:
         if offsets.dtype not in (torch.int32, torch.int64) or tuple(offsets.shape) != (E + 1,):
             raise ValueError(f"expert_gated_rows: offsets {tuple(offsets.shape)} {offsets.dtype}, expected "
@@ -210,6 +212,9 @@ def expert_gated_rows(rows: torch.Tensor, offsets: Union[torch.Tensor, Sequence[
         if len(off) != E + 1 or off[0] < 0 or off[-1] > N or any(a > b for a, b in zip(off, off[1:])):
             raise ValueError(f"expert_gated_rows: offsets must be {E + 1} ascending numbers within "
                              f"[0, {N}]")
+        if rows.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("expert_gated_rows: offsets on the host cannot be captured (the copy waits for the GPU): "
+                               "pass them as an int32 tensor on the rows' device")
         off = torch.tensor(off, dtype=torch.int32).to(rows.device)
     _no_tangent("expert_gated_rows", rows, w_gate, w_up)
     rows, w_gate, w_up = _unit_rows(rows), _unit_rows(w_gate), _unit_rows(w_up)
