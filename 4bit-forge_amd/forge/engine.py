@@ -234,7 +234,7 @@ def linear_int4(x: torch.Tensor, packed: Dict[str, torch.Tensor], bias: Optional
     """A layer's product with its packed weights, as ``export.pack_weight`` returns them:
     act(x W^T + bias) + residual with W[r, c] = (code - zero) * weight_scale[r, c / group_size], the layer's
     dequantised weight.  The record's nibbles are code - zero + 8 modulo 16: with a ``weight_zero_point`` (whole
-    numbers of an integer type, one per group) the codes are formed from both, without one every zero
+    numbers of an integer type, one per group; 0 .. 15 on the solver's grids, -240 .. 255 are exact) the codes are formed from both, without one every zero
     is 8 (symmetric records).  x [..., C] bf16, bias [R] bf16, residual [..., R] bf16;
     activation "silu", "gelu" (tanh form), "relu" or None; result [..., R] bf16, rounded once.
     group_size may be left out when the groups divide C evenly (or there is one) and no power of two gives as

@@ -191,3 +191,22 @@ def test_refusals_at_the_c_entry():
     assert call(gs=0) == 1 and call(act=-1) == 1 and call(R=0) == 1
     assert call(C=1 << 25, ldx=1 << 25) == 1 and b"too large" in err()
     assert call(M=0, x=None, zero=None) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("M,C,R,gs", [(300_100, 7168, 24, 128), (300_100, 7168, 10, 56), (70_000, 64, 32_000, 32)])
+def test_behind_two_to_the_31st_element(hip, M, C, R, gs, zeros):
+    """of x, or of the residual and y: the last rows against the same rows alone in float64, the first ones too"""
+    k = 70
+    codes, zero, scale, rec = record(R, C, gs, "each" if zeros else 8, 5)
+    if not zeros:
+        del rec["weight_zero_point"]
+    x = torch.zeros(M, C, dtype=torch.bfloat16, device=DEV)
+    x[:k], x[-k:] = _mk(1, k, C), _mk(2, k, C)
+    res = torch.zeros(M, R, dtype=torch.bfloat16, device=DEV)
+    res[-k:] = _mk(3, k, R)
+    y = engine.linear_int4(x, rec, residual=res, group_size=gs)
+    within(y[:k], *weights_64(x[:k], codes, zero, scale, gs, residual=res[:k]))
+    within(y[-k:], *weights_64(x[-k:], codes, zero, scale, gs, residual=res[-k:]))
+    assert not y[k:-k].any()
