@@ -96,9 +96,10 @@ struct Zero {
 __device__ __forceinline__ Zero zero_of(uint32_t z) {
     return {(z & 15u) * 0x11111111u, __builtin_fmaf(-0.0625f, (float)(int)z, 0.5f)};
 }
-// Eight times code - zero as bf16, divided by 16.  nibble + zero modulo 16 is code - 8 as a signed 4-bit integer
-// (added in the low three bits of every nibble, the top bit by exclusive or: nothing carries into a
-// neighbour); (code - 8) / 16 + (8 - zero) / 16 is exact, in the upper 16 bits too (zero within -240 .. 255).
+// The eight values code - zero of a word as bf16, divided by 16 like those above.  nibble + zero modulo 16 is code - 8
+// as a signed 4-bit integer (added in the low three bits of every nibble, the top bit by exclusive or: nothing
+// carries into a neighbour); (code - 8) / 16 + (8 - zero) / 16 is exact, in the upper 16 bits too (zero within
+// -240 .. 255).  26 instructions for 8 values: one row, 2048 -> 7168, 5.8 us against 4.9; 8192 rows 515 / 446.
 __device__ __forceinline__ bf16x8_t nibbles(uint32_t word, const Zero& z) {
     const uint32_t a = ((word & 0x77777777u) + (z.add & 0x77777777u)) ^ ((word ^ z.add) & 0x88888888u), b = a >> 4;
     auto value = [&](uint32_t v) { return __float_as_uint(__uint_as_float(v) + z.off); };
@@ -197,9 +198,9 @@ __global__ __launch_bounds__(512) void int4_few_kernel(Int4Args a) {
 // ---------------------------------------------------------------- many rows of x
 // 128 rows of x by 256 weight rows per workgroup, 64 columns a stage (mfma_tile.h).  A wavefront takes all of
 // the rows of x by 32 weight rows: a 32 x 16 fragment of W is one word per lane, converted by the only
-// wavefront that multiplies by it, a step ahead.  8192 rows, 7168 -> 4096: 450 us, 1070 TFLOP/s, the clock at 1.6 to
-// 1.7 GHz (2.1 and more where power allows), the matrix pipe busy for half of the cycles and the vector ALU
-// for half, so what counts is the work itself: 64 x 64 outputs per wavefront halve the reads of x from LDS
+// wavefront that multiplies by it, a step ahead.  8192 rows, 7168 -> 4096: 450 us, 1070 TFLOP/s
+// (469 with bias, activation and residual; 515 with zero points), the clock at 1.6 to 1.7 GHz (2.1 and more where power
+// allows), the matrix pipe busy for half of the cycles and the vector ALU for half, so what counts is the work itself: 64 x 64 outputs per wavefront halve the reads of x from LDS
 // but convert every word twice (585 us against 490 at that time).  Converted once, into LDS, words cost 16 KB of
 // writes and 64 KB of reads a stage.
 // Every group's sum is formed by itself and folded into the totals with its scale, one fma per output and
