@@ -180,7 +180,8 @@ def expert_gated_rows(rows: torch.Tensor, offsets: Union[torch.Tensor, Sequence[
 
     Differentiable in rows, w_gate and w_up (once: create_graph and forward mode are refused); gradients are bf16, with dg and du rounded to
     bf16 between the products.  A HIP graph of a training step captures ``kernels.gated_rows(...,
-    keep=True)`` and ``kernels.gated_rows_backward`` directly; under autograd a capture is refused."""
+    keep=True)`` and ``kernels.gated_rows_backward`` directly; under autograd a capture is refused, and the backward pass of an
+    eager call is not one to capture either: autograd runs it on that call's stream."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"expert_gated_rows: unknown activation {activation!r} (one of {list(ACTIVATIONS)})")
     for n, t in (("rows", rows), ("w_gate", w_gate), ("w_up", w_up)):

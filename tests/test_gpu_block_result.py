@@ -51,3 +51,55 @@ def test_tokens_results(hip, group_size):
     # (the sums over experts are in 64 bits on both sides)
     assert ((out - want).abs() <= bound + 1e-12).all()
     assert (out - stream.double()).abs().amax(1).min() > 0         # every token got something
+
+
+def test_two_threads_on_streams_of_their_own(hip):
+    """every operator from two threads at once, odd sizes (padded copies) among them: the bits of one after the other"""
+    import threading
+    g = torch.Generator(device=DEV).manual_seed(3)
+    mk = lambda s, *sh: (s * torch.randn(*sh, generator=g, device=DEV)).bfloat16()   # noqa: E731
+
+    def job(H, I):
+        x, w = mk(1.0, 500, H), mk(1.0, H)
+        leaves = [mk(1.0, 500, H), mk(0.05, 3, I, H), mk(0.05, 3, I, H)]
+        dh, offs = mk(1.0, 500, I), torch.tensor([0, 130, 130, 500], dtype=torch.int32, device=DEV)
+        codes = torch.randint(0, 16, (H, I), generator=g, device=DEV, dtype=torch.uint8)
+        scale = torch.rand(H, -(-I // 64), generator=g, device=DEV)
+        zero = torch.randint(0, 16, scale.shape, generator=g, device=DEV)
+        rec = export.pack_weight({"qweight": codes, "scale": scale, "zero": zero}, 4, False, 64)
+
+        def run():
+            y, s = engine.rms_norm(x, w, residual=leaves[0])
+            c, sc, _ = engine.rms_norm_fp8(x, w, residual=leaves[0])
+            t = [v.detach().requires_grad_(True) for v in leaves]
+            h = engine.expert_gated_rows(t[0], offs, t[1], t[2])
+            grads = torch.autograd.grad(h, t, dh)
+            out = engine.linear_int4(h.detach(), rec, residual=s, group_size=64)
+            return [y, s, c.view(torch.uint8), sc, h.detach(), *grads, out]
+        return run
+
+    jobs = [job(256, 192), job(131, 77)]
+    want = [j() for j in jobs]
+    got, errors = [[], []], []
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    got[i].append(jobs[i]())
+                stream.synchronize()
+        except Exception as e:                                     # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for i in range(2):
+        assert len(got[i]) == 20
+        for res in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(res, want[i]))
